@@ -378,6 +378,62 @@ int m2r_fp4_gemv_g16(const uint8_t* packed, const uint8_t* e4m3_scales, const fl
                      int64_t u_stride, void* y, int64_t y_stride, int64_t M, int64_t N, int64_t K,
                      hipStream_t stream);
 
+/*
+ * Selective-state scan with a full-precision (binary32) carry: linear
+ * attention with a decay for each head.  Per head:
+ *   dt_t = softplus(dt + dt_bias), S_t = exp(A dt_t) S_{t-1} + dt_t x_t (x) B_t,
+ *   y_t = half(S_t C_t + D x_t).
+ * The recurrence that mamba2_recall/state_codec.py:65-102 (_s16_scan) rounds
+ * to FP16 after every token, here without a codec.
+ *   x f16[B,L,H,P], dt f16[B,L,H], B, C f16[B,L,G,128] with element strides of
+ *   batch rows and tokens (a token's own elements dense); A f32[H]; D, dt_bias
+ *   f16 or f32 [H] (flag 1 = f32); state f32[pool,H,P,128], 16-byte aligned,
+ *   changed in place; slots i32[B] or null (row b uses carry b): outside
+ *   0..pool-1 for an idle row, no carry twice; lengths i32[B] or null (L),
+ *   clamped to 0..L; y f16[B,L,H,P], zero past a row's length.
+ *   workspace: 16-byte aligned device memory of m2r_full_scan_workspace()
+ *   bytes (null where that is 0), used on `stream` only.
+ */
+int m2r_full_scan(const void* x, int64_t xs_b, int64_t xs_l, const void* dt, int64_t ds_b, int64_t ds_l,
+                  const float* A, const void* B, int64_t bs_b, int64_t bs_l, const void* C, int64_t cs_b, int64_t cs_l,
+                  const void* D, int d_is_f32, const void* dt_bias, int db_is_f32, float* state, int64_t pool,
+                  const int32_t* slots, const int32_t* lengths, void* y, int64_t batch, int64_t L, int64_t H,
+                  int64_t P, int64_t G, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int64_t m2r_full_scan_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[m] = half(base[m] + scale[a] up[a] (down[a] x[m])), a = ids[m];
+ * out[m] = base[m] where ids[m] is outside 0..adapters-1.  The reference has
+ * one adapter for all requests (mamba2_recall/resurface_native.py:363-375).
+ *   x f16 rows of K, base and out f16 rows of N (element row strides; out may
+ *   be base); down f16[adapters,rank,K], up f16[adapters,N,rank], scale
+ *   f32[adapters], ids i32[M]; rank at most 256; workspace: 16-byte aligned
+ *   device memory of m2r_adapters_workspace() bytes, used on `stream` only.
+ */
+int m2r_adapters_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* down,
+                     const void* up, const float* scale, const int32_t* ids, void* out, int64_t out_stride, int64_t M,
+                     int64_t K, int64_t N, int64_t adapters, int64_t rank, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
+int64_t m2r_adapters_workspace(int64_t M, int64_t K, int64_t N, int64_t rank);
+
+/*
+ * One token a row from logits (dtype 0 binary16, 1 bfloat16, 2 binary32) and a
+ * uniform number f32 in [0, 1): temperature, then top-k, top-p of what is
+ * left, min-p relative to the likeliest token; each filter an array of B
+ * values, or null and one value for all rows.  Weights are whole multiples of
+ * 2^-31 of the likeliest token's; sums are exact.  ids i64[B] (-1 where a row
+ * holds nothing above -inf), logprobs f32[B] of the filtered distribution.
+ * The reference decodes greedily (scripts/infer_fp4_ridge_resurface_v1.py:102-109).
+ *   workspace: 16-byte aligned device memory of m2r_sample_workspace() bytes
+ *   (null where that is 0), used on `stream` only.
+ */
+int m2r_sample(const void* logits, int dtype, int64_t row_stride, const float* uniforms, const float* temperature,
+               float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+               const float* min_p, float min_p_all, int64_t* ids, float* logprobs, int64_t batch, int64_t V,
+               void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int64_t m2r_sample_workspace(int64_t batch, int64_t V);
+
 #ifdef __cplusplus
 }
 #endif

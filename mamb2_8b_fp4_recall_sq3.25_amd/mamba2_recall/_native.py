@@ -47,6 +47,13 @@ _SIGNATURES = {
     "m2r_causal_conv_tokens": ([P, I64, I64, I, P, I64, I64, P, P, P, P, P, I64, I64, I64, I64, I64, I, P], I),
     "m2r_gated_rmsnorm": ([P, I64, P, I64, P, P, I64, I64, I64, I64, F32, P], I),
     "m2r_fp4_gemv_g16": ([P, P, P, P, I64, P, I64, I64, I64, I64, P], I),
+    "m2r_full_scan_workspace": ([I64] * 5, I64),
+    "m2r_full_scan": ([P, I64, I64, P, I64, I64, P, P, I64, I64, P, I64, I64, P, I, P, I, P, I64] + [P] * 3 + [I64] * 5
+                      + [P, I64, P], I),
+    "m2r_adapters_workspace": ([I64] * 4, I64),
+    "m2r_adapters_add": ([P, I64, P, I64] + [P] * 5 + [I64] * 6 + [P, I64, P], I),
+    "m2r_sample_workspace": ([I64] * 2, I64),
+    "m2r_sample": ([P, I, I64, P, P, F32, P, I, P, F32, P, F32, P, P, I64, I64, P, I64, P], I),
     "m2r_state_step_ridge_layers_workspace": ([I], I64),
     "m2r_state_step_ridge_layers": ([P, I, I64, I64, I64, I64, P, I64, P], I),
     "m2r_state_step_ridge_layers_noalloc": ([P, I, I64, I64, I64, I64, P], I),

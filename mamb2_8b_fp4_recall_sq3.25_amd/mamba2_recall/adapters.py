@@ -1,0 +1,98 @@
+"""Low-rank adapters of many requests at once, beside a shared projection.
+
+A server keeps the adapters of one projection in an AdapterSet; `add` gives
+every row its own request's update in one call, whatever the mix of adapters:
+
+    out[m] = base[m] + scale[a] * (x[m] @ down[a].T) @ up[a].T,  a = ids[m]
+
+The reference has one adapter for all requests, installed as module hooks
+(mamba2_recall/resurface_native.py:363-375).  The products run the gfx950 HIP
+kernels of libm2r_hip.so (m2r_adapters_add)."""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+
+MAX_RANK = 256
+
+
+class AdapterSet:
+    """The adapters of one projection: `down` FP16[n,rank,K], `up`
+    FP16[n,N,rank], `scale` FP32[n] (default 1).  Adapters of a lower rank
+    are padded with zero rows of `down` and columns of `up`."""
+
+    def __init__(self, down, up, scale=None):
+        for t, name in ((down, "down"), (up, "up")):
+            if not isinstance(t, torch.Tensor) or t.ndim != 3 or t.dtype != torch.float16 or not t.is_cuda:
+                raise ValueError(f"{name} must be CUDA FP16 with three axes")
+        n, rank, _ = down.shape
+        if min(down.shape) < 1 or min(up.shape) < 1 or rank > MAX_RANK:
+            raise ValueError(f"Positive geometry and a rank of at most {MAX_RANK} required")
+        if up.shape[0] != n or up.shape[2] != rank or up.device != down.device:
+            raise ValueError("down [n,rank,K] and up [n,N,rank] differ in adapters, rank or device")
+        if scale is None:
+            scale = torch.ones(n, dtype=torch.float32, device=down.device)
+        if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (n,)
+                or scale.device != down.device):
+            raise ValueError("scale must be FP32[n] on the adapters' device")
+        self.down, self.up, self.scale = down.contiguous(), up.contiguous(), scale.contiguous()
+
+    @property
+    def count(self):
+        return self.down.shape[0]
+
+    @property
+    def rank(self):
+        return self.down.shape[1]
+
+    @property
+    def features(self):
+        """(K, N) of the projection."""
+        return self.down.shape[2], self.up.shape[1]
+
+
+def _rows(t, features, what):
+    """`t` [..., features] as FP16 rows with unit column stride: (t, rows, row stride)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or not t.is_cuda or t.ndim < 1 \
+            or t.shape[-1] != features:
+        raise ValueError(f"{what} must be CUDA FP16[..., {features}]")
+    if t.ndim != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < features):
+        t = t.reshape(-1, features).contiguous()
+    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else features
+
+
+@torch.no_grad()
+def add(base, x, adapters, ids, out=None):
+    """base[..., N] plus each row's adapter update of x[..., K]; a new FP16
+    tensor, or `out` (which may be `base`).  `ids` int32[...] names each row's
+    adapter: negative, or not below the set's count, for none (the row is
+    copied).  Rows with the same adapter cost least side by side."""
+    if not isinstance(adapters, AdapterSet):
+        raise ValueError("adapters must be an AdapterSet")
+    k, n = adapters.features
+    shape = tuple(base.shape) if isinstance(base, torch.Tensor) else None
+    b2, rows, bs = _rows(base, n, "base")
+    x2, xrows, xs = _rows(x, k, "x")
+    if rows != xrows or shape[:-1] != tuple(x.shape[:-1]):
+        raise ValueError("base and x must have the same rows")
+    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or tuple(ids.shape) != shape[:-1]:
+        raise ValueError("ids must be int32, one for each row")
+    if any(t.device != base.device for t in (x, ids, adapters.down)):
+        raise ValueError("Adapter operands must share one device")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float16, device=base.device)
+    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or tuple(out.shape) != shape
+          or out.device != base.device or not out.is_contiguous()):
+        raise ValueError("out must be contiguous FP16 of base's shape")
+    if rows == 0:
+        return out
+    ids = ids.contiguous()
+    ws_bytes = int(_native.lib().m2r_adapters_workspace(rows, k, n, adapters.rank))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=base.device)
+    p = _native.ptr
+    with _native.device_of(base):
+        _native.call("m2r_adapters_add", p(x2), xs, p(b2), bs, p(adapters.down), p(adapters.up), p(adapters.scale),
+                     p(ids), p(out), n, rows, k, n, adapters.count, adapters.rank, p(ws), ws_bytes,
+                     _native.stream_of(base))
+    return out
