@@ -37,4 +37,8 @@ __device__ __forceinline__ int64_t full_length(const FullArgs& a, int64_t b) {
   return n < 0 ? 0 : (n < a.L ? n : a.L);
 }
 
+// Many tokens in chunks, on the matrix cores (m2r_full_chunks.hip).
+int64_t full_chunks_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G);
+hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t stream);
+
 }  // namespace m2r

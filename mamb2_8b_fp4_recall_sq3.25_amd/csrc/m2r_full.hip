@@ -79,7 +79,13 @@ __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
 
 using namespace m2r;
 
-extern "C" int64_t m2r_full_scan_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) { return 0; }
+// Calls of this many tokens on take the chunked kernel.
+constexpr int64_t kChunkedFrom = 8;
+
+extern "C" int64_t m2r_full_scan_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) {
+  if (batch <= 0 || L < kChunkedFrom || H <= 0 || P <= 0 || G <= 0 || H % G) return 0;
+  return full_chunks_workspace(batch, L, H, P, G);
+}
 
 extern "C" int m2r_full_scan(const void* x, int64_t xs_b, int64_t xs_l, const void* dt, int64_t ds_b, int64_t ds_l,
                              const float* A, const void* B, int64_t bs_b, int64_t bs_l, const void* C, int64_t cs_b,
@@ -99,6 +105,12 @@ extern "C" int m2r_full_scan(const void* x, int64_t xs_b, int64_t xs_l, const vo
   FullArgs a{(const uint16_t*)x, (const uint16_t*)dt, xs_b, xs_l, ds_b, ds_l, A, (const uint16_t*)B,
              (const uint16_t*)C, bs_b, bs_l, cs_b, cs_l, D, dt_bias, d_is_f32, db_is_f32, state, pool, slots, lengths,
              (uint16_t*)y, batch, L, H, P, G};
+  if (L >= kChunkedFrom) {
+    const int64_t need = full_chunks_workspace(batch, L, H, P, G);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+      return m2r_fail("full scan: workspace too small or not 16-byte aligned");
+    return m2r_check(launch_full_chunks(a, workspace, stream), "full scan launch");
+  }
   constexpr int R = 4;
   const __int128 waves = (__int128)batch * H * ((P + 2 * R - 1) / (2 * R));
   if ((waves + 3) / 4 > 0x7fffffff) return m2r_fail("full scan: grid limits exceeded");
