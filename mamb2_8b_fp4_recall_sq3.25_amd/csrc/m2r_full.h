@@ -21,10 +21,33 @@ struct FullArgs {
   int64_t batch, L, H, P, G;
 };
 
-// softplus(v) = log(1 + exp(v)), v itself above 20 (where they agree to
-// binary32).  log1p keeps the relative precision of small steps, which
-// log(exp(v) + 1) in binary32 loses below v = -8.
-__device__ __forceinline__ float full_dt(float v) { return v <= 20.0f ? log1pf(expf(v)) : v; }
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, with
+// log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by its series to s^15 (the
+// rest is below 2^-26 of it).  e keeps the part of v log2(e) that the product
+// rounds away, so that small steps have the relative precision of large ones
+// (log(exp(v) + 1) in binary32 loses it below v = -8).  NaN and infinities
+// come through.
+__device__ __forceinline__ float full_dt(float v) {
+  constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0cp-26f, kLn2 = 0x1.62e43p-1f;
+  const float m = -__builtin_fabsf(v), t = m * kLog2e;
+  float e = __builtin_amdgcn_exp2f(t);
+  const float rest = __builtin_fmaf(m, kLog2eLow, __builtin_fmaf(m, kLog2e, -t));
+  e = t > -150.f ? __builtin_fmaf(e, rest * kLn2, e) : 0.f;   // (an infinite m has no rest)
+  const float d = 2.0f + e;
+  float r = __builtin_amdgcn_rcpf(d);
+  r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+  const float s = e * r, q = s * s;
+  float p = 1.0f / 15.0f;
+  p = __builtin_fmaf(p, q, 1.0f / 13.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 11.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 9.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 7.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 5.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 3.0f);
+  const float l = __builtin_fmaf(s * q, p, s);
+  const float y = (v > 0.f ? v : 0.f) + (l + l);
+  return v != v ? v : y;
+}
 
 // The carry of batch row b, or -1 for an idle row; and its token count.
 __device__ __forceinline__ int64_t full_slot(const FullArgs& a, int64_t b) {

@@ -157,6 +157,19 @@ __device__ __forceinline__ double dpp_add64(double v) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
   return v + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
+// The value of the last of the lane's 16 (row_newbcast:15).
+__device__ __forceinline__ double dpp_row_last64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x15F, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), 0x15F, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 // Inclusive sum over the wave: within rows of 16 lanes, then across them.
 __device__ __forceinline__ double scan_add64(double v) {
   const int lane = threadIdx.x & 63;
@@ -164,7 +177,7 @@ __device__ __forceinline__ double scan_add64(double v) {
   v = dpp_add64<0x112>(v);
   v = dpp_add64<0x114>(v);
   v = dpp_add64<0x118>(v);
-  const double e0 = __shfl(v, 15), e1 = __shfl(v, 31), e2 = __shfl(v, 47);
+  const double e0 = lane64(v, 15), e1 = lane64(v, 31), e2 = lane64(v, 47);
   const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e0 + e1 : (e0 + e1) + e2));
   return before + v;
 }
@@ -332,7 +345,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       ChunkScalars& hs = s.h[par][pair];
       const float dt = c0 + lane < n ? full_dt(h2f(rdt) + bias) : 0.f;
       const double l = scan_add64((double)av * (double)dt * 1.4426950408889634);
-      const double last = __shfl(l, 63), tile = __shfl(l, lane | 15);
+      const double last = lane64(l, 63), tile = dpp_row_last64(l);
       const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - l));
       hs.lh[lane] = lh;
       hs.ll[lane] = __builtin_fabsf(lh) < __builtin_inff() ? (float)(l - (double)lh) : 0.f;
