@@ -74,31 +74,68 @@ __device__ __forceinline__ uint32_t weight_of(const RowFilter& f, float l) {
   return away < 32.0f ? (uint32_t)(__builtin_amdgcn_exp2f(-away) * 0x1p31f) : 0u;
 }
 
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  return __builtin_bit_cast(float, key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// ---------------------------------------------------------------------------
+// Three launches.  A row is cut into at most kMaxSplits pieces of whole
+// 2,048-token blocks, one workgroup each.
+//   k_sample_top:    the largest logit of each piece;
+//   k_sample_bins:   the row's weight and token counts by bins of 1/16 in the
+//                    exponent (512 bins reach weight 0); the last workgroup
+//                    of a row then finds the bins in which top-k and top-p
+//                    end.  Without those filters a piece's weight is all that
+//                    is needed, and the last workgroup draws;
+//   k_sample_draw:   the tokens of those bins in a list, the weight above
+//                    them by piece; the last workgroup of a row sorts the
+//                    list, finds the cut and draws.
+// A row whose list would not fit (thousands of tokens in one bin: mostly
+// equal logits) is cut by its first workgroup alone, digit by digit.
+// Every sum is of whole numbers, so neither the order of the atomics nor the
+// order of the list decides anything.
+constexpr int kThreads = 256, kBlock = 8 * kThreads, kMaxSplits = 256, kBins = 512, kList = 4096;
+
+struct alignas(16) RowWork {
+  uint64_t weight[kBins];
+  uint64_t piece[kMaxSplits];    // weight kept for certain
+  uint64_t list[kList];          // (~key, index) of the tokens in the cut's bins
+  uint32_t count[kBins];
+  float top[kMaxSplits];
+  uint32_t ticket[2], listed, done;   // done: 1 drawn, 2 cut by one workgroup
+  // bins of the list: p0..p1 (top-p) and bk (top-k); kBins where that filter is off
+  uint32_t p0, p1, bk, unused;
+  uint64_t all;                       // weight of the row
+  uint64_t count_p, weight_p, count_k, weight_k;   // before bin p0 and before bin bk
+};
+
+struct SampleShared {
+  uint64_t bins[kBins];          // count << 46 | weight
+  uint64_t list[kList];
+  uint64_t piece[kMaxSplits];
+  uint64_t part[kThreads / 64];
+  float fpart[kThreads / 64];
+  uint32_t cnt[256];
+  uint64_t found[4];
+  uint32_t pick[4];
+  uint32_t last;
+};
+
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int by) {
   const uint32_t lo = __shfl_up((uint32_t)v, by), hi = __shfl_up((uint32_t)(v >> 32), by);
   return ((uint64_t)hi << 32) | lo;
 }
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {   // inclusive
   const int lane = threadIdx.x & 63;
+#pragma unroll
   for (int by = 1; by < 64; by *= 2) {
     const uint64_t o = shfl_up64(v, by);
     if (lane >= by) v += o;
   }
   return v;
 }
-
-constexpr int kRowThreads = 1024;
-
-struct RowShared {
-  uint32_t cnt[256];
-  uint64_t sum[256];
-  uint64_t part[kRowThreads / 64];
-  float fpart[kRowThreads / 64];
-  uint64_t found[4];   // digit, tokens before it, weight before it
-};
-
 // Exclusive prefix sum over the workgroup; `total` receives the sum.
-__device__ __forceinline__ uint64_t block_scan64(RowShared& s, uint64_t v, uint64_t& total) {
+__device__ __forceinline__ uint64_t block_scan64(SampleShared& s, uint64_t v, uint64_t& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const uint64_t inc = wave_scan64(v);
   __syncthreads();
@@ -106,11 +143,307 @@ __device__ __forceinline__ uint64_t block_scan64(RowShared& s, uint64_t v, uint6
   __syncthreads();
   uint64_t before = 0;
   total = 0;
-  for (int i = 0; i < kRowThreads / 64; ++i) {
-    if (i < w) before += s.part[i];
-    total += s.part[i];
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    const uint64_t p = s.part[i];
+    if (i < w) before += p;
+    total += p;
   }
   return before + inc - v;
+}
+__device__ __forceinline__ float block_max(float* part, float v) {
+#pragma unroll
+  for (int by = 32; by; by >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, by));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) v = __builtin_fmaxf(v, part[i]);
+  return v;
+}
+
+// Logits i .. i + 7 of a row, -inf past its end.  Rows of odd lengths start
+// at any element: the 16-byte loads need not be aligned.
+template <int DT>
+__device__ __forceinline__ void load_logits(const void* row, int64_t i, int64_t V, float* v) {
+  constexpr int kSize = DT == LOGITS_F32 ? 4 : 2;
+  if (i + 8 <= V) {
+    uint32_t w[2 * kSize];
+    __builtin_memcpy(w, (const char*)row + i * kSize, 8 * kSize);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f;
+      if constexpr (DT == LOGITS_F32) f = __builtin_bit_cast(float, w[j]);
+      else if constexpr (DT == LOGITS_F16) f = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+      else f = __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+      v[j] = f != f ? -__builtin_inff() : f + 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = i + j < V ? load_logit<DT>(row, i + j) : -__builtin_inff();
+  }
+}
+
+__device__ __forceinline__ uint64_t place_of(float l, int64_t i) {   // ascending = sorted order
+  return ((uint64_t)~order_key(l) << 32) | (uint32_t)i;
+}
+
+struct Piece { int64_t row; int64_t first, end; int piece; };
+struct Split { int pieces; int64_t size; };
+__device__ __forceinline__ Piece my_piece(const Split& sp, int64_t V) {
+  Piece p;
+  p.row = blockIdx.x / sp.pieces;
+  p.piece = (int)(blockIdx.x - p.row * sp.pieces);
+  p.first = p.piece * sp.size;
+  p.end = p.first + sp.size < V ? p.first + sp.size : V;
+  return p;
+}
+template <int DT>
+__device__ __forceinline__ const void* row_of(const SampleArgs& a, int64_t row) {
+  return (const char*)a.logits + row * a.ls * (DT == LOGITS_F32 ? 4 : 2);
+}
+
+// What the workgroups of a row hand to the last of them goes through
+// device-scope atomics, which all XCDs see at one place.  (Plain stores and a
+// device-wide fence per workgroup, which writes a whole L2 back, took 46 us
+// for 600 workgroups that do 4 us of work.)
+template <class T>
+__device__ __forceinline__ void put(T* p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class T>
+__device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// True in the workgroup that finishes its row's pass last: every workgroup
+// counts itself once its atomics have completed.
+__device__ __forceinline__ bool last_of_row(SampleShared& s, uint32_t* ticket, int pieces) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    s.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)pieces - 1;
+  __syncthreads();
+  return s.last;
+}
+
+__device__ __forceinline__ void put_token(const SampleArgs& a, int64_t row, const RowFilter& f, int64_t i, float l,
+                                          uint64_t total) {
+  a.ids[row] = i;
+  const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
+  a.logprobs[row] = -away * 0x1.62e43p-1f - logf((float)total * 0x1p-31f);
+}
+
+// The draw, with the kept weight of each piece in s.piece: a token is kept
+// when its place is at most `cut` and its weight at least f.least.
+template <int DT>
+__device__ void draw(SampleShared& s, const SampleArgs& a, const Split& sp, int64_t r, const RowFilter& f, uint64_t cut) {
+  const int tid = threadIdx.x;
+  const void* row = row_of<DT>(a, r);
+  uint64_t total;
+  const uint64_t mine = tid < sp.pieces ? s.piece[tid] : 0, before = block_scan64(s, mine, total);
+  const double at = __builtin_floor((double)a.u[r] * (double)total);
+  uint64_t target = at > 0.0 ? (uint64_t)at : 0;
+  target = target < total ? target : total - 1;
+  if (before <= target && target < before + mine) {
+    s.pick[0] = tid;
+    s.found[0] = target - before;
+  }
+  __syncthreads();
+  const int piece = s.pick[0];
+  uint64_t left = s.found[0];
+  const int64_t end = (piece + 1) * sp.size < a.V ? (piece + 1) * sp.size : a.V;
+  for (int64_t i0 = piece * sp.size; i0 < end; i0 += kBlock) {
+    const int64_t i = i0 + 8 * tid;
+    float v[8];
+    uint32_t w[8];
+    load_logits<DT>(row, i, a.V, v);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[j] = weight_of(f, v[j]);
+      w[j] = w[j] >= f.least && place_of(v[j], i + j) <= cut ? w[j] : 0;
+      sum += w[j];
+    }
+    uint64_t block;
+    uint64_t run = block_scan64(s, sum, block);
+    if (left < block) {
+      if (run <= left && left < run + sum) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (run <= left && left < run + w[j]) put_token(a, r, f, i + j, v[j], total);
+          run += w[j];
+        }
+      }
+      return;
+    }
+    left -= block;
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs a, Split sp, RowWork* work) {
+  __shared__ float part[kThreads / 64];
+  const Piece p = my_piece(sp, a.V);
+  RowWork& rw = work[p.row];
+  for (int i = p.piece * kThreads + threadIdx.x; i < kBins; i += sp.pieces * kThreads) {
+    rw.weight[i] = 0;
+    rw.count[i] = 0;
+  }
+  if (p.piece == 0 && threadIdx.x < 4) (&rw.ticket[0])[threadIdx.x] = 0;   // the tickets, listed and done
+  const void* row = row_of<DT>(a, p.row);
+  float top = -__builtin_inff();
+  for (int64_t i = p.first + 8 * threadIdx.x; i < p.end; i += kBlock) {
+    float v[8];
+    load_logits<DT>(row, i, a.V, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, v[j]);
+  }
+  top = block_max(part, top);
+  if (threadIdx.x == 0) rw.top[p.piece] = top;
+}
+
+// In which bin a running sum over the bins reaches `target`: s.found = bin,
+// count before it, weight before it.  Thread i holds bins 2 i and 2 i + 1.
+template <bool BY_WEIGHT>
+__device__ __forceinline__ void find_bin(SampleShared& s, uint64_t target, const uint64_t* n, const uint64_t* w,
+                                         uint64_t nb, uint64_t wb) {
+  __syncthreads();
+  for (int j = 0; j < 2; ++j) {
+    const uint64_t before = BY_WEIGHT ? wb : nb, size = BY_WEIGHT ? w[j] : n[j];
+    if (before < target && target <= before + size) {
+      s.found[0] = 2 * threadIdx.x + j;
+      s.found[1] = nb;
+      s.found[2] = wb;
+      s.found[3] = BY_WEIGHT ? n[j] : w[j];
+      s.pick[1] = (uint32_t)n[j];
+    }
+    nb += n[j];
+    wb += w[j];
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint64_t mass_of(double p, uint64_t all) {
+  const double m = __builtin_ceil(p * (double)all);
+  return m > 1.0 ? (uint64_t)m : 1;
+}
+
+__device__ __forceinline__ int bin_of(const RowFilter& f, float l) {
+  const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
+  return away < 32.0f ? (int)(away * 16.0f) : kBins;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp, RowWork* work) {
+  __shared__ SampleShared s;
+  const Piece p = my_piece(sp, a.V);
+  RowWork& rw = work[p.row];
+  const int tid = threadIdx.x;
+  const void* row = row_of<DT>(a, p.row);
+  RowFilter f = row_filter(a, p.row);
+  f.top = block_max(s.fpart, tid < sp.pieces ? rw.top[tid] : -__builtin_inff());
+  if (f.top == -__builtin_inff()) {   // every token masked
+    if (p.piece == 0 && tid == 0) {
+      a.ids[p.row] = -1;
+      a.logprobs[p.row] = -__builtin_inff();
+      rw.done = 1;
+    }
+    return;
+  }
+  const bool filtered = f.k < a.V || f.p < 1.0;
+  if (!filtered) {
+    uint64_t sum = 0, all;
+    for (int64_t i = p.first + 8 * tid; i < p.end; i += kBlock) {
+      float v[8];
+      load_logits<DT>(row, i, a.V, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = weight_of(f, v[j]);
+        sum += w >= f.least ? w : 0;
+      }
+    }
+    block_scan64(s, sum, all);
+    if (tid == 0) put(&rw.piece[p.piece], all);
+    if (!last_of_row(s, &rw.ticket[0], sp.pieces)) return;
+    s.piece[tid] = tid < sp.pieces ? get(&rw.piece[tid]) : 0;
+    if (tid == 0) rw.done = 1;
+    __syncthreads();
+    draw<DT>(s, a, sp, p.row, f, ~0ull);
+    return;
+  }
+  // 2^14 tokens of at most 2^31 each at a time: 15 bits of count, 46 of weight
+  for (int64_t from = p.first; from < p.end; from += 8 * kBlock) {
+    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+    __syncthreads();
+    const int64_t to = from + 8 * kBlock < p.end ? from + 8 * kBlock : p.end;
+    for (int64_t i = from + 8 * tid; i < to; i += kBlock) {
+      float v[8];
+      load_logits<DT>(row, i, a.V, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = weight_of(f, v[j]);
+        if (w) atomicAdd((unsigned long long*)&s.bins[bin_of(f, v[j])], (1ull << 46) | w);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads) {
+      const uint64_t b = s.bins[i];
+      if (b) {
+        atomicAdd((unsigned long long*)&rw.weight[i], (unsigned long long)(b & ((1ull << 46) - 1)));
+        atomicAdd(&rw.count[i], (uint32_t)(b >> 46));
+      }
+    }
+    __syncthreads();
+  }
+  if (!last_of_row(s, &rw.ticket[0], sp.pieces)) return;
+  uint64_t n[2], w[2], tokens, all;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    n[j] = get(&rw.count[2 * tid + j]);
+    w[j] = get(&rw.weight[2 * tid + j]);
+  }
+  const uint64_t nb = block_scan64(s, n[0] + n[1], tokens), wb = block_scan64(s, w[0] + w[1], all);
+  uint32_t bk = kBins, p0 = kBins, p1 = kBins;
+  uint64_t count_p = 0, weight_p = 0, count_k = 0, weight_k = 0, low = all, high = all, listed = 0;
+  if ((uint64_t)f.k < tokens) {
+    find_bin<false>(s, f.k, n, w, nb, wb);
+    bk = (uint32_t)s.found[0];
+    count_k = s.found[1];
+    weight_k = s.found[2];
+    // the first tokens of the bin weigh at least their share of it
+    const uint64_t in = s.found[3], size = s.pick[1], take = f.k - count_k;
+    low = weight_k + (uint64_t)((double)in * ((double)take / (double)size) * (1.0 - 0x1p-40));
+    high = weight_k + in;
+    listed = size;
+  }
+  if (f.p < 1.0) {
+    find_bin<true>(s, mass_of(f.p, high), n, w, nb, wb);
+    p1 = (uint32_t)s.found[0];
+    uint64_t in_p = s.pick[1];
+    find_bin<true>(s, mass_of(f.p, low), n, w, nb, wb);
+    p0 = (uint32_t)s.found[0];
+    count_p = s.found[1];
+    weight_p = s.found[2];
+    if (p0 != p1 || bk <= p1) {   // tokens from p0 to p1, and bk's where it is not among them
+      uint64_t in = 0, span;
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t b = 2 * tid + j;
+        if ((b >= p0 && b <= p1) || b == bk) in += n[j];
+      }
+      block_scan64(s, in, span);
+      listed = span;
+    } else {
+      listed += in_p;
+    }
+  }
+  if (tid == 0) {
+    rw.bk = bk;
+    rw.p0 = p0;
+    rw.p1 = p1;
+    rw.count_p = count_p;
+    rw.weight_p = weight_p;
+    rw.count_k = count_k;
+    rw.weight_k = weight_k;
+    rw.all = all;
+    if (listed > kList) rw.done = 2;
+  }
 }
 
 struct Cut { uint32_t key; uint64_t count, weight; };   // tokens and weight before the key's first one
@@ -119,21 +452,24 @@ struct Cut { uint32_t key; uint64_t count, weight; };   // tokens and weight bef
 // `target`, digit by digit; tokens of weight 0 do not count.  The target must
 // be reached.
 template <int DT, bool BY_WEIGHT>
-__device__ Cut select_key(RowShared& s, const void* row, int64_t V, const RowFilter& f, uint64_t target) {
+__device__ Cut select_key(SampleShared& s, const void* row, int64_t V, const RowFilter& f, uint64_t target) {
   Cut c{0, 0, 0};
+  uint64_t* sum = s.list;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    if (threadIdx.x < 256) {
-      s.cnt[threadIdx.x] = 0;
-      s.sum[threadIdx.x] = 0;
-    }
+    s.cnt[threadIdx.x] = 0;
+    sum[threadIdx.x] = 0;
     __syncthreads();
-    for (int64_t i = threadIdx.x; i < V; i += kRowThreads) {
-      const float l = load_logit<DT>(row, i);
-      const uint32_t key = order_key(l), w = weight_of(f, l);
-      if (w && (shift == 24 || (key >> (shift + 8)) == (c.key >> (shift + 8)))) {
-        atomicAdd(&s.cnt[(key >> shift) & 255], 1u);
-        atomicAdd((unsigned long long*)&s.sum[(key >> shift) & 255], (unsigned long long)w);
+    for (int64_t i = 8 * threadIdx.x; i < V; i += kBlock) {
+      float v[8];
+      load_logits<DT>(row, i, V, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t key = order_key(v[j]), w = weight_of(f, v[j]);
+        if (w && (shift == 24 || (key >> (shift + 8)) == (c.key >> (shift + 8)))) {
+          atomicAdd(&s.cnt[(key >> shift) & 255], 1u);
+          atomicAdd((unsigned long long*)&sum[(key >> shift) & 255], (unsigned long long)w);
+        }
       }
     }
     __syncthreads();
@@ -142,11 +478,11 @@ __device__ Cut select_key(RowShared& s, const void* row, int64_t V, const RowFil
       uint64_t n = 0, w = 0;
       for (int j = 0; j < 4; ++j) {
         n += s.cnt[d0 - j];
-        w += s.sum[d0 - j];
+        w += sum[d0 - j];
       }
       uint64_t nb = c.count + wave_scan64(n) - n, wb = c.weight + wave_scan64(w) - w;
       for (int j = 0; j < 4; ++j) {
-        const uint64_t nn = nb + s.cnt[d0 - j], ww = wb + s.sum[d0 - j];
+        const uint64_t nn = nb + s.cnt[d0 - j], ww = wb + sum[d0 - j];
         if (BY_WEIGHT ? wb < target && target <= ww : nb < target && target <= nn) {
           s.found[0] = d0 - j;
           s.found[1] = nb;
@@ -164,96 +500,215 @@ __device__ Cut select_key(RowShared& s, const void* row, int64_t V, const RowFil
   return c;
 }
 
-// One workgroup per row.
+// The cut of a whole row by one workgroup, for rows of many equal logits.
 template <int DT>
-__global__ __launch_bounds__(kRowThreads) void k_sample_row(SampleArgs a) {
-  __shared__ RowShared s;
-  const int64_t r = blockIdx.x, V = a.V;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const void* row = (const char*)a.logits + r * a.ls * (DT == LOGITS_F32 ? 4 : 2);
-  RowFilter f = row_filter(a, r);
-  float top = -__builtin_inff();
-  for (int64_t i = tid; i < V; i += kRowThreads) top = __builtin_fmaxf(top, load_logit<DT>(row, i));
-  for (int by = 32; by; by >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, by));
-  if (lane == 0) s.fpart[tid >> 6] = top;
+__device__ uint64_t cut_row(SampleShared& s, const RowWork& rw, const void* row, int64_t V, const RowFilter& f) {
+  uint32_t key = 0;
+  uint64_t ties = 0, all = rw.all;
+  if (rw.bk < (uint32_t)kBins) {
+    const Cut c = select_key<DT, false>(s, row, V, f, f.k);
+    key = c.key;
+    ties = f.k - c.count;
+    all = c.weight + ties * weight_of(f, logit_of(key));
+  }
+  if (f.p < 1.0) {   // at or above the top-k cut: the mass is at most all
+    const uint64_t mass = mass_of(f.p, all);
+    const Cut c = select_key<DT, true>(s, row, V, f, mass);
+    const uint64_t each = weight_of(f, logit_of(c.key));
+    key = c.key;
+    ties = (mass - c.weight + each - 1) / each;
+  }
+  // the index of the last of the key's `ties` first tokens
   __syncthreads();
-  for (int i = 0; i < kRowThreads / 64; ++i) top = __builtin_fmaxf(top, s.fpart[i]);
-  if (top == -__builtin_inff()) {   // every token masked
-    if (tid == 0) {
-      a.ids[r] = -1;
-      a.logprobs[r] = -__builtin_inff();
+  if (threadIdx.x == 0) s.found[0] = 0xffffffffu;
+  for (int64_t i0 = 0; i0 < V; i0 += kBlock) {
+    const int64_t i = i0 + 8 * threadIdx.x;
+    float v[8];
+    load_logits<DT>(row, i, V, v);
+    uint64_t n = 0, block;
+    for (int j = 0; j < 8; ++j) n += i + j < V && order_key(v[j]) == key;
+    uint64_t run = block_scan64(s, n, block);
+    if (ties <= block) {
+      for (int j = 0; j < 8; ++j) {
+        run += i + j < V && order_key(v[j]) == key;
+        if (run == ties && i + j < V && order_key(v[j]) == key) s.found[0] = (uint32_t)(i + j);
+      }
+      break;
     }
+    ties -= block;
+  }
+  __syncthreads();
+  return ((uint64_t)~key << 32) | (uint32_t)s.found[0];
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp, RowWork* work) {
+  __shared__ SampleShared s;
+  const Piece p = my_piece(sp, a.V);
+  RowWork& rw = work[p.row];
+  const int tid = threadIdx.x;
+  const uint32_t done = rw.done;
+  if (done == 1 || (done == 2 && p.piece)) return;
+  const void* row = row_of<DT>(a, p.row);
+  RowFilter f = row_filter(a, p.row);
+  f.top = block_max(s.fpart, tid < sp.pieces ? rw.top[tid] : -__builtin_inff());
+  const uint32_t p0 = rw.p0, p1 = rw.p1, bk = rw.bk;
+  if (done == 2) {
+    const uint64_t cut = cut_row<DT>(s, rw, row, a.V, f);
+    __syncthreads();
+    for (int q = 0; q < sp.pieces; ++q) {
+      const int64_t first = q * sp.size, end = first + sp.size < a.V ? first + sp.size : a.V;
+      uint64_t sum = 0, all;
+      for (int64_t i = first + 8 * tid; i < end; i += kBlock) {
+        float v[8];
+        load_logits<DT>(row, i, a.V, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = weight_of(f, v[j]);
+          sum += w >= f.least && place_of(v[j], i + j) <= cut ? w : 0;
+        }
+      }
+      block_scan64(s, sum, all);
+      if (tid == 0) s.piece[q] = all;
+    }
+    __syncthreads();
+    draw<DT>(s, a, sp, p.row, f, cut);
     return;
   }
-  f.top = top;
 
-  // the cut: tokens of larger keys, and the first `ties` tokens of its key
-  uint32_t cut = 0;
-  uint64_t ties = ~0ull;
-  uint64_t n = 0, w = 0, positive, all;
-  for (int64_t i = tid; i < V; i += kRowThreads) {
-    const uint32_t wi = weight_of(f, load_logit<DT>(row, i));
-    n += wi != 0;
-    w += wi;
-  }
-  block_scan64(s, n, positive);
-  block_scan64(s, w, all);
-  if ((uint64_t)f.k < positive) {
-    const Cut c = select_key<DT, false>(s, row, V, f, f.k);
-    cut = c.key;
-    ties = f.k - c.count;
-    const uint32_t b = cut ^ ((cut >> 31) ? 0x80000000u : 0xffffffffu);
-    all = c.weight + ties * weight_of(f, __builtin_bit_cast(float, b));
-  }
-  if (f.p < 1.0) {
-    const double m = __builtin_ceil(f.p * (double)all);
-    const uint64_t mass = m > 1.0 ? (uint64_t)m : 1;
-    const Cut c = select_key<DT, true>(s, row, V, f, mass);
-    const uint32_t b = c.key ^ ((c.key >> 31) ? 0x80000000u : 0xffffffffu);
-    const uint64_t each = weight_of(f, __builtin_bit_cast(float, b)), t = (mass - c.weight + each - 1) / each;
-    cut = c.key;      // at or above the top-k cut: mass <= all
-    ties = t;
-  }
-
-  // the draw: a thread's tokens are neighbours
-  const int64_t per = (V + kRowThreads - 1) / kRowThreads, i0 = tid * per, i1 = i0 + per < V ? i0 + per : V;
-  uint64_t equal = 0, unused;
-  for (int64_t i = i0; i < i1; ++i) equal += order_key(load_logit<DT>(row, i)) == cut;
-  const uint64_t rank0 = block_scan64(s, equal, unused);
-  uint64_t rank = rank0, kept = 0, total;
-  for (int64_t i = i0; i < i1; ++i) {
-    const float l = load_logit<DT>(row, i);
-    const uint32_t key = order_key(l), wi = weight_of(f, l);
-    if ((key > cut || (key == cut && rank < ties)) && wi >= f.least) kept += wi;
-    rank += key == cut;
-  }
-  const uint64_t before = block_scan64(s, kept, total);
-  const double at = __builtin_floor((double)a.u[r] * (double)total);
-  uint64_t target = at > 0.0 ? (uint64_t)at : 0;
-  target = target < total ? target : total - 1;
-  if (before <= target && target < before + kept) {
-    uint64_t run = before;
-    rank = rank0;
-    for (int64_t i = i0; i < i1; ++i) {
-      const float l = load_logit<DT>(row, i);
-      const uint32_t key = order_key(l), wi = weight_of(f, l);
-      if ((key > cut || (key == cut && rank < ties)) && wi >= f.least) run += wi;
-      rank += key == cut;
-      if (run > target) {
-        a.ids[r] = i;
-        const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
-        a.logprobs[r] = -away * 0x1.62e43p-1f - logf((float)total * 0x1p-31f);
-        break;
+  // weight above the cut's first bin, and the tokens of the cut's bins
+  const uint32_t above = p0 < (uint32_t)kBins ? p0 : bk;
+  if (tid == 0) s.pick[0] = 0;
+  __syncthreads();
+  uint64_t sum = 0;
+  for (int64_t i = p.first + 8 * tid; i < p.end; i += kBlock) {
+    float v[8];
+    load_logits<DT>(row, i, a.V, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = (uint32_t)bin_of(f, v[j]);
+      if (b < above) {
+        const uint32_t w = weight_of(f, v[j]);
+        sum += w >= f.least ? w : 0;
+      } else if (b < (uint32_t)kBins && ((b >= p0 && b <= p1) || b == bk) && weight_of(f, v[j])) {
+        s.list[atomicAdd(&s.pick[0], 1u)] = place_of(v[j], i + j);
       }
     }
   }
+  uint64_t kept;
+  block_scan64(s, sum, kept);
+  const uint32_t mine = s.pick[0];
+  if (tid == 0) {
+    put(&rw.piece[p.piece], kept);
+    s.pick[1] = mine ? atomicAdd(&rw.listed, mine) : 0;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < mine; i += kThreads) put(&rw.list[s.pick[1] + i], s.list[i]);
+  if (!last_of_row(s, &rw.ticket[1], sp.pieces)) return;
+
+  // sort the list
+  const uint32_t n = get(&rw.listed);
+  uint32_t size = 2;
+  while (size < n) size *= 2;
+  for (uint32_t i = tid; i < size; i += kThreads) s.list[i] = i < n ? get(&rw.list[i]) : ~0ull;
+  for (uint32_t k = 2; k <= size; k *= 2)
+    for (uint32_t j = k / 2; j; j /= 2) {
+      __syncthreads();
+      for (uint32_t i = tid; i < size / 2; i += kThreads) {
+        const uint32_t lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t x = s.list[lo], y = s.list[hi];
+        if ((x > y) == ((lo & k) == 0)) {
+          s.list[lo] = y;
+          s.list[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+
+  // The cut.  Two groups of bins that do not touch are two runs of the sorted
+  // row, each with its own count and weight before it.
+  const bool two = p1 < (uint32_t)kBins && bk < (uint32_t)kBins && p1 + 1 < bk;
+  const uint32_t per = (n + kThreads - 1) / kThreads, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
+  uint64_t wp = 0, wk = 0, np = 0, unused;
+  for (uint32_t i = i0; i < i1; ++i) {
+    const float l = logit_of(~(uint32_t)(s.list[i] >> 32));
+    const uint32_t w = weight_of(f, l);
+    if (two && (uint32_t)bin_of(f, l) == bk) wk += w;
+    else {
+      wp += w;
+      ++np;
+    }
+  }
+  uint64_t first_group;
+  const uint64_t before_p = block_scan64(s, wp, unused), before_k = block_scan64(s, wk, unused);
+  block_scan64(s, np, first_group);
+  const bool with_k = bk < (uint32_t)kBins;
+  // base of the first group: its bins start at p0, or at bk
+  const uint64_t count0 = p0 < (uint32_t)kBins ? rw.count_p : rw.count_k, weight0 = p0 < (uint32_t)kBins ? rw.weight_p : rw.weight_k;
+  const uint64_t count_k = rw.count_k, weight_k = rw.weight_k;
+  if (tid == 0) s.found[1] = rw.all;
+  __syncthreads();
+  if (with_k) {   // the weight that top-k leaves: at its last token
+    uint64_t run_p = before_p, run_k = before_k;
+    for (uint32_t i = i0; i < i1; ++i) {
+      const bool second = two && i >= first_group;
+      const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
+      const uint64_t place = second ? count_k + (i - first_group) : count0 + i;
+      (second ? run_k : run_p) += w;
+      if (place + 1 == (uint64_t)f.k) s.found[1] = second ? weight_k + run_k : weight0 + run_p;
+    }
+  }
+  __syncthreads();
+  const uint64_t mass = f.p < 1.0 ? mass_of(f.p, s.found[1]) : ~0ull;
+  uint64_t run = before_p;
+  __syncthreads();
+  for (uint32_t i = i0; i < i1 && i < first_group; ++i) {
+    const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
+    const bool keep = (!with_k || count0 + i < (uint64_t)f.k) && weight0 + run < mass;
+    const uint32_t wn = i + 1 < first_group ? weight_of(f, logit_of(~(uint32_t)(s.list[i + 1] >> 32))) : 0;
+    const bool next = i + 1 < first_group && wn && (!with_k || count0 + i + 1 < (uint64_t)f.k) && weight0 + run + w < mass;
+    if (keep && !next) s.found[0] = s.list[i];   // the last token kept
+    run += w;
+  }
+  s.piece[tid] = tid < sp.pieces ? get(&rw.piece[tid]) : 0;
+  __syncthreads();
+  const uint64_t cut = s.found[0];
+  for (uint32_t i = i0; i < i1; ++i)
+    if (s.list[i] <= cut) {
+      const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
+      if (w >= f.least) atomicAdd((unsigned long long*)&s.piece[(uint32_t)s.list[i] / (uint32_t)sp.size], (unsigned long long)w);
+    }
+  __syncthreads();
+  draw<DT>(s, a, sp, p.row, f, cut);
+}
+
+// Pieces of at least one 2,048-token block, so many that the rows together
+// make about four workgroups a compute unit.
+static Split sample_split(int64_t batch, int64_t V) {
+  const int64_t blocks = (V + kBlock - 1) / kBlock;
+  int64_t pieces = 1024 / (batch < 1024 ? batch : 1024);
+  pieces = pieces < 1 ? 1 : pieces;
+  pieces = pieces < blocks ? pieces : blocks;
+  pieces = pieces < kMaxSplits ? pieces : kMaxSplits;
+  const int64_t per = (blocks + pieces - 1) / pieces;
+  return Split{(int)((blocks + per - 1) / per), per * kBlock};
+}
+
+template <int DT>
+static void launch_sample(const SampleArgs& a, const Split& sp, RowWork* work, hipStream_t stream) {
+  const dim3 grid((unsigned)(a.batch * sp.pieces)), block(kThreads);
+  hipLaunchKernelGGL(k_sample_top<DT>, grid, block, 0, stream, a, sp, work);
+  hipLaunchKernelGGL(k_sample_bins<DT>, grid, block, 0, stream, a, sp, work);
+  hipLaunchKernelGGL(k_sample_draw<DT>, grid, block, 0, stream, a, sp, work);
 }
 
 }  // namespace m2r
 
 using namespace m2r;
 
-extern "C" int64_t m2r_sample_workspace(int64_t batch, int64_t V) { return 0; }
+extern "C" int64_t m2r_sample_workspace(int64_t batch, int64_t V) {
+  return batch > 0 ? batch * (int64_t)sizeof(RowWork) : 0;
+}
 
 extern "C" int m2r_sample(const void* logits, int dtype, int64_t row_stride, const float* uniforms,
                           const float* temperature, float temperature_all, const int32_t* top_k, int32_t top_k_all,
@@ -262,14 +717,18 @@ extern "C" int m2r_sample(const void* logits, int dtype, int64_t row_stride, con
                           hipStream_t stream) {
   if (batch <= 0 || V <= 0) return m2r_fail("sample: non-positive shape");
   if (batch > 0x7fffffff || V > 0x7fffffff) return m2r_fail("sample: size limits");
+  if (dtype < LOGITS_F16 || dtype > LOGITS_F32) return m2r_fail("sample: logits must be binary16 (0), bfloat16 (1) or binary32 (2)");
   if (!logits || !uniforms || !ids || !logprobs) return m2r_fail("sample: null pointer");
   if (row_stride < V && batch > 1) return m2r_fail("sample: rows overlap");
   SampleArgs a{logits, row_stride, uniforms, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all,
                top_k_all, ids, logprobs, batch, V};
-  const dim3 grid((unsigned)batch), block(kRowThreads);
-  if (dtype == LOGITS_F16) hipLaunchKernelGGL(k_sample_row<LOGITS_F16>, grid, block, 0, stream, a);
-  else if (dtype == LOGITS_BF16) hipLaunchKernelGGL(k_sample_row<LOGITS_BF16>, grid, block, 0, stream, a);
-  else if (dtype == LOGITS_F32) hipLaunchKernelGGL(k_sample_row<LOGITS_F32>, grid, block, 0, stream, a);
-  else return m2r_fail("sample: logits must be binary16 (0), bfloat16 (1) or binary32 (2)");
+  if (!workspace || workspace_bytes < m2r_sample_workspace(batch, V) || ((uintptr_t)workspace & 15))
+    return m2r_fail("sample: workspace too small or not 16-byte aligned");
+  const Split sp = sample_split(batch, V);
+  if (batch * sp.pieces > 0x7fffffff) return m2r_fail("sample: grid limits exceeded");
+  RowWork* work = (RowWork*)workspace;
+  if (dtype == LOGITS_F16) launch_sample<LOGITS_F16>(a, sp, work, stream);
+  else if (dtype == LOGITS_BF16) launch_sample<LOGITS_BF16>(a, sp, work, stream);
+  else launch_sample<LOGITS_F32>(a, sp, work, stream);
   return m2r_check(hipGetLastError(), "sample launch");
 }
