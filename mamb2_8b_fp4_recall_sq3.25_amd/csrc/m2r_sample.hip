@@ -31,19 +31,20 @@ struct SampleArgs {
   int64_t batch, V;
 };
 
-// A NaN counts as -inf (never drawn), -0 as +0.
+// A NaN counts as -inf (never drawn): the maximum of it and -inf.
+__device__ __forceinline__ float no_nan(float f) { return __builtin_fmaxf(f, -__builtin_inff()); }
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* row, int64_t i) {
   float f;
   if constexpr (DT == LOGITS_F32) f = ((const float*)row)[i];
   else if constexpr (DT == LOGITS_F16) f = h2f(((const uint16_t*)row)[i]);
   else f = __builtin_bit_cast(float, (uint32_t)((const uint16_t*)row)[i] << 16);
-  return f != f ? -__builtin_inff() : f + 0.0f;
+  return no_nan(f);
 }
 
-// Order-preserving map of a binary32 value (no NaN, no -0) to 32 bits.
+// Order-preserving map of a binary32 value (no NaN; -0 as +0) to 32 bits.
 __device__ __forceinline__ uint32_t order_key(float f) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, f);
+  const uint32_t b = __builtin_bit_cast(uint32_t, f + 0.0f);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
@@ -69,10 +70,17 @@ __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, int64_t row
   return f;
 }
 
-__device__ __forceinline__ uint32_t weight_of(const RowFilter& f, float l) {
-  const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
-  return away < 32.0f ? (uint32_t)(__builtin_amdgcn_exp2f(-away) * 0x1p31f) : 0u;
+// A token's distance from the largest logit as a power of two.  The maximum
+// with 0 answers 0 where the product is 0 * inf or inf - inf, the largest
+// logit's own distance.
+__device__ __forceinline__ float away_of(const RowFilter& f, float l) {
+  return __builtin_fmaxf((f.top - l) * f.rate, 0.0f);
 }
+// floor(2^31 2^-away); 0 from 32 on by itself.
+__device__ __forceinline__ uint32_t weight_at(float away) {
+  return (uint32_t)(__builtin_amdgcn_exp2f(-away) * 0x1p31f);
+}
+__device__ __forceinline__ uint32_t weight_of(const RowFilter& f, float l) { return weight_at(away_of(f, l)); }
 
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
@@ -176,7 +184,7 @@ __device__ __forceinline__ void load_logits(const void* row, int64_t i, int64_t 
       if constexpr (DT == LOGITS_F32) f = __builtin_bit_cast(float, w[j]);
       else if constexpr (DT == LOGITS_F16) f = h2f((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
       else f = __builtin_bit_cast(float, j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
-      v[j] = f != f ? -__builtin_inff() : f + 0.0f;
+      v[j] = no_nan(f);
     }
   } else {
 #pragma unroll
@@ -226,8 +234,7 @@ __device__ __forceinline__ bool last_of_row(SampleShared& s, uint32_t* ticket, i
 __device__ __forceinline__ void put_token(const SampleArgs& a, int64_t row, const RowFilter& f, int64_t i, float l,
                                           uint64_t total) {
   a.ids[row] = i;
-  const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
-  a.logprobs[row] = -away * 0x1.62e43p-1f - logf((float)total * 0x1p-31f);
+  a.logprobs[row] = -away_of(f, l) * 0x1.62e43p-1f - logf((float)total * 0x1p-31f);
 }
 
 // The draw, with the kept weight of each piece in s.piece: a token is kept
@@ -325,10 +332,9 @@ __device__ __forceinline__ uint64_t mass_of(double p, uint64_t all) {
   return m > 1.0 ? (uint64_t)m : 1;
 }
 
-__device__ __forceinline__ int bin_of(const RowFilter& f, float l) {
-  const float away = l == f.top ? 0.0f : (f.top - l) * f.rate;
-  return away < 32.0f ? (int)(away * 16.0f) : kBins;
-}
+// Bins of 1/16 of a power of two; kBins and more where the weight is 0.
+__device__ __forceinline__ uint32_t bin_at(float away) { return (uint32_t)__builtin_fminf(away * 16.0f, (float)kBins); }
+__device__ __forceinline__ uint32_t bin_of(const RowFilter& f, float l) { return bin_at(away_of(f, l)); }
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp, RowWork* work) {
@@ -378,8 +384,9 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp
       load_logits<DT>(row, i, a.V, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t w = weight_of(f, v[j]);
-        if (w) atomicAdd((unsigned long long*)&s.bins[bin_of(f, v[j])], (1ull << 46) | w);
+        const float away = away_of(f, v[j]);
+        const uint32_t w = weight_at(away);
+        if (w) atomicAdd((unsigned long long*)&s.bins[(uint32_t)(away * 16.0f)], (1ull << 46) | w);
       }
     }
     __syncthreads();
@@ -444,6 +451,114 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp
     rw.all = all;
     if (listed > kList) rw.done = 2;
   }
+}
+
+struct Place { uint64_t place, weight; };   // a token's place and the weight of the list before it
+
+// The token of s.list, among those of bins b0..b1, at which the running count
+// (BY_WEIGHT: weight) in the order of the places reaches `target`: digit by
+// digit from the first that differs.  The target must be reached.
+template <bool BY_WEIGHT>
+__device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, uint32_t b0, uint32_t b1, uint64_t target) {
+  const int tid = threadIdx.x;
+  uint64_t* sum = s.bins;   // 256 weights
+  auto takes = [&](uint64_t c) {
+    const uint32_t b = bin_of(f, logit_of(~(uint32_t)(c >> 32)));
+    return b >= b0 && b <= b1;
+  };
+  uint64_t any = 0, each = ~0ull;
+  for (uint32_t i = tid; i < n; i += kThreads)
+    if (takes(s.list[i])) {
+      any |= s.list[i];
+      each &= s.list[i];
+    }
+#pragma unroll
+  for (int by = 32; by; by >>= 1) {
+    any |= ((uint64_t)(uint32_t)__shfl_xor((int)(any >> 32), by) << 32) | (uint32_t)__shfl_xor((int)any, by);
+    each &= ((uint64_t)(uint32_t)__shfl_xor((int)(each >> 32), by) << 32) | (uint32_t)__shfl_xor((int)each, by);
+  }
+  __syncthreads();
+  if ((tid & 63) == 0) {
+    s.part[tid >> 6] = any;
+    s.found[tid >> 6] = each;
+  }
+  __syncthreads();
+  any = s.part[0] | s.part[1] | s.part[2] | s.part[3];
+  each = s.found[0] & s.found[1] & s.found[2] & s.found[3];
+  Place c{each, 0};
+  uint64_t count = 0;
+  if (n <= kThreads) {   // every token counts those before it
+    const uint64_t e = (uint32_t)tid < n ? s.list[tid] : 0;
+    const uint32_t w = weight_of(f, logit_of(~(uint32_t)(e >> 32)));
+    const bool in = (uint32_t)tid < n && takes(e);
+    __syncthreads();
+    sum[tid] = in ? w : 0;   // tokens that do not take part count nothing
+    __syncthreads();
+    for (uint32_t i = 0; i < n; ++i) {
+      const uint64_t wi = s.list[i] < e ? sum[i] : 0;
+      count += wi != 0;
+      c.weight += wi;
+    }
+    if (in && (BY_WEIGHT ? c.weight < target && target <= c.weight + w : count + 1 == target)) {
+      s.found[0] = e;
+      s.found[2] = c.weight;
+    }
+    __syncthreads();
+    c.place = s.found[0];
+    c.weight = s.found[2];
+    __syncthreads();
+    return c;
+  }
+  int shift = any == each ? -8 : (63 - __builtin_clzll(any ^ each)) & ~7;
+  if (shift >= 0) c.place = shift == 56 ? 0 : each >> (shift + 8) << (shift + 8);   // what all share
+  for (; shift >= 0; shift -= 8) {
+    __syncthreads();
+    s.cnt[tid] = 0;
+    sum[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += kThreads) {
+      const uint64_t e = s.list[i];
+      if (takes(e) && (shift == 56 || (e >> (shift + 8)) == (c.place >> (shift + 8)))) {
+        atomicAdd(&s.cnt[(e >> shift) & 255], 1u);
+        atomicAdd((unsigned long long*)&sum[(e >> shift) & 255],
+                  (unsigned long long)weight_of(f, logit_of(~(uint32_t)(e >> 32))));
+      }
+    }
+    __syncthreads();
+    if (tid < 64) {   // lane i: digits 4 i to 4 i + 3
+      uint64_t nn = 0, ww = 0;
+      for (int j = 0; j < 4; ++j) {
+        nn += s.cnt[4 * tid + j];
+        ww += sum[4 * tid + j];
+      }
+      uint64_t nb = count + wave_scan64(nn) - nn, wb = c.weight + wave_scan64(ww) - ww;
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t ne = nb + s.cnt[4 * tid + j], we = wb + sum[4 * tid + j];
+        if (BY_WEIGHT ? wb < target && target <= we : nb < target && target <= ne) {
+          s.found[0] = 4 * tid + j;
+          s.found[1] = nb;
+          s.found[2] = wb;
+          s.found[3] = ne - nb;
+        }
+        nb = ne;
+        wb = we;
+      }
+    }
+    __syncthreads();
+    c.place |= s.found[0] << shift;
+    count = s.found[1];
+    c.weight = s.found[2];
+    if (s.found[3] == 1) {   // one token has these digits
+      __syncthreads();
+      for (uint32_t i = tid; i < n; i += kThreads)
+        if (takes(s.list[i]) && (s.list[i] >> shift) == (c.place >> shift)) s.found[0] = s.list[i];
+      __syncthreads();
+      c.place = s.found[0];
+      break;
+    }
+  }
+  __syncthreads();
+  return c;
 }
 
 struct Cut { uint32_t key; uint64_t count, weight; };   // tokens and weight before the key's first one
@@ -577,7 +692,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
   }
 
   // weight above the cut's first bin, and the tokens of the cut's bins
-  const uint32_t above = p0 < (uint32_t)kBins ? p0 : bk;
+  const uint32_t above = p0 < (uint32_t)kBins ? p0 : bk, end = bk < (uint32_t)kBins ? bk + 1 : p1 + 1;
+  const float above16 = (float)above, end16 = (float)end;
   if (tid == 0) s.pick[0] = 0;
   __syncthreads();
   uint64_t sum = 0;
@@ -586,12 +702,11 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
     load_logits<DT>(row, i, a.V, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t b = (uint32_t)bin_of(f, v[j]);
-      if (b < above) {
-        const uint32_t w = weight_of(f, v[j]);
-        sum += w >= f.least ? w : 0;
-      } else if (b < (uint32_t)kBins && ((b >= p0 && b <= p1) || b == bk) && weight_of(f, v[j])) {
-        s.list[atomicAdd(&s.pick[0], 1u)] = place_of(v[j], i + j);
+      const float away = away_of(f, v[j]), t = away * 16.0f;
+      if (t < end16) {   // few tokens, and few waves that hold one
+        const uint32_t w = weight_at(away), b = (uint32_t)t;
+        if (t < above16) sum += w >= f.least ? w : 0;
+        else if (w && ((p0 <= b && b <= p1) || b == bk)) s.list[atomicAdd(&s.pick[0], 1u)] = place_of(v[j], i + j);
       }
     }
   }
@@ -606,73 +721,24 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
   for (uint32_t i = tid; i < mine; i += kThreads) put(&rw.list[s.pick[1] + i], s.list[i]);
   if (!last_of_row(s, &rw.ticket[1], sp.pieces)) return;
 
-  // sort the list
   const uint32_t n = get(&rw.listed);
-  uint32_t size = 2;
-  while (size < n) size *= 2;
-  for (uint32_t i = tid; i < size; i += kThreads) s.list[i] = i < n ? get(&rw.list[i]) : ~0ull;
-  for (uint32_t k = 2; k <= size; k *= 2)
-    for (uint32_t j = k / 2; j; j /= 2) {
-      __syncthreads();
-      for (uint32_t i = tid; i < size / 2; i += kThreads) {
-        const uint32_t lo = 2 * i - (i & (j - 1)), hi = lo + j;
-        const uint64_t x = s.list[lo], y = s.list[hi];
-        if ((x > y) == ((lo & k) == 0)) {
-          s.list[lo] = y;
-          s.list[hi] = x;
-        }
-      }
-    }
+  for (uint32_t i = tid; i < n; i += kThreads) s.list[i] = get(&rw.list[i]);
   __syncthreads();
-
-  // The cut.  Two groups of bins that do not touch are two runs of the sorted
-  // row, each with its own count and weight before it.
-  const bool two = p1 < (uint32_t)kBins && bk < (uint32_t)kBins && p1 + 1 < bk;
+  // Bins that do not touch are two runs of the sorted row, each with its own
+  // count and weight before it; top-p ends in the first, top-k in the second.
+  const bool with_k = bk < (uint32_t)kBins, with_p = p0 < (uint32_t)kBins, two = with_k && with_p && p1 + 1 < bk;
+  const uint64_t first_k = two || !with_p ? rw.count_k : rw.count_p, weight_k = two || !with_p ? rw.weight_k : rw.weight_p;
+  uint64_t all = rw.all, cut = ~0ull;
+  if (with_k) {
+    const Place c = select_place<false>(s, n, f, two ? bk : 0, kBins, (uint64_t)f.k - first_k);
+    cut = c.place;
+    all = weight_k + c.weight + weight_of(f, logit_of(~(uint32_t)(cut >> 32)));
+  }
+  if (with_p) cut = select_place<true>(s, n, f, 0, two ? p1 : kBins, mass_of(f.p, all) - rw.weight_p).place;
   const uint32_t per = (n + kThreads - 1) / kThreads, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
-  uint64_t wp = 0, wk = 0, np = 0, unused;
-  for (uint32_t i = i0; i < i1; ++i) {
-    const float l = logit_of(~(uint32_t)(s.list[i] >> 32));
-    const uint32_t w = weight_of(f, l);
-    if (two && (uint32_t)bin_of(f, l) == bk) wk += w;
-    else {
-      wp += w;
-      ++np;
-    }
-  }
-  uint64_t first_group;
-  const uint64_t before_p = block_scan64(s, wp, unused), before_k = block_scan64(s, wk, unused);
-  block_scan64(s, np, first_group);
-  const bool with_k = bk < (uint32_t)kBins;
-  // base of the first group: its bins start at p0, or at bk
-  const uint64_t count0 = p0 < (uint32_t)kBins ? rw.count_p : rw.count_k, weight0 = p0 < (uint32_t)kBins ? rw.weight_p : rw.weight_k;
-  const uint64_t count_k = rw.count_k, weight_k = rw.weight_k;
-  if (tid == 0) s.found[1] = rw.all;
   __syncthreads();
-  if (with_k) {   // the weight that top-k leaves: at its last token
-    uint64_t run_p = before_p, run_k = before_k;
-    for (uint32_t i = i0; i < i1; ++i) {
-      const bool second = two && i >= first_group;
-      const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
-      const uint64_t place = second ? count_k + (i - first_group) : count0 + i;
-      (second ? run_k : run_p) += w;
-      if (place + 1 == (uint64_t)f.k) s.found[1] = second ? weight_k + run_k : weight0 + run_p;
-    }
-  }
-  __syncthreads();
-  const uint64_t mass = f.p < 1.0 ? mass_of(f.p, s.found[1]) : ~0ull;
-  uint64_t run = before_p;
-  __syncthreads();
-  for (uint32_t i = i0; i < i1 && i < first_group; ++i) {
-    const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
-    const bool keep = (!with_k || count0 + i < (uint64_t)f.k) && weight0 + run < mass;
-    const uint32_t wn = i + 1 < first_group ? weight_of(f, logit_of(~(uint32_t)(s.list[i + 1] >> 32))) : 0;
-    const bool next = i + 1 < first_group && wn && (!with_k || count0 + i + 1 < (uint64_t)f.k) && weight0 + run + w < mass;
-    if (keep && !next) s.found[0] = s.list[i];   // the last token kept
-    run += w;
-  }
   s.piece[tid] = tid < sp.pieces ? get(&rw.piece[tid]) : 0;
   __syncthreads();
-  const uint64_t cut = s.found[0];
   for (uint32_t i = i0; i < i1; ++i)
     if (s.list[i] <= cut) {
       const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
