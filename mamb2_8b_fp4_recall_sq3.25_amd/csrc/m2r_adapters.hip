@@ -2,8 +2,14 @@
 //   out[m] = half(base[m] + scale[a] up[a] (down[a] x[m])),  a = ids[m],
 // and out[m] = base[m] where ids[m] names no adapter (negative, or not below
 // the number of adapters).  x [M, K], base and out [M, N] binary16 rows,
-// down [n, r, K], up [n, N, r] binary16, scale [n] binary32.  The hidden
-// values scale[a] (down[a] x[m]) pass between the two kernels in binary32.
+// down [n, r, Kp], up [n, N, r] binary16, scale [n] binary32; r a multiple of
+// 8 and Kp = K rounded up to 8, the rest zeros.
+//
+// Two launches on the matrix cores, rows in tiles of 16.  The first forms the
+// hidden values down x of a tile over a slice of K, in binary32; the second
+// adds the slices up and multiplies by up.  The rows of a tile that share an
+// adapter are one product, whose other columns are computed and dropped: a
+// prompt's rows are mostly one such group, a decode step's rows one each.
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 #include "m2r_tile.h"
@@ -11,6 +17,10 @@
 #include <initializer_list>
 
 namespace m2r {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t h16x8 __attribute__((ext_vector_type(8)));
 
 struct AdapterArgs {
   const uint16_t* x;
@@ -22,47 +32,282 @@ struct AdapterArgs {
   const int32_t* ids;
   uint16_t* out;
   int64_t os;
-  float* hidden;   // [M, r]
-  int64_t M, K, N, n;
+  float* hidden;        // [slices, M, r]
+  int64_t M, K, Kp, N, n;
   int r;
+  int slices;           // of K, `slice` long each (a multiple of 32)
+  int64_t slice;
+  int members;          // 16: a workgroup per row that leads its group; 1: a workgroup per tile
+  int64_t span;         // outputs of a wave in the second launch, a multiple of 32
 };
 
-// One wave per hidden value.
-__global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= a.M * a.r) return;
-  const int64_t m = w / a.r, j = w % a.r;
-  const int64_t id = a.ids[m];
-  if (id < 0 || id >= a.n) return;
-  const uint16_t *xr = a.x + m * a.xs, *d = a.down + (id * a.r + j) * a.K;
-  float acc = 0.f;
-  for (int64_t k = lane; k < a.K; k += 64) acc = __builtin_fmaf(h2f(xr[k]), h2f(d[k]), acc);
-  acc = wave_sum(acc);
-  if (lane == 0) a.hidden[w] = acc * a.scale[id];
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// 8 binary16 values at p (2-byte aligned), zeros from `valid` on.
+__device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p, int64_t valid) {
+  h16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (valid >= 8) __builtin_memcpy(&v, p, 16);
+  else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < valid) v[j] = p[j];
+  }
+  return __builtin_bit_cast(f16x8, v);
+}
+// The adapter of row m; -1 for none and past the last row.
+__device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t m) {
+  const int id = m < a.M ? a.ids[m] : -1;
+  return id >= 0 && id < a.n ? id : -1;
 }
 
-// One thread per output.
-__global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
-  const int64_t m = blockIdx.y, c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.N) return;
-  const int64_t id = a.ids[m];
-  uint16_t v = a.base[m * a.bs + c];
-  if (id >= 0 && id < a.n) {
-    const float* hid = a.hidden + m * a.r;
-    const uint16_t* u = a.up + (id * a.N + c) * a.r;
-    float acc = 0.f;
-    for (int j = 0; j < a.r; ++j) acc = __builtin_fmaf(hid[j], h2f(u[j]), acc);
-    v = f2h(h2f(v) + acc);
+// One wave per (tile, slice of K / 4): its four quarters meet in LDS.
+// RT: 16-rank tiles at a time.
+template <int RT>
+__global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
+  __shared__ f32x4 part[3][RT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+  int64_t w = blockIdx.x;
+  const int member = (int)(w % a.members);
+  w /= a.members;
+  const int slice = (int)(w % a.slices);
+  const int64_t m0 = w / a.slices * 16, m = m0 + lr;
+  const int id = adapter_of(a, m);
+  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xffffu;
+  if (a.members > 1) {   // only this row's group, if it is the first of it
+    const int mine = __builtin_amdgcn_readlane(id, member);
+    const uint32_t group = (uint32_t)__ballot(id == mine) & 0xffffu;
+    if (mine < 0 || (group & ((1u << member) - 1))) return;
+    todo = group;
   }
-  a.out[m * a.os + c] = v;
+  const int64_t quarter = (a.slice / 32 + 3) / 4 * 32;
+  const int64_t s1 = (slice + 1) * a.slice < a.Kp ? (slice + 1) * a.slice : a.Kp;
+  const int64_t k0 = slice * a.slice + wave * quarter, k1 = k0 + quarter < s1 ? k0 + quarter : s1;
+  const uint16_t* xr = a.x + (m < a.M ? m : a.M - 1) * a.xs;
+  while (todo) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+    const bool mine = id == cur;
+    todo &= ~(uint32_t)__ballot(mine);
+    for (int r0 = 0; r0 < a.r; r0 += 16 * RT) {
+      f32x4 acc[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const uint16_t* dr[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {   // ranks past the last read its row and are not stored
+        const int j = r0 + 16 * t + lr;
+        dr[t] = a.down + ((int64_t)cur * a.r + (j < a.r ? j : a.r - 1)) * a.Kp;
+      }
+#pragma unroll 4
+      for (int64_t k = k0 + 8 * lg; k < k1 + 8 * lg; k += 32) {
+        const bool in = k < k1;
+        const f16x8 xv = load_f16x8(xr + k, in ? a.K - k : 0);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = mfma16(load_f16x8(dr[t] + k, in ? 8 : 0), xv, acc[t]);
+      }
+      __syncthreads();
+      if (wave) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) part[wave - 1][t][lane] = acc[t];
+      }
+      __syncthreads();
+      if (wave == 0 && mine && m < a.M) {   // columns = rows m, rows = ranks 4 lg ...
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          f32x4 v = acc[t];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) v += part[q][t][lane];
+          const int j = r0 + 16 * t + 4 * lg;
+          if (j < a.r) *(f32x4*)(a.hidden + (slice * a.M + m) * a.r + j) = v;
+        }
+      }
+    }
+  }
+}
+
+// v 2^k as the sum of two binary16.
+__device__ __forceinline__ void split_f16(const float* v, float scale, f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const f16x2 h = __builtin_convertvector((f32x2{v[j] * scale, v[j + 1] * scale}), f16x2);
+    const f16x2 l = __builtin_convertvector(
+        (f32x2{__builtin_fmaf(v[j], scale, -(float)h[0]), __builtin_fmaf(v[j + 1], scale, -(float)h[1])}), f16x2);
+    hi[j] = h[0];
+    hi[j + 1] = h[1];
+    lo[j] = l[0];
+    lo[j + 1] = l[1];
+  }
+}
+
+// One wave per (MT tiles of 16 rows, span of outputs).  A lane holds row
+// 16 i + lr of each tile and 8 neighbouring outputs of 32: output tile T of
+// the pair takes outputs 8 q + 4 T + k of the 32 as its rows 4 q + k.  The
+// hidden values go in as two binary16, scaled by each row's largest.
+// KS: 32-rank steps.
+template <int MT, int KS>
+__global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int64_t spans = (a.N + a.span - 1) / a.span;
+  int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t span = w % spans;
+  w /= spans;
+  const int member = (int)(w % a.members);
+  const int64_t m0 = w / a.members * (16 * MT);
+  if (m0 >= a.M) return;
+  const int64_t n0 = span * a.span, n1 = n0 + a.span < a.N ? n0 + a.span : a.N;
+  int id[MT];
+  uint64_t todo = 0;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + 16 * i + lr;
+    id[i] = adapter_of(a, m);
+    todo |= (__ballot(m < a.M) & 0xffffull) << (16 * i);
+  }
+  if (MT == 1 && a.members > 1) {
+    const int mine = __builtin_amdgcn_readlane(id[0], member);
+    const uint64_t group = __ballot(id[0] == mine) & todo;
+    if (!(todo >> member & 1) || (group & ((1ull << member) - 1))) return;
+    todo = group;
+  }
+  while (todo) {
+    const int first = __builtin_ctzll(todo);
+    int cur = 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      if (first >> 4 == i) cur = __builtin_amdgcn_readlane(id[i], first & 15);
+    bool mine[MT];
+    const uint16_t* br[MT];
+    uint16_t* orow[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + 16 * i + lr;
+      mine[i] = id[i] == cur && m < a.M;
+      todo &= ~((__ballot(mine[i]) & 0xffffull) << (16 * i));
+      br[i] = a.base + (m < a.M ? m : 0) * a.bs;
+      orow[i] = a.out + (m < a.M ? m : 0) * a.os;
+    }
+    if (cur < 0) {   // rows without an adapter
+      for (int64_t n = n0 + 8 * lg; n < n1; n += 32)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          if (mine[i]) {
+            if (n + 8 <= a.N) __builtin_memcpy(orow[i] + n, br[i] + n, 16);
+            else
+              for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) orow[i][n + j] = br[i][n + j];
+          }
+      continue;
+    }
+    f16x8 hi[MT][KS], lo[MT][KS];
+    float back[MT];
+    const float sc = a.scale[cur];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      float v[KS][8], mx = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+        const int j0 = 32 * k + 8 * lg;
+        if (mine[i] && j0 < a.r) {
+          const float* h = a.hidden + (m0 + 16 * i + lr) * a.r + j0;
+          for (int q = 0; q < a.slices; ++q) {
+            const f32x4 u0 = *(const f32x4*)(h + (int64_t)q * a.M * a.r), u1 = *(const f32x4*)(h + (int64_t)q * a.M * a.r + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              v[k][j] += u0[j];
+              v[k][4 + j] += u1[j];
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[k][j] *= sc;
+            mx = __builtin_fmaxf(mx, __builtin_fabsf(v[k][j]));
+          }
+        }
+      }
+      // the row's largest, over its four lanes
+      const int iv = __builtin_bit_cast(int, mx);
+      const auto p = __builtin_amdgcn_permlane16_swap(iv, iv, false, false);
+      mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
+      const int jv = __builtin_bit_cast(int, mx);
+      const auto q = __builtin_amdgcn_permlane32_swap(jv, jv, false, false);
+      mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)q[0]), __builtin_bit_cast(float, (int)q[1]));
+      int e = 14 - (((__builtin_bit_cast(int, mx) >> 23) & 255) - 127);   // the largest below 2^15
+      e = e > 100 ? 100 : e;
+      const float up = __builtin_ldexpf(1.0f, e);
+      back[i] = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) split_f16(v[k], up, hi[i][k], lo[i][k]);
+    }
+    const uint16_t* ub = a.up + (int64_t)cur * a.N * a.r;
+    for (int64_t nb = n0; nb < n1; nb += 32) {
+      f32x4 acc[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int64_t n = nb + 8 * lg;
+      h16x8 bv[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        if (mine[i]) bv[i] = __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        const int64_t row = nb + 8 * (lr >> 2) + 4 * T + (lr & 3);
+        const uint16_t* ur = ub + (row < a.N ? row : a.N - 1) * a.r + 8 * lg;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const f16x8 uf = load_f16x8(ur + 32 * k, 32 * k + 8 * lg < a.r ? 8 : 0);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf, hi[i][k], acc[i][T]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf, lo[i][k], acc[i][T]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        if (mine[i]) {
+          h16x8 o;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = f2h(__builtin_fmaf(acc[i][j >> 2][j & 3], back[i], h2f(bv[i][j])));
+          if (n + 8 <= a.N) __builtin_memcpy(orow[i] + n, &o, 16);
+          else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (n + j < a.N) orow[i][n + j] = o[j];
+          }
+        }
+    }
+  }
+}
+
+// Few rows: a workgroup for each row that leads its group, so that groups run
+// side by side; many: a workgroup walks through its tile's groups, mostly one.
+constexpr int64_t kMemberRows = 512;
+
+static void adapter_plan(AdapterArgs& a) {
+  const int64_t tiles = (a.M + 15) / 16;
+  a.members = a.M <= kMemberRows ? (int)(a.M < 16 ? a.M : 16) : 1;
+  // slices of K for about 512 workgroups, of at least 512 each
+  int64_t s = 512 / (tiles * a.members);
+  const int64_t most = (a.Kp + 511) / 512;
+  s = s < most ? s : most;
+  s = s < 1 ? 1 : (s > 8 ? 8 : s);
+  a.slice = ((a.Kp + s - 1) / s + 31) / 32 * 32;
+  a.slices = (int)((a.Kp + a.slice - 1) / a.slice);
 }
 
 }  // namespace m2r
 
 using namespace m2r;
 
-extern "C" int64_t m2r_adapters_workspace(int64_t M, int64_t K, int64_t N, int64_t r) { return 4 * M * r; }
+extern "C" int64_t m2r_adapters_workspace(int64_t M, int64_t K, int64_t N, int64_t r) {
+  if (M <= 0 || K <= 0 || N <= 0 || r <= 0) return 0;
+  AdapterArgs a{};
+  a.M = M;
+  a.Kp = (K + 7) / 8 * 8;
+  adapter_plan(a);
+  return 4 * a.slices * M * r;
+}
 
 extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride,
                                 const void* down, const void* up, const float* scale, const int32_t* ids, void* out,
@@ -71,18 +316,43 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   if (M <= 0 || K <= 0 || N <= 0 || adapters <= 0 || rank <= 0) return m2r_fail("adapters: non-positive shape");
   const int64_t lim = (int64_t)1 << 24;
   if (M > lim || K > lim || N > lim || adapters > lim || rank > 256) return m2r_fail("adapters: size limits");
+  if (rank % 8) return m2r_fail("adapters: the rank must be a multiple of 8");
   for (const void* p : {x, base, down, up, (const void*)scale, (const void*)ids, (const void*)out, (const void*)workspace})
     if (!p) return m2r_fail("adapters: null pointer");
+  if (((uintptr_t)down | (uintptr_t)up) & 15) return m2r_fail("adapters: down and up must be 16-byte aligned");
   if (x_stride < K || base_stride < N || out_stride < N) return m2r_fail("adapters: rows overlap");
   if ((uintptr_t)workspace & 15 || workspace_bytes < m2r_adapters_workspace(M, K, N, rank))
     return m2r_fail("adapters: workspace too small or not 16-byte aligned");
   AdapterArgs a{(const uint16_t*)x, x_stride, (const uint16_t*)base, base_stride, (const uint16_t*)down,
-                (const uint16_t*)up, scale, ids, (uint16_t*)out, out_stride, (float*)workspace, M, K, N, adapters,
-                (int)rank};
-  if (M > 65535) return m2r_fail("adapters: grid limits exceeded");
-  hipLaunchKernelGGL(k_adapter_down, dim3((unsigned)((M * rank + 3) / 4)), dim3(256), 0, stream, a);
+                (const uint16_t*)up, scale, ids, (uint16_t*)out, out_stride, (float*)workspace, M, K, (K + 7) / 8 * 8, N,
+                adapters, (int)rank};
+  adapter_plan(a);
+  const int64_t tiles = (M + 15) / 16;
+  if (tiles * a.members * a.slices > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
+  const dim3 down_grid((unsigned)(tiles * a.members * a.slices)), block(256);
+  if (rank <= 16) hipLaunchKernelGGL(k_adapter_down<1>, down_grid, block, 0, stream, a);
+  else if (rank <= 32) hipLaunchKernelGGL(k_adapter_down<2>, down_grid, block, 0, stream, a);
+  else hipLaunchKernelGGL(k_adapter_down<4>, down_grid, block, 0, stream, a);
   int rc = m2r_check(hipGetLastError(), "adapters down launch");
   if (rc) return rc;
-  hipLaunchKernelGGL(k_adapter_up, dim3((unsigned)((N + 255) / 256), (unsigned)M), dim3(256), 0, stream, a);
+  // four tiles share a pass over `up` where rows are many and the rank small
+  const bool wide = a.members == 1 && rank <= 64;
+  const int64_t groups = wide ? (M + 63) / 64 : tiles * a.members;
+  int64_t spans = 2048 / groups;
+  const int64_t most = (N + 63) / 64;
+  spans = spans < 1 ? 1 : (spans < most ? spans : most);
+  a.span = ((N + spans - 1) / spans + 31) / 32 * 32;
+  spans = (N + a.span - 1) / a.span;
+  if ((groups * spans + 3) / 4 > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
+  const dim3 up_grid((unsigned)((groups * spans + 3) / 4));
+  if (wide) {
+    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<4, 1>), up_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_up<4, 2>), up_grid, block, 0, stream, a);
+  } else {
+    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<1, 1>), up_grid, block, 0, stream, a);
+    else if (rank <= 64) hipLaunchKernelGGL((k_adapter_up<1, 2>), up_grid, block, 0, stream, a);
+    else if (rank <= 128) hipLaunchKernelGGL((k_adapter_up<1, 4>), up_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_up<1, 8>), up_grid, block, 0, stream, a);
+  }
   return m2r_check(hipGetLastError(), "adapters up launch");
 }

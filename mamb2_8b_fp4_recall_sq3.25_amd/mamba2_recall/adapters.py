@@ -11,6 +11,7 @@ kernels of libm2r_hip.so (m2r_adapters_add)."""
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
 
 from . import _native
 
@@ -36,20 +37,13 @@ class AdapterSet:
         if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (n,)
                 or scale.device != down.device):
             raise ValueError("scale must be FP32[n] on the adapters' device")
-        self.down, self.up, self.scale = down.contiguous(), up.contiguous(), scale.contiguous()
-
-    @property
-    def count(self):
-        return self.down.shape[0]
-
-    @property
-    def rank(self):
-        return self.down.shape[1]
-
-    @property
-    def features(self):
-        """(K, N) of the projection."""
-        return self.down.shape[2], self.up.shape[1]
+        self.count, self.rank = n, rank
+        self.features = down.shape[2], up.shape[1]     # (K, N) of the projection
+        # the kernels read ranks and inputs in eights: zeros fill the last
+        fill, tail = -rank % 8, -down.shape[2] % 8
+        self.down = F.pad(down, (0, tail, 0, fill)) if fill or tail else down.contiguous()
+        self.up = F.pad(up, (0, fill)) if fill else up.contiguous()
+        self.scale = scale.contiguous()
 
 
 def _rows(t, features, what):
@@ -88,11 +82,12 @@ def add(base, x, adapters, ids, out=None):
     if rows == 0:
         return out
     ids = ids.contiguous()
-    ws_bytes = int(_native.lib().m2r_adapters_workspace(rows, k, n, adapters.rank))
+    rank = adapters.down.shape[1]
+    ws_bytes = int(_native.lib().m2r_adapters_workspace(rows, k, n, rank))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=base.device)
     p = _native.ptr
     with _native.device_of(base):
         _native.call("m2r_adapters_add", p(x2), xs, p(b2), bs, p(adapters.down), p(adapters.up), p(adapters.scale),
-                     p(ids), p(out), n, rows, k, n, adapters.count, adapters.rank, p(ws), ws_bytes,
+                     p(ids), p(out), n, rows, k, n, adapters.count, rank, p(ws), ws_bytes,
                      _native.stream_of(base))
     return out
