@@ -241,28 +241,38 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
       for (int k = 0; k < KS; ++k) split_f16(v[k], up, hi[i][k], lo[i][k]);
     }
     const uint16_t* ub = a.up + (int64_t)cur * a.N * a.r;
-    for (int64_t nb = n0; nb < n1; nb += 32) {
-      f32x4 acc[MT][2];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // the next 32 outputs' operands are on their way while these are formed
+    h16x8 bv[MT], bn[MT];
+    f16x8 uf[2][KS], un[2][KS];
+    auto fetch = [&](int64_t nb, h16x8 (&bd)[MT], f16x8 (&ud)[2][KS]) {
       const int64_t n = nb + 8 * lg;
-      h16x8 bv[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        if (mine[i]) bv[i] = __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
+        if (mine[i]) bd[i] = __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
         const int64_t row = nb + 8 * (lr >> 2) + 4 * T + (lr & 3);
         const uint16_t* ur = ub + (row < a.N ? row : a.N - 1) * a.r + 8 * lg;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const f16x8 uf = load_f16x8(ur + 32 * k, 32 * k + 8 * lg < a.r ? 8 : 0);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf, hi[i][k], acc[i][T]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf, lo[i][k], acc[i][T]);
-        }
+        for (int k = 0; k < KS; ++k) ud[T][k] = load_f16x8(ur + 32 * k, 32 * k + 8 * lg < a.r ? 8 : 0);
       }
+    };
+    fetch(n0, bv, uf);
+    for (int64_t nb = n0; nb < n1; nb += 32) {
+      const int64_t n = nb + 8 * lg;
+      if (nb + 32 < n1) fetch(nb + 32, bn, un);
+      f32x4 acc[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf[T][k], hi[i][k], acc[i][T]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][T] = mfma16(uf[T][k], lo[i][k], acc[i][T]);
+        }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
         if (mine[i]) {
@@ -276,6 +286,12 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
               if (n + j < a.N) orow[i][n + j] = o[j];
           }
         }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) bv[i] = bn[i];
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) uf[T][k] = un[T][k];
     }
   }
 }
@@ -335,10 +351,10 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   else hipLaunchKernelGGL(k_adapter_down<4>, down_grid, block, 0, stream, a);
   int rc = m2r_check(hipGetLastError(), "adapters down launch");
   if (rc) return rc;
-  // four tiles share a pass over `up` where rows are many and the rank small
-  const bool wide = a.members == 1 && rank <= 64;
-  const int64_t groups = wide ? (M + 63) / 64 : tiles * a.members;
-  int64_t spans = 2048 / groups;
+  // two tiles share a pass over `up` where rows are many and the rank small
+  const bool wide = a.M > kMemberRows && rank <= 64;
+  const int64_t groups = wide ? (M + 31) / 32 : tiles * a.members;
+  int64_t spans = 4096 / groups;
   const int64_t most = (N + 63) / 64;
   spans = spans < 1 ? 1 : (spans < most ? spans : most);
   a.span = ((N + spans - 1) / spans + 31) / 32 * 32;
@@ -346,8 +362,8 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   if ((groups * spans + 3) / 4 > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
   const dim3 up_grid((unsigned)((groups * spans + 3) / 4));
   if (wide) {
-    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<4, 1>), up_grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((k_adapter_up<4, 2>), up_grid, block, 0, stream, a);
+    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<2, 1>), up_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_up<2, 2>), up_grid, block, 0, stream, a);
   } else {
     if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<1, 1>), up_grid, block, 0, stream, a);
     else if (rank <= 64) hipLaunchKernelGGL((k_adapter_up<1, 2>), up_grid, block, 0, stream, a);

@@ -51,12 +51,14 @@ def _rows(t, features, what):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or not t.is_cuda or t.ndim < 1 \
             or t.shape[-1] != features:
         raise ValueError(f"{what} must be CUDA FP16[..., {features}]")
-    if t.ndim != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < features):
-        t = t.reshape(-1, features).contiguous()
-    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else features
+    if t.ndim != 2:
+        t = t.reshape(-1, features)
+    rows, (stride, column) = t.shape[0], t.stride()
+    if column != 1 and features > 1 or rows > 1 and stride < features:
+        t, stride = t.contiguous(), features
+    return t, rows, stride if rows > 1 else features
 
 
-@torch.no_grad()
 def add(base, x, adapters, ids, out=None):
     """base[..., N] plus each row's adapter update of x[..., K]; a new FP16
     tensor, or `out` (which may be `base`).  `ids` int32[...] names each row's

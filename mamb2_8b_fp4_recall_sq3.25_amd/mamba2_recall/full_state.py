@@ -25,7 +25,8 @@ def allocate_state(slots, heads, dim, dstate, device):
     return torch.zeros((slots, heads, dim, N), dtype=torch.float32, device=device)
 
 
-def _check(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
+def _refuse(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
+    """The reason why a call is not taken."""
     if not isinstance(x, torch.Tensor) or x.ndim != 4 or x.dtype != torch.float16 or not x.is_cuda:
         raise ValueError("x must be CUDA FP16[batch,tokens,heads,dim]")
     batch, length, heads, dim = x.shape
@@ -37,7 +38,7 @@ def _check(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
         raise ValueError("state must be contiguous FP32[slots,heads,dim,128] on the device of x")
     if slots is None and state.shape[0] < batch:
         raise ValueError("A carry for every batch row, or slots, required")
-    if B.ndim != 4:
+    if not isinstance(B, torch.Tensor) or B.ndim != 4:
         raise ValueError("B must have four axes")
     groups = B.shape[2]
     if groups < 1 or heads % groups:
@@ -45,7 +46,7 @@ def _check(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
     shapes = ((dt, (batch, length, heads)), (A, (heads,)), (B, (batch, length, groups, N)),
               (C, (batch, length, groups, N)), (D, (heads,)), (dt_bias, (heads,)))
     for t, shape in shapes:
-        if tuple(t.shape) != shape or t.device != x.device:
+        if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.device != x.device:
             raise ValueError("Input device/geometry mismatch")
     if A.dtype != torch.float32 or any(t.dtype != torch.float16 for t in (dt, B, C)):
         raise ValueError("A must be FP32; dt/B/C must be FP16")
@@ -55,22 +56,39 @@ def _check(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
         if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (batch,)
                               or t.device != x.device):
             raise ValueError(f"{name} must be int32[batch] on the device of x")
-    return batch, length, heads, dim, groups
+
+
+def _taken(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
+    """The same conditions at once, for the call that meets them: a step of a
+    few microseconds is bound by the host."""
+    try:
+        batch, length, heads, dim = xs = x.shape
+        groups = B.shape[2]
+        bc, h, dev, f16, f32, i32 = (batch, length, groups, N), (heads,), x.device, torch.float16, torch.float32, torch.int32
+        return (x.dtype is f16 and x.is_cuda and 0 not in xs and state.dtype is f32 and state.is_contiguous()
+                and state.shape[1:] == (heads, dim, N) and state.shape[0] >= (1 if slots is not None else batch)
+                and groups > 0 and heads % groups == 0 and dt.shape == xs[:3] and B.shape == bc and C.shape == bc
+                and A.shape == h and D.shape == h and dt_bias.shape == h and A.dtype is f32
+                and dt.dtype is f16 and B.dtype is f16 and C.dtype is f16
+                and (D.dtype is f16 or D.dtype is f32) and (dt_bias.dtype is f16 or dt_bias.dtype is f32)
+                and state.device == dt.device == A.device == B.device == C.device == D.device == dt_bias.device == dev
+                and (lengths is None or lengths.dtype is i32 and lengths.shape == (batch,) and lengths.device == dev)
+                and (slots is None or slots.dtype is i32 and slots.shape == (batch,) and slots.device == dev))
+    except (AttributeError, ValueError, IndexError):
+        return False
 
 
 def _token_rows(t):
-    """`t` [batch, tokens, ...] with dense trailing dimensions and its two
-    leading strides; any view whose tokens are dense rows is read in place."""
-    inner = 1
-    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
-        if size > 1 and stride != inner:
-            t = t.contiguous()
-            break
-        inner *= size
-    return t, t.stride(0), t.stride(1)
+    """`t` [batch, tokens, ...] and its strides of batch rows and tokens; any
+    view whose tokens are dense rows is read in place."""
+    s, n = t.stride(), t.shape
+    dense = s[2] == 1 or n[2] == 1 if len(n) == 3 else (s[3] == 1 or n[3] == 1) and (s[2] == n[3] or n[2] == 1)
+    if not dense:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[0], s[1]
 
 
-@torch.no_grad()
 def scan(x, dt, A, B, C, D, dt_bias, state, *, lengths=None, slots=None):
     """Advance carries over the tokens of x; return (FP16 readouts, None).
 
@@ -82,20 +100,29 @@ def scan(x, dt, A, B, C, D, dt_bias, state, *, lengths=None, slots=None):
     count (default: L; values are clamped to 0..L).  Readouts past a row's
     length, and an idle row's, are zero; the carry stands after the row's last
     token.  A non-finite input makes the affected readouts of its own and
-    later tokens non-finite, and no earlier ones."""
-    geo = _check(x, dt, A, B, C, D, dt_bias, state, lengths, slots)
-    (x, *xs), (dt, *ds), (B, *bs), (C, *cs) = map(_token_rows, (x, dt, B, C))
+    later tokens non-finite, and no earlier ones.  Forward only."""
+    if not _taken(x, dt, A, B, C, D, dt_bias, state, lengths, slots):
+        _refuse(x, dt, A, B, C, D, dt_bias, state, lengths, slots)
+    batch, length, heads, dim = x.shape
+    groups = B.shape[2]
+    x, xb, xl = _token_rows(x)
+    dt, db, dl = _token_rows(dt)
+    B, bb, bl = _token_rows(B)
+    C, cb, cl = _token_rows(C)
     A, D, dt_bias = A.contiguous(), D.contiguous(), dt_bias.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    slots = None if slots is None else slots.contiguous()
-    y = torch.empty(x.shape, dtype=torch.float16, device=x.device)
-    ws_bytes = int(_native.lib().m2r_full_scan_workspace(*geo))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    slots = slots.contiguous() if slots is not None else None
+    y = torch.empty((batch, length, heads, dim), dtype=torch.float16, device=x.device)
+    ws, ws_bytes = None, 0
+    if length > 1:
+        ws_bytes = _native.lib().m2r_full_scan_workspace(batch, length, heads, dim, groups)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     p = _native.ptr
     with _native.device_of(x):
-        _native.call("m2r_full_scan", p(x), *xs, p(dt), *ds, p(A), p(B), *bs, p(C), *cs, p(D),
-                     int(D.dtype == torch.float32), p(dt_bias), int(dt_bias.dtype == torch.float32), p(state),
-                     state.shape[0], p(slots), p(lengths), p(y), *geo, p(ws), ws_bytes, _native.stream_of(x))
+        _native.call("m2r_full_scan", x.data_ptr(), xb, xl, dt.data_ptr(), db, dl, A.data_ptr(), B.data_ptr(), bb, bl,
+                     C.data_ptr(), cb, cl, D.data_ptr(), D.dtype is torch.float32, dt_bias.data_ptr(),
+                     dt_bias.dtype is torch.float32, state.data_ptr(), state.shape[0], p(slots), p(lengths),
+                     y.data_ptr(), batch, length, heads, dim, groups, p(ws), ws_bytes, _native.stream_of(x))
     return y, None
 
 

@@ -24,7 +24,6 @@ def _filter(value, name, dtype, logits, low, high):
     return None, value
 
 
-@torch.no_grad()
 def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draw one token a row: (ids int64[B], logprobs float32[B]).
 
