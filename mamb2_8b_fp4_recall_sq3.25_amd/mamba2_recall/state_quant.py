@@ -26,7 +26,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _native, fp4, state_codec
+from . import _native, adapters, fp4, state_codec
 
 # Installed controllers, keyed by the identity of the model each owns.  Values
 # are held weakly; the installed per-layer hooks keep a controller alive until
@@ -274,6 +274,7 @@ class _MixerController:
         self._running = False     # inside backbone()
         self._rates = {}
         self._packed = None
+        self._adapters = None     # (a dict of AdapterSet or None for each layer, ids int32[batch])
         self._stat_sums = {}      # layer index -> FP64 [groups, 128] totals
         self._stat_counts = [0] * len(self._mixers)
 
@@ -503,6 +504,7 @@ class _MixerController:
             zxbcdt = self._project(index, "in_proj", mx, u[:, 0])[:, None]
         else:
             zxbcdt = mx.in_proj(u)
+        zxbcdt = self._adapt(index, "in_proj", zxbcdt, u)
         z, xbc, dt = torch.split(zxbcdt, self._in_sizes, dim=-1)
         if step:
             parts = torch.split(self._conv_step(mx, xbc[:, 0], layer)[:, None], self._conv_sizes, dim=-1)
@@ -520,9 +522,13 @@ class _MixerController:
         # the gated norm is called as a module, so its hooks see (y, z)
         y = y.reshape(batch, tokens, self.D_INNER)
         if step:
-            out = self._project(index, "out_proj", mx, mx.norm(y[:, 0], z[:, 0]))[:, None]
+            v = mx.norm(y[:, 0], z[:, 0])
+            out = self._project(index, "out_proj", mx, v)[:, None]
+            v = v[:, None]
         else:
-            out = mx.out_proj(mx.norm(y, z))
+            v = mx.norm(y, z)
+            out = mx.out_proj(v)
+        out = self._adapt(index, "out_proj", out, v)
         layer.tokens += tokens
         return out
 
@@ -576,6 +582,45 @@ class _MixerController:
         if entry is not None and fp4.gemv_supported(value.shape[0], value.shape[1]):
             return fp4.gemv_g16(*entry[name], value)
         return getattr(mx, name)(value)
+
+    def use_adapters(self, sets, ids=None):
+        """Give every request its own low-rank adapter of the projections.
+        `sets[i]` is a dict of adapters.AdapterSet for layer i under
+        "in_proj" and "out_proj" (either may be left out), or None; `ids`
+        int32[batch] names each batch row's adapter in every set (outside a
+        set's count: none).  `sets=None` turns adapters off.  The update joins
+        the projection's FP16 output, of prompts and of single tokens, whether
+        the projection ran as its module or as a packed GEMV; a row without an
+        adapter keeps its bits."""
+        if sets is None:
+            self._adapters = None
+            return self
+        if len(sets) != len(self._mixers):
+            raise ValueError("One adapter entry per layer required")
+        if (not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.ndim != 1 or ids.shape[0] < 1
+                or ids.device != self.device):
+            raise ValueError("ids must be int32[batch] on the model device")
+        for mx, entry in zip(self._mixers, sets):
+            for name, item in (entry or {}).items():
+                if name not in ("in_proj", "out_proj") or not isinstance(item, adapters.AdapterSet):
+                    raise ValueError("Adapter entries are AdapterSets under in_proj and out_proj")
+                if item.features != tuple(reversed(getattr(mx, name).weight.shape)) or item.down.device != self.device:
+                    raise ValueError(f"Adapters of {name} do not match the layer's projection")
+        self._adapters = (list(sets), ids.contiguous())
+        return self
+
+    def _adapt(self, index, name, out, value):
+        """`out`, one layer's projection of `value` [batch, tokens, K], with
+        the requests' adapters."""
+        if self._adapters is None:
+            return out
+        sets, ids = self._adapters
+        item = (sets[index] or {}).get(name)
+        if item is None:
+            return out
+        if ids.shape[0] != out.shape[0]:
+            raise ValueError("Adapter ids and batch differ")
+        return adapters.add(out, value, item, ids[:, None].expand(out.shape[:2]))
 
     def _decay_rates(self, index, mx):
         """A = -exp(float(A_log)) of one layer (state_quant.py:256), kept
