@@ -33,7 +33,7 @@ __device__ __forceinline__ int x_at(int row, int col) { return row * kPitchX + 8
 // tile j; powers are of two.
 struct ChunkScalars {
   float lh[kChunk], ll[kChunk];   // l as a sum of two binary32
-  float dlh[kChunk], dll[kChunk]; // l - log2 dt, likewise
+  float lt[kChunk];               // l - r of the tile before
   float dt[kChunk];
   float ws[kChunk];               // dt 2^(r_tile - l)
   float w[kChunk];                // dt 2^(l_63 - l)
@@ -62,22 +62,27 @@ struct Segments {
   float* decay;       // [count, batch, H]
 };
 
-__device__ __forceinline__ float wave_max(float v) {   // of non-negative values; NaN is passed over
-#define M2R_MAX_DPP(ctrl)                                                                                        \
-  v = __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, \
-                                                                              0xF, 0xF, true)))
-  M2R_MAX_DPP(0xB1);
-  M2R_MAX_DPP(0x4E);
-  M2R_MAX_DPP(0x141);
-  M2R_MAX_DPP(0x140);
+// The largest over the wave.  Non-negative binary32 values order as their
+// bits do, NaN above infinity.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+#define M2R_MAX_DPP(ctrl)                                                                     \
+  {                                                                                          \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, true); \
+    v = v > o ? v : o;                                                                       \
+  }
+  M2R_MAX_DPP(0xB1)
+  M2R_MAX_DPP(0x4E)
+  M2R_MAX_DPP(0x141)
+  M2R_MAX_DPP(0x140)
 #undef M2R_MAX_DPP
-  const int iv = __builtin_bit_cast(int, v);
-  const auto r = __builtin_amdgcn_permlane16_swap(iv, iv, false, false);
-  v = __builtin_fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
-  const int jv = __builtin_bit_cast(int, v);
-  const auto q = __builtin_amdgcn_permlane32_swap(jv, jv, false, false);
-  v = __builtin_fmaxf(__builtin_bit_cast(float, (int)q[0]), __builtin_bit_cast(float, (int)q[1]));
-  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  const auto r = __builtin_amdgcn_permlane16_swap((int)v, (int)v, false, false);
+  v = (uint32_t)r[0] > (uint32_t)r[1] ? (uint32_t)r[0] : (uint32_t)r[1];
+  const auto q = __builtin_amdgcn_permlane32_swap((int)v, (int)v, false, false);
+  v = (uint32_t)q[0] > (uint32_t)q[1] ? (uint32_t)q[0] : (uint32_t)q[1];
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return __builtin_bit_cast(float, wave_max_bits(__builtin_bit_cast(uint32_t, v)));
 }
 // floor(log2 v) of a positive normal v (-127 for zero and subnormals).
 __device__ __forceinline__ int exponent_of(float v) { return ((__builtin_bit_cast(int, v) >> 23) & 255) - 127; }
@@ -89,6 +94,20 @@ __device__ __forceinline__ float pow2(int k) { return __builtin_ldexpf(1.0f, k);
 // 22 bits, and is summed in binary32 by the matrix instruction.  `scale`, a
 // power of two, comes with the conversions: v scale - high is one mixed fma.
 struct Split { f16x8 hi, lo; };
+__device__ __forceinline__ Split split8(const float* v, float one) {   // one: 1, not known to the compiler
+  Split s;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const f16x2 h = __builtin_convertvector((f32x2{v[j], v[j + 1]}), f16x2);
+    const f16x2 l = __builtin_convertvector(
+        (f32x2{__builtin_fmaf(v[j], one, -(float)h[0]), __builtin_fmaf(v[j + 1], one, -(float)h[1])}), f16x2);
+    s.hi[j] = h[0];
+    s.hi[j + 1] = h[1];
+    s.lo[j] = l[0];
+    s.lo[j + 1] = l[1];
+  }
+  return s;
+}
 __device__ __forceinline__ Split split8_scaled(const float* v, float scale) {
   Split s;
 #pragma unroll
@@ -194,8 +213,7 @@ __device__ __forceinline__ uint32_t max_magnitudes(uint32_t m, u32x2 v) {
 }
 __device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
   const uint32_t lo = m & 0xffffu, hi = m >> 16;
-  // non-negative binary32 values order as their bits do
-  return __builtin_bit_cast(uint32_t, wave_max(__builtin_bit_cast(float, lo > hi ? lo : hi)));
+  return wave_max_bits(lo > hi ? lo : hi);
 }
 // A workgroup steps four blocks of 64 columns (a head's channels) of one
 // group, two waves each, over one segment of one batch row's tokens.  OUT:
@@ -346,13 +364,12 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       const float dt = c0 + lane < n ? full_dt(h2f(rdt) + bias) : 0.f;
       const double l = scan_add64((double)av * (double)dt * 1.4426950408889634);
       const double last = lane64(l, 63), tile = dpp_row_last64(l);
+      const double e0 = lane64(l, 15), e1 = lane64(l, 31), e2 = lane64(l, 47);
+      const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e1 : e2));
       const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - l));
       hs.lh[lane] = lh;
       hs.ll[lane] = __builtin_fabsf(lh) < __builtin_inff() ? (float)(l - (double)lh) : 0.f;
-      const double ld = l - (double)__builtin_amdgcn_logf(dt);   // infinite for a step of 0
-      const float dlh = (float)ld;
-      hs.dlh[lane] = dlh;
-      hs.dll[lane] = __builtin_fabsf(dlh) < __builtin_inff() ? (float)(ld - (double)dlh) : 0.f;
+      hs.lt[lane] = (float)(l - before);
       hs.dt[lane] = dt;
       hs.ws[lane] = dt * __builtin_amdgcn_exp2f((float)(tile - l));
       hs.w[lane] = w;
@@ -545,11 +562,14 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
           {
             const f32x4 gt = s.scores[i * (i + 1) / 2 + i][lane];
-            const f32x4 sh = *(const f32x4*)(hs.dlh + 16 * i + 4 * lg), sl = *(const f32x4*)(hs.dll + 16 * i + 4 * lg);
+            const f32x4 sd = *(const f32x4*)(hs.dt + 16 * i + 4 * lg), sl = *(const f32x4*)(hs.lt + 16 * i + 4 * lg);
+            const float tt = hs.lt[16 * i + lr] + fkm;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const float e = __builtin_amdgcn_exp2f((th - sh[k]) + (tl - sl[k]));
-              v[4 * i + k] = 4 * lg + k <= lr ? __builtin_fmaf(gt[k], e, dk[k]) : 0.f;
+              const float e = __builtin_amdgcn_exp2f(tt - sl[k]);
+              float m = __builtin_fmaf(gt[k] * sd[k], e, dk[k]);
+              asm volatile("" : "+v"(m));   // formed by all lanes, without a branch around it
+              v[4 * i + k] = 4 * lg + k <= lr ? m : 0.f;
             }
           }
 #pragma unroll
@@ -561,7 +581,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
             for (int r = 0; r < 4; ++r) acc[i][pt][r] *= f;
 #pragma unroll
           for (int kk = 0; kk <= i / 2; ++kk) {
-            const Split m = split8_scaled(v + 8 * kk, one);
+            const Split m = split8(v + 8 * kk, one);
 #pragma unroll
             for (int pt = 0; pt < 2; ++pt) acc[i][pt] = mfma(join(xf[pt][2 * kk], xf[pt][2 * kk + 1]), m.hi, acc[i][pt]);
 #pragma unroll
@@ -635,7 +655,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
             v[i] = (float)xf[pt][2 * kk][i] * w0[i];
             v[4 + i] = (float)xf[pt][2 * kk + 1][i] * w1[i];
           }
-          f[pt] = split8_scaled(v, one);
+          f[pt] = split8(v, one);
         }
         const uint16_t* br4 = bt + (32 * kk + 4 * lg + (lr >> 2)) * kPitchB + 4 * (lr & 3);
 #pragma unroll
