@@ -54,10 +54,11 @@ struct ChunkShared {
 struct Segments {
   int64_t tokens;     // of a segment, a multiple of kChunk
   int count;
-  // carries of rows that go on past their first segment, [count, batch, H, P,
-  // 128]: 0 the row's first carry (the pool's own is overwritten by the last
-  // segment while others still start), 1 the carry after segment 0, q > 1 what
-  // segment q - 1 adds to a zero carry; and the decay over segment q - 1
+  // For rows that go on past their first segment, [count, batch, H, P, 128]:
+  // 0 the row's first carry (the pool's own is overwritten by the last segment
+  // while others still start), q > 0 first what segment q - 1 adds to a zero
+  // carry, then (k_full_join) the carry before segment q; and the decay over
+  // segment q - 1.
   float* state;
   float* decay;       // [count, batch, H]
 };
@@ -217,21 +218,15 @@ __device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
 }
 // A workgroup steps four blocks of 64 columns (a head's channels) of one
 // group, two waves each, over one segment of one batch row's tokens.  OUT:
-// readouts and the pool's carry; else the segment's end for the segments
-// after it.
+// readouts and the pool's carry; else what the segment adds to a zero carry.
 template <bool ALIGNED, bool OUT>
 __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg) {
   __shared__ ChunkShared s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave >> 1, half = wave & 1;
   const int lr = lane & 15, lg = lane >> 4;
-  const int64_t hpg = a.H / a.G, per_head = (a.P + 63) / 64, blocks = (hpg * per_head + 3) / 4;
-  int64_t id = blockIdx.x;
-  const int64_t blk = id % blocks;
-  id /= blocks;
-  const int64_t g = id % a.G;
-  id /= a.G;
-  const int64_t b = id % a.batch;
-  const int64_t seg = id / a.batch;
+  const int hpg = (int)(a.H / a.G), per_head = (int)((a.P + 63) / 64), blocks = (hpg * per_head + 3) / 4;
+  const int g = blockIdx.x / blocks, blk = blockIdx.x - g * blocks;
+  const int64_t b = blockIdx.y, seg = blockIdx.z;
 
   const int64_t slot = full_slot(a, b);
   const int64_t len = slot < 0 ? 0 : full_length(a, b);
@@ -240,7 +235,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   if (!OUT && len <= t1) return;                                   // no later segment reads this one
 
   // this pair's head and columns (idle past the group's last block)
-  const int64_t unit = blk * 4 + pair;
+  const int unit = blk * 4 + pair;
   const bool live = unit < hpg * per_head;
   const int64_t h = g * hpg + (live ? unit / per_head : 0), pc = (live ? unit % per_head : 0) * 64;
   const int64_t cols = live ? (a.P - pc < 64 ? a.P - pc : 64) : 0;
@@ -254,39 +249,6 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   }
   if (n == 0) return;
 
-  // the carry: S[16 nt + 4 lg + i][column] as s_[nt][pt][i], 2^-eS times its value
-  f32x4 st[8][2];
-  int eS = 0;
-#pragma unroll
-  for (int pt = 0; pt < 2; ++pt) {
-    const int64_t p = pw + 16 * pt;
-    const bool in = p < cols;
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    auto row = [&](const float* base, int64_t at) { return base + ((at * a.H + h) * a.P + pc + p) * 128 + 4 * lg; };
-    const int64_t per = a.batch;
-    // the row's only segment, or the first of the states' pass: the pool's carry
-    const bool from_pool = seg == 0 && (!OUT || len <= t1);
-    const float* src = from_pool ? row(a.state, slot) : row(sg.state, (seg ? per : 0) + b);
-    const bool read = in && (OUT || seg == 0);
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) st[nt][pt] = read ? *(const f32x4*)(src + 16 * nt) : zero;
-    if (!OUT && seg == 0 && in) {
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) *(f32x4*)(const_cast<float*>(row(sg.state, b)) + 16 * nt) = st[nt][pt];
-    }
-    if (OUT) {
-      for (int64_t q = 2; q <= seg; ++q) {
-        const float d = sg.decay[(q * per + b) * a.H + h];
-        const float* add = row(sg.state, q * per + b);
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const f32x4 v = in ? *(const f32x4*)(add + 16 * nt) : zero;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st[nt][pt][i] = __builtin_fmaf(st[nt][pt][i], d, v[i]);
-        }
-      }
-    }
-  }
   const float av = a.A[h], dh = load_param(a.D, a.d_f32, (int)h), bias = load_param(a.dt_bias, a.db_f32, (int)h);
   double seg_log = 0.0;   // the segment's decay so far, as a power of two
 
@@ -384,6 +346,22 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     }
   };
 
+  load_chunk(0, 0);
+
+  // the carry: S[16 nt + 4 lg + i][column] as st[nt][pt][i], 2^-eS times its value
+  f32x4 st[8][2];
+  int eS = 0;
+  {
+    // the row's only segment: the pool's own carry
+    const float* base = seg == 0 && len <= t1 ? a.state + slot * a.H * a.P * 128 : sg.state + (seg * a.batch + b) * a.H * a.P * 128;
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt) {
+      const float* src = base + (h * a.P + pc + pw + 16 * pt) * 128 + 4 * lg;
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+        st[nt][pt] = OUT && pw + 16 * pt < cols ? *(const f32x4*)(src + 16 * nt) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
   float one = 1.0f;   // keeps the halves' differences mixed-precision fmas
   asm volatile("" : "+s"(one));
   uint32_t yoff[2];
@@ -406,7 +384,6 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   smax = wave_max(smax);
   int eb = exponent_of(smax) + 1;
 
-  load_chunk(0, 0);
   store_chunk(0, 0);
   __syncthreads();
 
@@ -687,6 +664,39 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   }
 }
 
+// The carries before each segment, of rows of more than one: a running fma over
+// the segments' additions, four values a thread, all of a thread's loads in
+// flight.
+__global__ __launch_bounds__(256) void k_full_join(FullArgs a, Segments sg) {
+  const int64_t b = blockIdx.y, i = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = a.H * a.P * 32;
+  if (i >= per_row) return;
+  const int64_t slot = full_slot(a, b), len = slot < 0 ? 0 : full_length(a, b);
+  const int64_t started = (len + sg.tokens - 1) / sg.tokens;
+  if (started < 2) return;
+  const int64_t h = i / (a.P * 32);
+  f32x4 cur = *(const f32x4*)(a.state + (slot * per_row + i) * 4);
+  f32x4* at = (f32x4*)sg.state + b * per_row + i;
+  const int64_t step = a.batch * per_row;
+  at[0] = cur;
+  for (int64_t q0 = 1; q0 < started; q0 += 8) {
+    f32x4 v[8];
+    float d[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (q0 + k < started) {
+        v[k] = at[(q0 + k) * step];
+        d[k] = sg.decay[((q0 + k) * a.batch + b) * a.H + h];
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (q0 + k < started) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cur[e] = __builtin_fmaf(cur[e], d[k], v[k][e]);
+        at[(q0 + k) * step] = cur;
+      }
+  }
+}
+
 }  // namespace m2r
 
 using namespace m2r;
@@ -710,7 +720,7 @@ int64_t full_chunks_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, in
 
 hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t stream) {
   Segments sg = full_segments(a.batch, a.L, a.H, a.P, a.G);
-  const int64_t hpg = a.H / a.G, blocks = (hpg * ((a.P + 63) / 64) + 3) / 4, groups = blocks * a.G * a.batch;
+  const int64_t hpg = a.H / a.G, blocks = (hpg * ((a.P + 63) / 64) + 3) / 4;
   if (sg.count > 1) {
     sg.state = (float*)workspace;
     sg.decay = sg.state + (int64_t)sg.count * a.batch * a.H * a.P * 128;
@@ -722,14 +732,16 @@ hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t st
                        (((uintptr_t)a.x | (uintptr_t)a.Bm | (uintptr_t)a.Cm | (uintptr_t)a.y) & 15) == 0 &&
                        a.xs_l >= dense && a.bs_l >= a.G * 128 && a.cs_l >= a.G * 128 && a.ds_l >= a.H &&
                        a.xs_l < far && a.bs_l < far && a.cs_l < far && a.ds_l < far;
-  if (groups * sg.count > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 block(512);
+  dim3 grid((unsigned)(blocks * a.G), (unsigned)a.batch, (unsigned)sg.count);
   if (sg.count > 1) {
-    const dim3 grid((unsigned)(groups * (sg.count - 1)));
+    grid.z = sg.count - 1;
     if (aligned) hipLaunchKernelGGL((k_full_chunks<true, false>), grid, block, 0, stream, a, sg);
     else hipLaunchKernelGGL((k_full_chunks<false, false>), grid, block, 0, stream, a, sg);
+    const dim3 join((unsigned)((a.H * a.P * 32 + 255) / 256), (unsigned)a.batch);
+    hipLaunchKernelGGL(k_full_join, join, dim3(256), 0, stream, a, sg);
+    grid.z = sg.count;
   }
-  const dim3 grid((unsigned)(groups * sg.count));
   if (aligned) hipLaunchKernelGGL((k_full_chunks<true, true>), grid, block, 0, stream, a, sg);
   else hipLaunchKernelGGL((k_full_chunks<false, true>), grid, block, 0, stream, a, sg);
   return hipGetLastError();
