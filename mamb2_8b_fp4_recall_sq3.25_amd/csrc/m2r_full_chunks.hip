@@ -17,38 +17,43 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 
 constexpr int kChunk = 64;
-// LDS row pitches in binary16 elements.  C is read as 16 bytes of 16 rows (a
-// pitch of 4 banks past a multiple of 64 puts them on all banks once), B
-// by transposing reads of 4 rows by 32 bytes per 16 lanes (8 banks apart).
-// x comes by direct transfers (64 lanes x 16 bytes in a row), so its rows are
-// dense and their 16-byte pieces are exchanged instead: the piece of columns
-// 8 c .. 8 c + 7 of row r stands at c ^ x_turn(r), which spreads the 4 rows x
-// 32 bytes that 16 lanes read over all banks.
-constexpr int kPitchC = 136, kPitchB = 144, kPitchX = 64;
+// B, C and x come by direct transfers (64 lanes x 16 bytes in a row), so their
+// rows in LDS are dense, and their 16-byte pieces are exchanged instead, so that
+// the rows that one read touches stand on different banks: piece p of row r is
+// at p ^ bc_turn(r) (16 rows x 16 bytes, or transposing 8 rows x 32 bytes) or
+// p ^ x_turn(r) (rows of half the length).
+constexpr int kRowB = 128, kRowX = 64;
+__device__ __forceinline__ int bc_turn(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
+__device__ __forceinline__ int bc_at(int row, int n) { return row * kRowB + 8 * ((n >> 3) ^ bc_turn(row)) + (n & 7); }
 __device__ __forceinline__ int x_turn(int row) { return ((row >> 1) & 3) << 1; }
-__device__ __forceinline__ int x_at(int row, int col) { return row * kPitchX + 8 * ((col >> 3) ^ x_turn(row)) + (col & 7); }
+__device__ __forceinline__ int x_at(int row, int col) { return row * kRowX + 8 * ((col >> 3) ^ x_turn(row)) + (col & 7); }
 
 // What the heads' tokens need besides B, C and x.  l is the running sum of
 // A dt log2(e) over the chunk, r_j its value at the last token of the 16-token
 // tile j; powers are of two.
+template <bool OUT>
 struct ChunkScalars {
-  float lh[kChunk], ll[kChunk];   // l as a sum of two binary32
-  float lt[kChunk];               // l - r of the tile before
-  float dt[kChunk];
-  float ws[kChunk];               // dt 2^(r_tile - l)
-  float w[kChunk];                // dt 2^(l_63 - l)
-  float el[kChunk];               // 2^l
+  static constexpr int kOut = OUT ? kChunk : 1;
+  float lh[kOut], ll[kOut];       // l as a sum of two binary32
+  float lt[kOut];                 // l - r of the tile before
+  float dt[kOut];
+  float ws[kOut];                 // dt 2^(r_tile - l)
+  float el[kOut];                 // 2^l
+  alignas(16) float w[kChunk];    // dt 2^(l_63 - l)
   float tot, wmax, dtmax, unused; // 2^l_63, the largest w and dt
 };
 
+// `Ahead`: chunks on their way besides the one in work.
+template <bool OUT>
 struct ChunkShared {
-  uint16_t c[kChunk * kPitchC];          // each 32 coordinates in the order of the carry's fragments
-  uint16_t b[2][kChunk * kPitchB];
-  uint16_t x[2][4][kChunk * kPitchX];
-  f32x4 scores[10][64];                  // (C B^T) tiles on and below the diagonal, by lane
-  ChunkScalars h[2][4];
+  static constexpr int kAhead = OUT ? 1 : 2, kBuffers = kAhead + 1;
+  uint16_t c[OUT ? kBuffers : 1][OUT ? kChunk * kRowB : 8];
+  uint16_t b[kBuffers][kChunk * kRowB];
+  uint16_t x[kBuffers][4][kChunk * kRowX];
+  uint32_t dt[kBuffers][4][kChunk];      // as loaded, one value a word
+  f32x4 scores[OUT ? 10 : 1][64];        // (C B^T) tiles on and below the diagonal, by lane
+  ChunkScalars<OUT> h[2][4];
   float gmax[8];                         // largest score, by wave
-  uint32_t bmax[2][8];                   // largest magnitude of B as binary16, by wave
 };
 
 struct Segments {
@@ -155,10 +160,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const uint16_t* p,
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, bytes, 0x00020000);
 }
 
-// Direct transfer of 16 bytes a lane to lds + 16 lane, from `off` into the
-// buffer; zeros for offsets outside.  The caller waits (wait_vmcnt).
+// Direct transfers of 16 bytes a lane to lds + 16 lane, or of two to a word at
+// lds + 4 lane, from `off` into the buffer; zeros for offsets outside.  The
+// compiler does not count them: the caller waits (wait_vmcnt).
 __device__ __forceinline__ void buffer_to_lds(u32x4 rsrc, uint32_t off, uint32_t lds) {
   asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+__device__ __forceinline__ void buffer_to_lds_u16(u32x4 rsrc, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc),
                "{m0}"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
 }
@@ -221,7 +232,8 @@ __device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
 // readouts and the pool's carry; else what the segment adds to a zero carry.
 template <bool ALIGNED, bool OUT>
 __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg) {
-  __shared__ ChunkShared s;
+  __shared__ ChunkShared<OUT> s;
+  constexpr int kAhead = ChunkShared<OUT>::kAhead, kBuffers = ChunkShared<OUT>::kBuffers;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave >> 1, half = wave & 1;
   const int lr = lane & 15, lg = lane >> 4;
   const int hpg = (int)(a.H / a.G), per_head = (int)((a.P + 63) / 64), blocks = (hpg * per_head + 3) / 4;
@@ -252,101 +264,82 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   const float av = a.A[h], dh = load_param(a.D, a.d_f32, (int)h), bias = load_param(a.dt_bias, a.db_f32, (int)h);
   double seg_log = 0.0;   // the segment's decay so far, as a power of two
 
-  // the loads of a chunk: B and C two, x four 16-byte pieces a thread
-  u32x4 rb[2], rc[2], rx[ALIGNED ? 1 : 4];
-  uint16_t rdt = 0;
-  // x: transfer k of a wave fills rows 16 k + 8 half ... + 7, the lane's piece
-  // of them at its turned place
-  const int br = tid >> 4, bpart = tid & 15, xr = 8 * half + (lane >> 3), xpart = (lane & 7) ^ x_turn(lane >> 3);
+  // the loads of a chunk: B and C two, x four 16-byte pieces a thread, dt.
+  // Transfer k of a wave fills rows 32 k + 4 wave ... + 3 of B and C, rows
+  // 16 k + 8 half ... + 7 of its pair's x, the lane's piece at its turned place.
+  const int br = 4 * wave + (lane >> 4), bpart = (lane & 15) ^ bc_turn(br);
+  const int xr = 8 * half + (lane >> 3), xpart = (lane & 7) ^ x_turn(lane >> 3);
   const uint16_t *bp = a.Bm + b * a.bs_b + t0 * a.bs_l + g * 128, *cp = a.Cm + b * a.cs_b + t0 * a.cs_l + g * 128;
   const uint16_t *xp = a.x + b * a.xs_b + t0 * a.xs_l + h * a.P + pc, *dp = a.dt + b * a.ds_b + t0 * a.ds_l + h;
   const int xcols = (int)cols - 8 * xpart;
   const uint32_t xoff = xcols > 0 ? (uint32_t)(2 * (xr * a.xs_l + 8 * xpart)) : kOutside;
   const uint32_t boff = (uint32_t)(2 * (br * a.bs_l + 8 * bpart)), coff = (uint32_t)(2 * (br * a.cs_l + 8 * bpart));
+  const uint32_t doff = (uint32_t)(2 * lane * a.ds_l);
   // the wave that prepares its pair's scalars: one of the two on each SIMD
   const bool scalars = half == pair >> 1;
-  auto load_chunk = [&](int64_t c0, int par) {   // tokens t0 + c0 ...: the pointers stand there
+  auto load_chunk = [&](int64_t c0, int buf) {   // tokens t0 + c0 ...
     const int left = (int)(n - c0 < kChunk ? n - c0 : kChunk);
+    const uint16_t *bs = bp + c0 * a.bs_l, *cs = cp + c0 * a.cs_l, *xs = xp + c0 * a.xs_l, *ds = dp + c0 * a.ds_l;
     if constexpr (ALIGNED) {
-      const auto bb = rows_buffer(bp, a.bs_l, left, 128), cb = rows_buffer(cp, a.cs_l, left, 128);
-      const auto db = rows_buffer(dp, a.ds_l, left, 1);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        rb[k] = __builtin_amdgcn_raw_buffer_load_b128(bb, boff + (uint32_t)(64 * k * a.bs_l), 0, 0);
-        if (OUT) rc[k] = __builtin_amdgcn_raw_buffer_load_b128(cb, coff + (uint32_t)(64 * k * a.cs_l), 0, 0);
-      }
-      if (scalars) rdt = __builtin_amdgcn_raw_buffer_load_b16(db, (uint32_t)(2 * lane * a.ds_l), 0, 0);
-      const u32x4 xb = rows_resource(xp, a.xs_l, left, (int)cols);
+      const u32x4 xb = rows_resource(xs, a.xs_l, left, (int)cols), bb = rows_resource(bs, a.bs_l, left, 128);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        buffer_to_lds(xb, xoff + (uint32_t)(32 * k * a.xs_l), lds_address(s.x[par][pair] + (16 * k + 8 * half) * kPitchX));
+        buffer_to_lds(xb, xoff + (uint32_t)(32 * k * a.xs_l), lds_address(s.x[buf][pair] + (16 * k + 8 * half) * kRowX));
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        buffer_to_lds(bb, boff + (uint32_t)(64 * k * a.bs_l), lds_address(s.b[buf] + (32 * k + 4 * wave) * kRowB));
+      if constexpr (OUT) {
+        const u32x4 cb = rows_resource(cs, a.cs_l, left, 128);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          buffer_to_lds(cb, coff + (uint32_t)(64 * k * a.cs_l), lds_address(s.c[buf] + (32 * k + 4 * wave) * kRowB));
+      }
+      if (scalars) buffer_to_lds_u16(rows_resource(ds, a.ds_l, left, 1), doff, lds_address(s.dt[buf][pair]));
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int r = 32 * k + br, in = r < left ? 8 : 0;
-        rb[k] = load8(bp + r * a.bs_l + 8 * bpart, in);
-        if (OUT) rc[k] = load8(cp + r * a.cs_l + 8 * bpart, in);
+        *(u32x4*)(s.b[buf] + (32 * k + 4 * wave) * kRowB + 8 * lane) = load8(bs + r * a.bs_l + 8 * bpart, in);
+        if constexpr (OUT) *(u32x4*)(s.c[buf] + (32 * k + 4 * wave) * kRowB + 8 * lane) = load8(cs + r * a.cs_l + 8 * bpart, in);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        rx[k] = load8(xp + (16 * k + xr) * a.xs_l + 8 * xpart, 16 * k + xr < left ? xcols : 0);
-      if (scalars) rdt = lane < left ? dp[lane * a.ds_l] : 0;
+        *(u32x4*)(s.x[buf][pair] + (16 * k + 8 * half) * kRowX + 8 * lane) =
+            load8(xs + (16 * k + xr) * a.xs_l + 8 * xpart, 16 * k + xr < left ? xcols : 0);
+      if (scalars) s.dt[buf][pair][lane] = lane < left ? ds[lane * a.ds_l] : 0u;
     }
-    bp += kChunk * a.bs_l;
-    cp += kChunk * a.cs_l;
-    xp += kChunk * a.xs_l;
-    dp += kChunk * a.ds_l;
   };
-  // the loaded chunk into LDS (B, x and the scalars: buffer `par`)
-  auto store_chunk = [&](int64_t c0, int par) {
-    uint32_t bm = 0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = 32 * k + br;
-      *(u32x4*)(s.b[par] + r * kPitchB + 8 * bpart) = rb[k];
-      bm = max_magnitudes(bm, rb[k]);
-      if (OUT) {
-        // coordinates 32 kk + 16 T + 4 q + i of a row stand at 32 kk + 8 q + 4 T + i
-        const int kk = bpart >> 2, T = (bpart >> 1) & 1, q = 2 * (bpart & 1);
-        uint16_t* d = s.c + r * kPitchC + 32 * kk + 8 * q + 4 * T;
-        *(u32x2*)d = u32x2{rc[k][0], rc[k][1]};
-        *(u32x2*)(d + 8) = u32x2{rc[k][2], rc[k][3]};
-      }
-    }
-    if constexpr (ALIGNED) {
-      wait_vmcnt<0>();   // the transfers have landed
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) *(u32x4*)(s.x[par][pair] + (16 * k + 8 * half) * kPitchX + 8 * lane) = rx[k];
-    }
-    bm = wave_max_half(bm);
-    if (lane == 0) s.bmax[par][wave] = bm;
-    if (scalars) {   // lane = token
-      ChunkScalars& hs = s.h[par][pair];
-      const float dt = c0 + lane < n ? full_dt(h2f(rdt) + bias) : 0.f;
-      const double l = scan_add64((double)av * (double)dt * 1.4426950408889634);
-      const double last = lane64(l, 63), tile = dpp_row_last64(l);
-      const double e0 = lane64(l, 15), e1 = lane64(l, 31), e2 = lane64(l, 47);
-      const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e1 : e2));
-      const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - l));
+  // the scalars of a chunk whose dt this wave has loaded
+  auto prepare = [&](int64_t c0, int buf, int par) {   // lane = token
+    ChunkScalars<OUT>& hs = s.h[par][pair];
+    const float dt = c0 + lane < n ? full_dt(h2f((uint16_t)s.dt[buf][pair][lane]) + bias) : 0.f;
+    const double l = scan_add64((double)av * (double)dt * 1.4426950408889634);
+    const double last = lane64(l, 63), tile = dpp_row_last64(l);
+    const double e0 = lane64(l, 15), e1 = lane64(l, 31), e2 = lane64(l, 47);
+    const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e1 : e2));
+    const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - l));
+    hs.w[lane] = w;
+    if constexpr (OUT) {
       hs.lh[lane] = lh;
       hs.ll[lane] = __builtin_fabsf(lh) < __builtin_inff() ? (float)(l - (double)lh) : 0.f;
       hs.lt[lane] = (float)(l - before);
       hs.dt[lane] = dt;
       hs.ws[lane] = dt * __builtin_amdgcn_exp2f((float)(tile - l));
-      hs.w[lane] = w;
       hs.el[lane] = __builtin_amdgcn_exp2f(lh);
-      const float wm = wave_max(w), dm = wave_max(dt);
-      if (lane == 0) {
-        hs.tot = __builtin_amdgcn_exp2f((float)last);
-        hs.wmax = wm;
-        hs.dtmax = dm;
-      }
-      seg_log += last;
     }
+    const float wm = wave_max(w), dm = wave_max(dt);
+    if (lane == 0) {
+      hs.tot = __builtin_amdgcn_exp2f((float)last);
+      hs.wmax = wm;
+      hs.dtmax = dm;
+    }
+    seg_log += last;
   };
 
-  load_chunk(0, 0);
+  const int64_t chunks = (n + kChunk - 1) / kChunk;
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (k < chunks) load_chunk(k * kChunk, k);
 
   // the carry: S[16 nt + 4 lg + i][column] as st[nt][pt][i], 2^-eS times its value
   f32x4 st[8][2];
@@ -362,6 +355,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         st[nt][pt] = OUT && pw + 16 * pt < cols ? *(const f32x4*)(src + 16 * nt) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
+  float sbound = 0.f;   // a bound of the carry's magnitudes
+  const int turned_at = bc_at(4 * lg + (lr >> 2), 4 * (lr & 3));   // for transposing reads of B
   float one = 1.0f;   // keeps the halves' differences mixed-precision fmas
   asm volatile("" : "+s"(one));
   uint32_t yoff[2];
@@ -370,30 +365,44 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     const int p = 32 * half + 16 * pt + 4 * lg;
     yoff[pt] = p < cols ? (uint32_t)(2 * (lr * a.H * a.P + p)) : kOutside;
   }
-  // a bound of the carry's magnitudes, 2^eb
-  float smax = 0.f;
+  // the carry's largest magnitude; an infinite channel must set no scale
+  auto largest = [&]() {
+    float m = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < 8; ++nt)
+    for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt)
+      for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = __builtin_fabsf(st[nt][pt][i]);
-        smax = __builtin_fmaxf(smax, v < __builtin_inff() ? v : 0.f);   // an infinite channel sets no scale
-      }
-  smax = wave_max(smax);
-  int eb = exponent_of(smax) + 1;
+        for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(st[nt][pt][i]));
+    m = wave_max(m);
+    if (!(m < __builtin_inff())) {
+      m = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = __builtin_fabsf(st[nt][pt][i]);
+            m = __builtin_fmaxf(m, v < __builtin_inff() ? v : 0.f);
+          }
+      m = wave_max(m);
+    }
+    return m;
+  };
 
-  store_chunk(0, 0);
+  wait_vmcnt<0>();   // the transfers have landed
+  if (scalars) prepare(0, 0, 0);
   __syncthreads();
 
-  const int64_t chunks = (n + kChunk - 1) / kChunk;
+  int buf = 0;
   for (int64_t ch = 0; ch < chunks; ++ch) {
     const int64_t c0 = ch * kChunk;
-    const int par = (int)(ch & 1);
-    const ChunkScalars& hs = s.h[par][pair];
-    const uint16_t *xt = s.x[par][pair], *bt = s.b[par];
-    if (ch + 1 < chunks) load_chunk(c0 + kChunk, par ^ 1);
+    const int par = (int)(ch & 1), next = buf + 1 < kBuffers ? buf + 1 : 0;
+    const ChunkScalars<OUT>& hs = s.h[par][pair];
+    const uint16_t *xt = s.x[buf][pair], *bt = s.b[buf], *ct = s.c[OUT ? buf : 0];
+    const bool more = ch + kAhead < chunks;   // a chunk to be loaded: into the buffer that the last one left
+    if (more) load_chunk(c0 + kAhead * kChunk, buf + kAhead < kBuffers ? buf + kAhead : buf + kAhead - kBuffers);
 
     // x fragments: tokens 16 T + 4 lg + r of column pw + 16 pt
     f16x4 xf[2][4];
@@ -402,11 +411,18 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
       for (int T = 0; T < 4; ++T) {
-        xf[pt][T] = read_transposed(xt + 16 * T * kPitchX + x_at(4 * lg + (lr >> 2), 32 * half + 16 * pt + 4 * (lr & 3)));
+        xf[pt][T] = read_transposed(xt + 16 * T * kRowX + x_at(4 * lg + (lr >> 2), 32 * half + 16 * pt + 4 * (lr & 3)));
         xm = max_magnitudes(xm, __builtin_bit_cast(u32x2, xf[pt][T]));
       }
     xm = wave_max_half(xm);
 
+    // 8 coordinates of row 16 tile + lr of B or C in the order of the carry's
+    // fragments: 32 kk + 4 lg + ..., and 16 further
+    const int row_at = bc_at(lr, 4 * lg);
+    auto row_fragment = [&](const uint16_t* m, int tile, int kk) {
+      const uint16_t* r = m + 16 * tile * kRowB;
+      return join(*(const f16x4*)(r + (row_at ^ (32 * kk))), *(const f16x4*)(r + (row_at ^ (32 * kk + 16))));
+    };
     const bool odd = OUT && xm >= 0x7c00u;
     if constexpr (OUT) {
       // ---- C B^T, the same for all heads: two waves without scalars two tiles, the others one.
@@ -415,10 +431,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       auto score_tile = [&](int at) {
         const int i = at < 1 ? 0 : (at < 3 ? 1 : (at < 6 ? 2 : 3)), j = at - i * (i + 1) / 2;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        const uint16_t *cr = s.c + (16 * i + lr) * kPitchC + 8 * lg, *r = bt + (16 * j + lr) * kPitchB + 4 * lg;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          acc = mfma(join(*(const f16x4*)(r + 32 * kk), *(const f16x4*)(r + 32 * kk + 16)), *(const f16x8*)(cr + 32 * kk), acc);
+        for (int kk = 0; kk < 4; ++kk) acc = mfma(row_fragment(bt, j, kk), row_fragment(ct, i, kk), acc);
         s.scores[at][lane] = acc;
 #pragma unroll
         for (int k = 0; k < 4; ++k) gm = __builtin_fmaxf(gm, __builtin_fabsf(acc[k]));
@@ -433,7 +447,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt) acc[i][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int kS = 14 - eb > 100 ? 100 : 14 - eb;
+      const float smax = largest();
+      sbound = __builtin_ldexpf(smax, -eS);
+      const int kS = 13 - exponent_of(smax) > 100 ? 100 : 13 - exponent_of(smax);   // in units of st
       if (odd) {
         // A non-finite x must not reach earlier tokens, which the matrix
         // products would let it do (0 * inf): this chunk token by token.
@@ -454,8 +470,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
             for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float bv = h2f(bt[t * kPitchB + 16 * nt + 4 * lg + i]);
-                const float cv = h2f(s.c[t * kPitchC + 32 * (nt >> 1) + 8 * lg + 4 * (nt & 1) + i]);
+                const float bv = h2f(bt[bc_at(t, 16 * nt + 4 * lg + i)]);
+                const float cv = h2f(ct[bc_at(t, 16 * nt + 4 * lg + i)]);
                 st[nt][pt][i] = __builtin_fmaf(st[nt][pt][i], decay, in * bv);
                 acc = __builtin_fmaf(st[nt][pt][i], cv, acc);
               }
@@ -464,22 +480,11 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
               a.y[((b * a.L + t0 + c0 + t) * a.H + h) * a.P + pc + pw + 16 * pt] = f2h(__builtin_fmaf(xv, dh, acc));
           }
         }
-        smax = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = __builtin_fabsf(st[nt][pt][i]);
-              smax = __builtin_fmaxf(smax, v < __builtin_inff() ? v : 0.f);
-            }
-        smax = wave_max(smax);
-        eb = exponent_of(smax) + 1;
         eS = 0;
+        wait_vmcnt<0>();   // the next chunk, before these stores
       } else {
         // ---- S C_t: rows = columns of x, columns = tokens
-        const float ss = pow2(kS - eS);
+        const float ss = pow2(kS);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           Split f[2];
@@ -492,7 +497,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
           f16x8 cf[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) cf[i] = *(const f16x8*)(s.c + (16 * i + lr) * kPitchC + 32 * kk + 8 * lg);
+          for (int i = 0; i < 4; ++i) cf[i] = row_fragment(ct, i, kk);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
 #pragma unroll
           for (int k = 4 * i + 4; k < 16; ++k) v[k] = 0.f;
-          const float f = __builtin_ldexpf(hs.el[16 * i + lr], km - kS);
+          const float f = __builtin_ldexpf(hs.el[16 * i + lr], km - kS - eS);
 #pragma unroll
           for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
@@ -590,27 +595,19 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       }
     }
 
-    // ---- the carry after the chunk.  The bound: the decayed carry's and 64
-    // products', each factor below twice its power of two.
+    // ---- the carry after the chunk: x w 2^e1 below 2^15, unless a bound of
+    // the carry (the decayed one and 64 products) would leave binary32.
     if (!odd) {
-      uint32_t bm8 = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) bm8 = bm8 > s.bmax[par][k] ? bm8 : s.bmax[par][k];
       const float tot = hs.tot, wmax = hs.wmax;
-      const int ex = xm >= 0x7c00u ? 16 : exponent_of(h2f((uint16_t)xm)), ebm = bm8 >= 0x7c00u ? 16 : exponent_of(h2f((uint16_t)bm8));
-      const int old = eb + (tot < __builtin_inff() ? exponent_of(tot) + 1 : 128);
-      int add = ex + exponent_of(wmax) + ebm + 9;
-      if (!(wmax < __builtin_inff())) add = 128;
-      eb = (old > add ? old : add) + 1;
-      eb = eb > 128 ? 128 : (eb < -126 ? -126 : eb);
-      // x w 2^e1 below 2^15, unless the carry would leave binary32
+      const float xmax = xm >= 0x7c00u ? 65536.0f : h2f((uint16_t)xm);
+      sbound = __builtin_fmaf(sbound, tot, 64.0f * 65504.0f * xmax * wmax);
+      const int eb = sbound < 0x1p120f ? exponent_of(sbound) : 121;
       int e1 = eS;
       if (xm && wmax > 0.f && wmax < __builtin_inff()) {
-        e1 = 13 - ex - exponent_of(wmax);
-        e1 = e1 < 110 - eb ? e1 : 110 - eb;
+        e1 = 13 - exponent_of(xmax) - exponent_of(wmax);
+        e1 = e1 < 120 - eb ? e1 : 120 - eb;
         e1 = e1 < 110 ? (e1 > -110 ? e1 : -110) : 110;
       }
-      eb = __builtin_amdgcn_readfirstlane(eb);
       e1 = __builtin_amdgcn_readfirstlane(e1);
       const float keep = __builtin_ldexpf(tot, e1 - eS), sx = pow2(e1);
       eS = e1;
@@ -634,19 +631,31 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
           f[pt] = split8(v, one);
         }
-        const uint16_t* br4 = bt + (32 * kk + 4 * lg + (lr >> 2)) * kPitchB + 4 * (lr & 3);
+        const uint16_t* r = bt + 32 * kk * kRowB;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-          const f16x8 bf = join(read_transposed(br4 + 16 * nt), read_transposed(br4 + 16 * kPitchB + 16 * nt));
+          const f16x8 bf = join(read_transposed(r + (turned_at ^ (16 * nt))), read_transposed(r + 16 * kRowB + (turned_at ^ (16 * nt))));
 #pragma unroll
           for (int pt = 0; pt < 2; ++pt) st[nt][pt] = mfma(bf, f[pt].hi, st[nt][pt]);
 #pragma unroll
           for (int pt = 0; pt < 2; ++pt) st[nt][pt] = mfma(bf, f[pt].lo, st[nt][pt]);
         }
       }
+      // The next chunk has landed: behind its transfers are the 8 stores of
+      // readouts, or the transfers of the chunk after it.
+      if constexpr (ALIGNED) {
+        if constexpr (OUT) {
+          wait_vmcnt<8>();
+        } else {
+          if (!more) wait_vmcnt<0>();
+          else if (scalars) wait_vmcnt<7>();
+          else wait_vmcnt<6>();
+        }
+      }
     }
-    if (ch + 1 < chunks) store_chunk(c0 + kChunk, par ^ 1);
+    if (scalars && ch + 1 < chunks) prepare(c0 + kChunk, next, par ^ 1);
     __syncthreads();
+    buf = next;
   }
 
   if (!OUT || len <= t1) {

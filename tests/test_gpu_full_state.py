@@ -150,6 +150,33 @@ def test_magnitudes(device, scale, dt_shift):
     _check(i, *_scan(i), _reference(i), 130)
 
 
+@pytest.mark.parametrize("batch,tokens", [(200, 8256), (1, 20000)])
+def test_long_memory(device, batch, tokens):
+    """Carries that hardly decay over many chunks, in one segment (many rows)
+    and in several (one row); all batch rows stepped at once in 64 bits."""
+    i = _inputs(device, batch, tokens, heads=1, dim=8, groups=1, seed=41, dt_shift=-3.0)
+    i["A"] = torch.full((1,), -2.0 ** -9, device=device)
+    y, state = _scan(i)
+    v = i["dt"].double() + i["dt_bias"].double()
+    dt = torch.logaddexp(v, torch.zeros_like(v))[..., 0]
+    decay = torch.exp(dt * i["A"].double())
+    s, m = i["state"].double()[:, 0], i["state"].double()[:, 0].abs()
+    eps, worst = (4 * tokens + 256) * 2.0 ** -24, 0.0
+    for t in range(tokens):
+        x, b, c = i["x"][:, t, 0].double(), i["B"][:, t, 0].double(), i["C"][:, t, 0].double()
+        add = (dt[:, t, None] * x)[..., None] * b[:, None]
+        s, m = s * decay[:, t, None, None] + add, m * decay[:, t, None, None] + add.abs()
+        if t % 509 == 0 or t >= tokens - 70:
+            want = (s * c[:, None]).sum(-1) + i["D"].double() * x
+            mag = (m * c[:, None].abs()).sum(-1) + (i["D"].double() * x).abs()
+            over = (y[:, t, 0].double() - want).abs() - want.abs() * 2.0 ** -11 - 2.0 ** -25 - eps * mag
+            assert float(over.max()) <= 0, f"token {t}"
+            worst = max(worst, float(((y[:, t, 0].double() - want).norm() / want.norm())))
+    # the binary16 rounding alone is 2^-12.2 in the mean square
+    assert worst < 2.0 ** -11
+    assert float((state[:, 0].double() - s).norm() / s.norm()) < 2.0 ** -19
+
+
 @pytest.mark.parametrize("key", ["x", "B", "C", "dt"])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_non_finite_inputs_stay_where_they_are(device, key, value):
