@@ -79,11 +79,21 @@ __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
 
 using namespace m2r;
 
-// Calls of this many tokens on take the chunked kernel.
-constexpr int64_t kChunkedFrom = 8;
+// Whether a call of L tokens takes the chunked kernel, whose time hardly
+// depends on L up to 64, or steps token by token.  The step's time is its
+// carries' plus a chain per token; few rows leave the chain bare, so the
+// chunked kernel's fixed cost is made up later.  us per call, step / chunked,
+// at 128 heads of 64: batch 1 12 tokens 15.5 / 18.8, 16 tokens 19.0 / 18.8;
+// batch 4 8 tokens 18.5 / 20.6, 12 tokens 24.0 / 20.5; batch 16 4 tokens
+// 35.7 / 43.7, 6 tokens 44.6 / 43.6; batch 64 4 tokens 134 / 162, 6 tokens
+// 168 / 163, 64 tokens 1,253 / 196.
+static bool full_chunked(int64_t batch, int64_t L, int64_t H, int64_t P) {
+  const int64_t rows = batch * H * P;
+  return L >= (rows <= 16384 ? 16 : (rows <= 65536 ? 10 : 6));
+}
 
 extern "C" int64_t m2r_full_scan_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) {
-  if (batch <= 0 || L < kChunkedFrom || H <= 0 || P <= 0 || G <= 0 || H % G) return 0;
+  if (batch <= 0 || H <= 0 || P <= 0 || G <= 0 || H % G || batch > 65535 || !full_chunked(batch, L, H, P)) return 0;
   return full_chunks_workspace(batch, L, H, P, G);
 }
 
@@ -105,7 +115,8 @@ extern "C" int m2r_full_scan(const void* x, int64_t xs_b, int64_t xs_l, const vo
   FullArgs a{(const uint16_t*)x, (const uint16_t*)dt, xs_b, xs_l, ds_b, ds_l, A, (const uint16_t*)B,
              (const uint16_t*)C, bs_b, bs_l, cs_b, cs_l, D, dt_bias, d_is_f32, db_is_f32, state, pool, slots, lengths,
              (uint16_t*)y, batch, L, H, P, G};
-  if (L >= kChunkedFrom) {
+  // (a grid's second axis holds the batch rows)
+  if (batch <= 65535 && full_chunked(batch, L, H, P)) {
     const int64_t need = full_chunks_workspace(batch, L, H, P, G);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
       return m2r_fail("full scan: workspace too small or not 16-byte aligned");
