@@ -2,8 +2,8 @@
 //   out[m] = half(base[m] + scale[a] up[a] (down[a] x[m])),  a = ids[m],
 // and out[m] = base[m] where ids[m] names no adapter (negative, or not below
 // the number of adapters).  x [M, K], base and out [M, N] binary16 rows,
-// down [n, r, Kp], up [n, N, r] binary16, scale [n] binary32; r a multiple of
-// 8 and Kp = K rounded up to 8, the rest zeros.
+// down [n, r, Kp], up [n, N, r] binary16, scale [n] binary32; r the rank and
+// Kp = K, each rounded up to 8, the rest zeros.
 //
 // Two launches on the matrix cores, rows in tiles of 16.  The first forms the
 // hidden values down x of a tile over a slice of K, in binary32; the second
@@ -35,10 +35,11 @@ struct AdapterArgs {
   float* hidden;        // [slices, M, r]
   int64_t M, K, Kp, N, n;
   int r;
-  int slices;           // of K, `slice` long each (a multiple of 32)
+  int rank;             // r - 7 ... r: a hidden value past it counts as 0, whatever x holds
+  int slices;           // of K, `slice` long each (a multiple of 64)
   int64_t slice;
   int members;          // 16: a workgroup per row that leads its group; 1: a workgroup per tile
-  int64_t span;         // outputs of a wave in the second launch, a multiple of 32
+  int64_t span;         // outputs of a wave in the second launch, a multiple of 64
 };
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
@@ -54,6 +55,17 @@ __device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p, int64_t valid) {
       if (j < valid) v[j] = p[j];
   }
   return __builtin_bit_cast(f16x8, v);
+}
+__device__ __forceinline__ h16x8 load_h16x8(const uint16_t* p) {   // all 8, without a branch
+  h16x8 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// Ranks at ... at + 7 of a row of `up`, zeros from r on.
+__device__ __forceinline__ f16x8 load_ranks(const uint16_t* row, int at, int r) {
+  const h16x8 v = load_h16x8(row + (at < r ? at : 0));
+  const h16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+  return __builtin_bit_cast(f16x8, at < r ? v : zero);
 }
 // The adapter of row m; -1 for none and past the last row.
 __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t m) {
@@ -80,7 +92,7 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
     if (mine < 0 || (group & ((1u << member) - 1))) return;
     todo = group;
   }
-  const int64_t quarter = (a.slice / 32 + 3) / 4 * 32;
+  const int64_t quarter = (a.slice / 64 + 3) / 4 * 64;
   const int64_t s1 = (slice + 1) * a.slice < a.Kp ? (slice + 1) * a.slice : a.Kp;
   const int64_t k0 = slice * a.slice + wave * quarter, k1 = k0 + quarter < s1 ? k0 + quarter : s1;
   const uint16_t* xr = a.x + (m < a.M ? m : a.M - 1) * a.xs;
@@ -98,12 +110,33 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
         const int j = r0 + 16 * t + lr;
         dr[t] = a.down + ((int64_t)cur * a.r + (j < a.r ? j : a.r - 1)) * a.Kp;
       }
-#pragma unroll 4
-      for (int64_t k = k0 + 8 * lg; k < k1 + 8 * lg; k += 32) {
-        const bool in = k < k1;
-        const f16x8 xv = load_f16x8(xr + k, in ? a.K - k : 0);
+      // 64 inputs at a time in two products, the lane's 16 of them neighbours:
+      // the pair of loads covers whole 128-byte lines of a row
+#pragma unroll 2
+      for (int64_t kb = k0; kb < k1; kb += 64) {
+        f16x8 xv[2], dv[2][RT];
+        if (kb + 64 <= k1 && kb + 64 <= a.K) {   // (one answer for the wave)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = mfma16(load_f16x8(dr[t] + k, in ? 8 : 0), xv, acc[t]);
+          for (int u = 0; u < 2; ++u) {
+            const int64_t k = kb + 16 * lg + 8 * u;
+            xv[u] = __builtin_bit_cast(f16x8, load_h16x8(xr + k));
+#pragma unroll
+            for (int t = 0; t < RT; ++t) dv[u][t] = __builtin_bit_cast(f16x8, load_h16x8(dr[t] + k));
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int64_t k = kb + 16 * lg + 8 * u;
+            const bool in = k < k1;
+            xv[u] = load_f16x8(xr + k, in ? a.K - k : 0);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) dv[u][t] = load_f16x8(dr[t] + k, in ? 8 : 0);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) acc[t] = mfma16(dv[u][t], xv[u], acc[t]);
       }
       __syncthreads();
       if (wave) {
@@ -125,18 +158,63 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
   }
 }
 
-// v 2^k as the sum of two binary16.
+// v 2^k as the sum of two binary16: 22 bits of the product's operand, where one
+// alone would round the hidden values to 11.  An infinity's second part is 0.
 __device__ __forceinline__ void split_f16(const float* v, float scale, f16x8& hi, f16x8& lo) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     const f16x2 h = __builtin_convertvector((f32x2{v[j] * scale, v[j + 1] * scale}), f16x2);
+    const float r0 = __builtin_fmaf(v[j], scale, -(float)h[0]), r1 = __builtin_fmaf(v[j + 1], scale, -(float)h[1]);
     const f16x2 l = __builtin_convertvector(
-        (f32x2{__builtin_fmaf(v[j], scale, -(float)h[0]), __builtin_fmaf(v[j + 1], scale, -(float)h[1])}), f16x2);
+        (f32x2{__builtin_isinf(v[j]) ? 0.f : r0, __builtin_isinf(v[j + 1]) ? 0.f : r1}), f16x2);
     hi[j] = h[0];
     hi[j + 1] = h[1];
     lo[j] = l[0];
     lo[j + 1] = l[1];
   }
+}
+
+// The hidden values of row m (where `mine`) in the layout of a product's
+// columns, times 2^k as two binary16; returns 2^-k.
+template <int KS>
+__device__ __forceinline__ float hidden_fragments(const AdapterArgs& a, int64_t m, bool mine, float sc, f16x8* hi, f16x8* lo) {
+  const int lg = (threadIdx.x & 63) >> 4;
+  float v[KS][8], mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+    const int j0 = 32 * k + 8 * lg;
+    if (mine && j0 < a.r) {
+      const float* h = a.hidden + m * a.r + j0;
+      for (int q = 0; q < a.slices; ++q) {
+        const f32x4 u0 = *(const f32x4*)(h + (int64_t)q * a.M * a.r), u1 = *(const f32x4*)(h + (int64_t)q * a.M * a.r + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[k][j] += u0[j];
+          v[k][4 + j] += u1[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[k][j] = j0 + j < a.rank ? v[k][j] * sc : 0.f;
+        mx = __builtin_fmaxf(mx, __builtin_fabsf(v[k][j]));
+      }
+    }
+  }
+  // the row's largest, over its four lanes
+  const int iv = __builtin_bit_cast(int, mx);
+  const auto p = __builtin_amdgcn_permlane16_swap(iv, iv, false, false);
+  mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
+  const int jv = __builtin_bit_cast(int, mx);
+  const auto q = __builtin_amdgcn_permlane32_swap(jv, jv, false, false);
+  mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)q[0]), __builtin_bit_cast(float, (int)q[1]));
+  int e = 14 - (((__builtin_bit_cast(int, mx) >> 23) & 255) - 127);   // the largest below 2^15
+  e = e > 100 ? 100 : e;
+  const float up = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+  for (int k = 0; k < KS; ++k) split_f16(v[k], up, hi[k], lo[k]);
+  return __builtin_ldexpf(1.0f, -e);
 }
 
 // One wave per (MT tiles of 16 rows, span of outputs).  A lane holds row
@@ -202,44 +280,7 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
     float back[MT];
     const float sc = a.scale[cur];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float v[KS][8], mx = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
-        const int j0 = 32 * k + 8 * lg;
-        if (mine[i] && j0 < a.r) {
-          const float* h = a.hidden + (m0 + 16 * i + lr) * a.r + j0;
-          for (int q = 0; q < a.slices; ++q) {
-            const f32x4 u0 = *(const f32x4*)(h + (int64_t)q * a.M * a.r), u1 = *(const f32x4*)(h + (int64_t)q * a.M * a.r + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              v[k][j] += u0[j];
-              v[k][4 + j] += u1[j];
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[k][j] *= sc;
-            mx = __builtin_fmaxf(mx, __builtin_fabsf(v[k][j]));
-          }
-        }
-      }
-      // the row's largest, over its four lanes
-      const int iv = __builtin_bit_cast(int, mx);
-      const auto p = __builtin_amdgcn_permlane16_swap(iv, iv, false, false);
-      mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
-      const int jv = __builtin_bit_cast(int, mx);
-      const auto q = __builtin_amdgcn_permlane32_swap(jv, jv, false, false);
-      mx = __builtin_fmaxf(__builtin_bit_cast(float, (int)q[0]), __builtin_bit_cast(float, (int)q[1]));
-      int e = 14 - (((__builtin_bit_cast(int, mx) >> 23) & 255) - 127);   // the largest below 2^15
-      e = e > 100 ? 100 : e;
-      const float up = __builtin_ldexpf(1.0f, e);
-      back[i] = __builtin_ldexpf(1.0f, -e);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) split_f16(v[k], up, hi[i][k], lo[i][k]);
-    }
+    for (int i = 0; i < MT; ++i) back[i] = hidden_fragments<KS>(a, m0 + 16 * i + lr, mine[i], sc, hi[i], lo[i]);
     const uint16_t* ub = a.up + (int64_t)cur * a.N * a.r;
     // the next 32 outputs' operands are on their way while these are formed
     h16x8 bv[MT], bn[MT];
@@ -248,13 +289,13 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
       const int64_t n = nb + 8 * lg;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        if (mine[i]) bd[i] = __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
+        bd[i] = nb + 32 <= a.N ? load_h16x8(br[i] + n) : __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
         const int64_t row = nb + 8 * (lr >> 2) + 4 * T + (lr & 3);
-        const uint16_t* ur = ub + (row < a.N ? row : a.N - 1) * a.r + 8 * lg;
+        const uint16_t* ur = ub + (row < a.N ? row : a.N - 1) * a.r;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) ud[T][k] = load_f16x8(ur + 32 * k, 32 * k + 8 * lg < a.r ? 8 : 0);
+        for (int k = 0; k < KS; ++k) ud[T][k] = load_ranks(ur, 32 * k + 8 * lg, a.r);
       }
     };
     fetch(n0, bv, uf);
@@ -299,6 +340,8 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
 // Few rows: a workgroup for each row that leads its group, so that groups run
 // side by side; many: a workgroup walks through its tile's groups, mostly one.
 constexpr int64_t kMemberRows = 512;
+// Waves to aim for in the second launch.
+constexpr int64_t kSpanWaves = 8192;
 
 static void adapter_plan(AdapterArgs& a) {
   const int64_t tiles = (a.M + 15) / 16;
@@ -308,7 +351,7 @@ static void adapter_plan(AdapterArgs& a) {
   const int64_t most = (a.Kp + 511) / 512;
   s = s < most ? s : most;
   s = s < 1 ? 1 : (s > 8 ? 8 : s);
-  a.slice = ((a.Kp + s - 1) / s + 31) / 32 * 32;
+  a.slice = ((a.Kp + s - 1) / s + 63) / 64 * 64;
   a.slices = (int)((a.Kp + a.slice - 1) / a.slice);
 }
 
@@ -322,7 +365,7 @@ extern "C" int64_t m2r_adapters_workspace(int64_t M, int64_t K, int64_t N, int64
   a.M = M;
   a.Kp = (K + 7) / 8 * 8;
   adapter_plan(a);
-  return 4 * a.slices * M * r;
+  return 4 * a.slices * M * ((r + 7) / 8 * 8);
 }
 
 extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride,
@@ -332,7 +375,6 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   if (M <= 0 || K <= 0 || N <= 0 || adapters <= 0 || rank <= 0) return m2r_fail("adapters: non-positive shape");
   const int64_t lim = (int64_t)1 << 24;
   if (M > lim || K > lim || N > lim || adapters > lim || rank > 256) return m2r_fail("adapters: size limits");
-  if (rank % 8) return m2r_fail("adapters: the rank must be a multiple of 8");
   for (const void* p : {x, base, down, up, (const void*)scale, (const void*)ids, (const void*)out, (const void*)workspace})
     if (!p) return m2r_fail("adapters: null pointer");
   if (((uintptr_t)down | (uintptr_t)up) & 15) return m2r_fail("adapters: down and up must be 16-byte aligned");
@@ -341,7 +383,7 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
     return m2r_fail("adapters: workspace too small or not 16-byte aligned");
   AdapterArgs a{(const uint16_t*)x, x_stride, (const uint16_t*)base, base_stride, (const uint16_t*)down,
                 (const uint16_t*)up, scale, ids, (uint16_t*)out, out_stride, (float*)workspace, M, K, (K + 7) / 8 * 8, N,
-                adapters, (int)rank};
+                adapters, (int)((rank + 7) / 8 * 8), (int)rank};
   adapter_plan(a);
   const int64_t tiles = (M + 15) / 16;
   if (tiles * a.members * a.slices > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
@@ -354,10 +396,10 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   // two tiles share a pass over `up` where rows are many and the rank small
   const bool wide = a.M > kMemberRows && rank <= 64;
   const int64_t groups = wide ? (M + 31) / 32 : tiles * a.members;
-  int64_t spans = 4096 / groups;
+  int64_t spans = kSpanWaves / groups;
   const int64_t most = (N + 63) / 64;
   spans = spans < 1 ? 1 : (spans < most ? spans : most);
-  a.span = ((N + spans - 1) / spans + 31) / 32 * 32;
+  a.span = ((N + spans - 1) / spans + 63) / 64 * 64;
   spans = (N + a.span - 1) / a.span;
   if ((groups * spans + 3) / 4 > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
   const dim3 up_grid((unsigned)((groups * spans + 3) / 4));

@@ -18,6 +18,11 @@ from . import _native
 MAX_RANK = 256
 
 
+def _aligned(t):
+    """`t` from a 16-byte boundary on, which a view may not be."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class AdapterSet:
     """The adapters of one projection: `down` FP16[n,rank,K], `up`
     FP16[n,N,rank], `scale` FP32[n] (default 1).  Adapters of a lower rank
@@ -41,8 +46,8 @@ class AdapterSet:
         self.features = down.shape[2], up.shape[1]     # (K, N) of the projection
         # the kernels read ranks and inputs in eights: zeros fill the last
         fill, tail = -rank % 8, -down.shape[2] % 8
-        self.down = F.pad(down, (0, tail, 0, fill)) if fill or tail else down.contiguous()
-        self.up = F.pad(up, (0, fill)) if fill else up.contiguous()
+        self.down = _aligned(F.pad(down, (0, tail, 0, fill)) if fill or tail else down.contiguous())
+        self.up = _aligned(F.pad(up, (0, fill)) if fill else up.contiguous())
         self.scale = scale.contiguous()
 
 
@@ -84,7 +89,7 @@ def add(base, x, adapters, ids, out=None):
     if rows == 0:
         return out
     ids = ids.contiguous()
-    rank = adapters.down.shape[1]
+    rank = adapters.rank
     ws_bytes = int(_native.lib().m2r_adapters_workspace(rows, k, n, rank))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=base.device)
     p = _native.ptr

@@ -97,6 +97,31 @@ def test_non_finite_rows_stay_apart(device):
     assert bool(got[5].isnan().all()) and not bool(torch.isfinite(got[30]).all())
 
 
+@pytest.mark.parametrize("rank", [1, 3, 8])
+def test_infinite_hidden_values(device, rank):
+    """An infinity comes out as in the formula, also where the rank is padded."""
+    c = _case(device, 20, 100, 70, 2, rank, seed=10)
+    c["x"][4, 9] = math.inf
+    c["x"][7, 11] = -math.inf
+    c["ids"][4], c["ids"][7] = 0, 1
+    c["up"] = c["up"].abs() + 0.5
+    c["down"] = c["down"].abs() + 0.5     # all hidden values of a row share the sign
+    got, (want, _) = _add(c), _reference(c)
+    assert bool((got[4] == math.inf).all()) and bool((got[7] == -math.inf).all())
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want))
+
+
+@pytest.mark.parametrize("rank", [8, 5])
+def test_weights_off_a_16_byte_boundary(device, rank):
+    c = _case(device, 20, 64, 40, 3, rank, seed=11)
+    want = _add(c)
+    off = dict(c)
+    for key in ("down", "up"):
+        buf = torch.empty(c[key].numel() + 3, dtype=torch.float16, device=device)
+        off[key] = buf[3:].view(c[key].shape).copy_(c[key])
+    assert torch.equal(_add(off), want)
+
+
 @pytest.mark.parametrize("scale", [1e-4, 200.0])
 def test_magnitudes(device, scale):
     c = _case(device, 20, 1024, 256, 3, 16, seed=12)
