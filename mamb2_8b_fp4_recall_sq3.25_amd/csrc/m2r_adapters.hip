@@ -222,8 +222,8 @@ __device__ __forceinline__ float hidden_fragments(const AdapterArgs& a, int64_t 
 // the pair takes outputs 8 q + 4 T + k of the 32 as its rows 4 q + k.  The
 // hidden values go in as two binary16, scaled by each row's largest.
 // KS: 32-rank steps.
-template <int MT, int KS>
-__global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
+template <int MT, int KS, int NT>
+__global__ __launch_bounds__(256, KS == 1 ? 3 : 1) void k_adapter_up(AdapterArgs a) {
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
   const int64_t spans = (a.N + a.span - 1) / a.span;
   int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -282,31 +282,37 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) back[i] = hidden_fragments<KS>(a, m0 + 16 * i + lr, mine[i], sc, hi[i], lo[i]);
     const uint16_t* ub = a.up + (int64_t)cur * a.N * a.r;
-    // the next 32 outputs' operands are on their way while these are formed
-    h16x8 bv[MT], bn[MT];
-    f16x8 uf[2][KS], un[2][KS];
-    auto fetch = [&](int64_t nb, h16x8 (&bd)[MT], f16x8 (&ud)[2][KS]) {
-      const int64_t n = nb + 8 * lg;
+    // the next step's base is on its way while this one is formed; `up` comes
+    // from the L2, and a second set of its registers would cost a wave a SIMD
+    h16x8 bv[MT][NT / 2], bn[MT][NT / 2];
+    auto fetch = [&](int64_t nb, h16x8 (&bd)[MT][NT / 2]) {
+      const int64_t n = nb + 4 * NT * lg;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        bd[i] = nb + 32 <= a.N ? load_h16x8(br[i] + n) : __builtin_bit_cast(h16x8, load_f16x8(br[i] + n, a.N - n));
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        const int64_t row = nb + 8 * (lr >> 2) + 4 * T + (lr & 3);
+        for (int u = 0; u < NT / 2; ++u)
+          bd[i][u] = nb + 16 * NT <= a.N ? load_h16x8(br[i] + n + 8 * u)
+                                         : __builtin_bit_cast(h16x8, load_f16x8(br[i] + n + 8 * u, a.N - n - 8 * u));
+    };
+    fetch(n0, bv);
+    for (int64_t nb = n0; nb < n1; nb += 16 * NT) {
+      f16x8 uf[NT][KS];
+#pragma unroll
+      for (int T = 0; T < NT; ++T) {
+        const int64_t row = nb + 4 * NT * (lr >> 2) + 4 * T + (lr & 3);
         const uint16_t* ur = ub + (row < a.N ? row : a.N - 1) * a.r;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) ud[T][k] = load_ranks(ur, 32 * k + 8 * lg, a.r);
+        for (int k = 0; k < KS; ++k) uf[T][k] = load_ranks(ur, 32 * k + 8 * lg, a.r);
       }
-    };
-    fetch(n0, bv, uf);
-    for (int64_t nb = n0; nb < n1; nb += 32) {
-      const int64_t n = nb + 8 * lg;
-      if (nb + 32 < n1) fetch(nb + 32, bn, un);
-      f32x4 acc[MT][2];
+      // (behind the loads of `up`, which are waited for first)
+      if (nb + 16 * NT < n1) fetch(nb + 16 * NT, bn);
+      f32x4 acc[MT][NT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
+        for (int T = 0; T < NT; ++T) acc[i][T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int T = 0; T < NT; ++T)
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
 #pragma unroll
@@ -316,23 +322,25 @@ __global__ __launch_bounds__(256) void k_adapter_up(AdapterArgs a) {
         }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        if (mine[i]) {
-          h16x8 o;
+        if (mine[i])
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = f2h(__builtin_fmaf(acc[i][j >> 2][j & 3], back[i], h2f(bv[i][j])));
-          if (n + 8 <= a.N) __builtin_memcpy(orow[i] + n, &o, 16);
-          else {
+          for (int u = 0; u < NT / 2; ++u) {
+            const int64_t n = nb + 4 * NT * lg + 8 * u;
+            h16x8 o;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (n + j < a.N) orow[i][n + j] = o[j];
+              o[j] = f2h(__builtin_fmaf(acc[i][2 * u + (j >> 2)][j & 3], back[i], h2f(bv[i][u][j])));
+            if (n + 8 <= a.N) __builtin_memcpy(orow[i] + n, &o, 16);
+            else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) orow[i][n + j] = o[j];
+            }
           }
-        }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) bv[i] = bn[i];
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) uf[T][k] = un[T][k];
+        for (int u = 0; u < NT / 2; ++u) bv[i][u] = bn[i][u];
     }
   }
 }
@@ -404,13 +412,13 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   if ((groups * spans + 3) / 4 > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
   const dim3 up_grid((unsigned)((groups * spans + 3) / 4));
   if (wide) {
-    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<2, 1>), up_grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((k_adapter_up<2, 2>), up_grid, block, 0, stream, a);
+    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<2, 1, 4>), up_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_up<2, 2, 4>), up_grid, block, 0, stream, a);
   } else {
-    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<1, 1>), up_grid, block, 0, stream, a);
-    else if (rank <= 64) hipLaunchKernelGGL((k_adapter_up<1, 2>), up_grid, block, 0, stream, a);
-    else if (rank <= 128) hipLaunchKernelGGL((k_adapter_up<1, 4>), up_grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((k_adapter_up<1, 8>), up_grid, block, 0, stream, a);
+    if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<1, 1, 2>), up_grid, block, 0, stream, a);
+    else if (rank <= 64) hipLaunchKernelGGL((k_adapter_up<1, 2, 2>), up_grid, block, 0, stream, a);
+    else if (rank <= 128) hipLaunchKernelGGL((k_adapter_up<1, 4, 2>), up_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_up<1, 8, 2>), up_grid, block, 0, stream, a);
   }
   return m2r_check(hipGetLastError(), "adapters up launch");
 }
