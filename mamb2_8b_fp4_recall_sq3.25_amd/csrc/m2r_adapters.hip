@@ -354,11 +354,12 @@ constexpr int64_t kSpanWaves = 8192;
 static void adapter_plan(AdapterArgs& a) {
   const int64_t tiles = (a.M + 15) / 16;
   a.members = a.M <= kMemberRows ? (int)(a.M < 16 ? a.M : 16) : 1;
-  // slices of K for about 512 workgroups, of at least 512 each
+  // Slices of K for about 512 workgroups, of at least 512 each and at most four,
+  // since the second launch adds them up for each span.
   int64_t s = 512 / (tiles * a.members);
   const int64_t most = (a.Kp + 511) / 512;
   s = s < most ? s : most;
-  s = s < 1 ? 1 : (s > 8 ? 8 : s);
+  s = s < 1 ? 1 : (s > 4 ? 4 : s);
   a.slice = ((a.Kp + s - 1) / s + 63) / 64 * 64;
   a.slices = (int)((a.Kp + a.slice - 1) / a.slice);
 }

@@ -88,7 +88,9 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 
 // ---------------------------------------------------------------------------
 // Three launches.  A row is cut into at most kMaxSplits pieces of whole
-// 2,048-token blocks, one workgroup each.
+// 2,048-token blocks, one workgroup each; the kept weight is counted by units
+// of at most kUnits a row, a block each but in the longest rows, so that the
+// draw reads one of them.
 //   k_sample_top:    the largest logit of each piece;
 //   k_sample_bins:   the row's weight and token counts by bins of 1/16 in the
 //                    exponent (512 bins reach weight 0); the last workgroup
@@ -102,11 +104,11 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 // equal logits) is cut by its first workgroup alone, digit by digit.
 // Every sum is of whole numbers, so neither the order of the atomics nor the
 // order of the list decides anything.
-constexpr int kThreads = 256, kBlock = 8 * kThreads, kMaxSplits = 256, kBins = 512, kList = 4096;
+constexpr int kThreads = 256, kBlock = 8 * kThreads, kMaxSplits = 256, kUnits = kThreads, kBins = 512, kList = 4096;
 
 struct alignas(16) RowWork {
   uint64_t weight[kBins];
-  uint64_t piece[kMaxSplits];    // weight kept for certain
+  uint64_t unit[kUnits];         // weight kept for certain
   uint64_t list[kList];          // (~key, index) of the tokens in the cut's bins
   uint32_t count[kBins];
   float top[kMaxSplits];
@@ -120,7 +122,7 @@ struct alignas(16) RowWork {
 struct SampleShared {
   uint64_t bins[kBins];          // count << 46 | weight
   uint64_t list[kList];
-  uint64_t piece[kMaxSplits];
+  uint64_t unit[kUnits];
   uint64_t part[kThreads / 64];
   float fpart[kThreads / 64];
   uint32_t cnt[256];
@@ -141,6 +143,12 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {   // inclusive
     if (lane >= by) v += o;
   }
   return v;
+}
+// Adds the lanes' values to *sum in LDS.
+__device__ __forceinline__ void wave_add64(uint64_t* sum, uint64_t v) {
+  if (!__ballot(v != 0)) return;
+  v = wave_scan64(v);
+  if ((threadIdx.x & 63) == 63) atomicAdd((unsigned long long*)sum, (unsigned long long)v);
 }
 // Exclusive prefix sum over the workgroup; `total` receives the sum.
 __device__ __forceinline__ uint64_t block_scan64(SampleShared& s, uint64_t v, uint64_t& total) {
@@ -197,7 +205,7 @@ __device__ __forceinline__ uint64_t place_of(float l, int64_t i) {   // ascendin
 }
 
 struct Piece { int64_t row; int64_t first, end; int piece; };
-struct Split { int pieces; int64_t size; };
+struct Split { int pieces; int64_t size; int units; int64_t unit; };   // `size` whole units
 __device__ __forceinline__ Piece my_piece(const Split& sp, int64_t V) {
   Piece p;
   p.row = blockIdx.x / sp.pieces;
@@ -220,6 +228,13 @@ __device__ __forceinline__ void put(T* p, T v) { __hip_atomic_store(p, v, __ATOM
 template <class T>
 __device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// A piece's units, from the front of s.unit.
+__device__ __forceinline__ void put_units(SampleShared& s, RowWork& rw, const Piece& p, const Split& sp) {
+  const int first = (int)(p.first / sp.unit), n = (int)((p.end - p.first + sp.unit - 1) / sp.unit);
+  __syncthreads();
+  if ((int)threadIdx.x < n) put(&rw.unit[first + threadIdx.x], s.unit[threadIdx.x]);
+}
+
 // True in the workgroup that finishes its row's pass last: every workgroup
 // counts itself once its atomics have completed.
 __device__ __forceinline__ bool last_of_row(SampleShared& s, uint32_t* ticket, int pieces) {
@@ -237,14 +252,14 @@ __device__ __forceinline__ void put_token(const SampleArgs& a, int64_t row, cons
   a.logprobs[row] = -away_of(f, l) * 0x1.62e43p-1f - logf((float)total * 0x1p-31f);
 }
 
-// The draw, with the kept weight of each piece in s.piece: a token is kept
+// The draw, with the kept weight of each unit in s.unit: a token is kept
 // when its place is at most `cut` and its weight at least f.least.
 template <int DT>
 __device__ void draw(SampleShared& s, const SampleArgs& a, const Split& sp, int64_t r, const RowFilter& f, uint64_t cut) {
   const int tid = threadIdx.x;
   const void* row = row_of<DT>(a, r);
   uint64_t total;
-  const uint64_t mine = tid < sp.pieces ? s.piece[tid] : 0, before = block_scan64(s, mine, total);
+  const uint64_t mine = tid < sp.units ? s.unit[tid] : 0, before = block_scan64(s, mine, total);
   const double at = __builtin_floor((double)a.u[r] * (double)total);
   uint64_t target = at > 0.0 ? (uint64_t)at : 0;
   target = target < total ? target : total - 1;
@@ -253,10 +268,10 @@ __device__ void draw(SampleShared& s, const SampleArgs& a, const Split& sp, int6
     s.found[0] = target - before;
   }
   __syncthreads();
-  const int piece = s.pick[0];
+  const int unit = s.pick[0];
   uint64_t left = s.found[0];
-  const int64_t end = (piece + 1) * sp.size < a.V ? (piece + 1) * sp.size : a.V;
-  for (int64_t i0 = piece * sp.size; i0 < end; i0 += kBlock) {
+  const int64_t end = (unit + 1) * sp.unit < a.V ? (unit + 1) * sp.unit : a.V;
+  for (int64_t i0 = unit * sp.unit; i0 < end; i0 += kBlock) {
     const int64_t i = i0 + 8 * tid;
     float v[8];
     uint32_t w[8];
@@ -355,20 +370,25 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp
   }
   const bool filtered = f.k < a.V || f.p < 1.0;
   if (!filtered) {
-    uint64_t sum = 0, all;
-    for (int64_t i = p.first + 8 * tid; i < p.end; i += kBlock) {
-      float v[8];
-      load_logits<DT>(row, i, a.V, v);
+    s.unit[tid] = 0;
+    __syncthreads();
+    for (int64_t from = p.first, q = 0; from < p.end; from += sp.unit, ++q) {
+      const int64_t to = from + sp.unit < p.end ? from + sp.unit : p.end;
+      uint64_t sum = 0;
+      for (int64_t i = from + 8 * tid; i < to; i += kBlock) {
+        float v[8];
+        load_logits<DT>(row, i, a.V, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t w = weight_of(f, v[j]);
-        sum += w >= f.least ? w : 0;
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = weight_of(f, v[j]);
+          sum += w >= f.least ? w : 0;
+        }
       }
+      wave_add64(&s.unit[q], sum);
     }
-    block_scan64(s, sum, all);
-    if (tid == 0) put(&rw.piece[p.piece], all);
+    put_units(s, rw, p, sp);
     if (!last_of_row(s, &rw.ticket[0], sp.pieces)) return;
-    s.piece[tid] = tid < sp.pieces ? get(&rw.piece[tid]) : 0;
+    s.unit[tid] = tid < sp.units ? get(&rw.unit[tid]) : 0;
     if (tid == 0) rw.done = 1;
     __syncthreads();
     draw<DT>(s, a, sp, p.row, f, ~0ull);
@@ -466,6 +486,38 @@ __device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, u
     const uint32_t b = bin_of(f, logit_of(~(uint32_t)(c >> 32)));
     return b >= b0 && b <= b1;
   };
+  if (n <= 64) {   // every token counts those before it, each wave a quarter of them
+    const uint32_t at = tid & 63, q = tid >> 6;
+    const uint64_t e = at < n ? s.list[at] : 0;
+    const uint32_t w = weight_of(f, logit_of(~(uint32_t)(e >> 32)));
+    const bool in = at < n && takes(e);
+    __syncthreads();
+    if (q == 0) sum[at] = in ? w : 0;   // tokens that do not take part count nothing
+    __syncthreads();
+    uint64_t weight = 0;
+    uint32_t count = 0;
+    const uint32_t end = 16 * q + 16 < n ? 16 * q + 16 : n;
+    for (uint32_t i = 16 * q; i < end; ++i) {
+      const uint64_t wi = s.list[i] < e ? sum[i] : 0;
+      count += wi != 0;
+      weight += wi;
+    }
+    sum[64 + tid] = weight;
+    s.cnt[tid] = count;
+    __syncthreads();
+    if (q == 0 && in) {
+      weight = sum[64 + at] + sum[128 + at] + sum[192 + at] + sum[256 + at];
+      count = s.cnt[at] + s.cnt[64 + at] + s.cnt[128 + at] + s.cnt[192 + at];
+      if (BY_WEIGHT ? weight < target && target <= weight + w : count + 1 == target) {
+        s.found[0] = e;
+        s.found[2] = weight;
+      }
+    }
+    __syncthreads();
+    const Place c{s.found[0], s.found[2]};
+    __syncthreads();
+    return c;
+  }
   uint64_t any = 0, each = ~0ull;
   for (uint32_t i = tid; i < n; i += kThreads)
     if (takes(s.list[i])) {
@@ -487,28 +539,6 @@ __device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, u
   each = s.found[0] & s.found[1] & s.found[2] & s.found[3];
   Place c{each, 0};
   uint64_t count = 0;
-  if (n <= kThreads) {   // every token counts those before it
-    const uint64_t e = (uint32_t)tid < n ? s.list[tid] : 0;
-    const uint32_t w = weight_of(f, logit_of(~(uint32_t)(e >> 32)));
-    const bool in = (uint32_t)tid < n && takes(e);
-    __syncthreads();
-    sum[tid] = in ? w : 0;   // tokens that do not take part count nothing
-    __syncthreads();
-    for (uint32_t i = 0; i < n; ++i) {
-      const uint64_t wi = s.list[i] < e ? sum[i] : 0;
-      count += wi != 0;
-      c.weight += wi;
-    }
-    if (in && (BY_WEIGHT ? c.weight < target && target <= c.weight + w : count + 1 == target)) {
-      s.found[0] = e;
-      s.found[2] = c.weight;
-    }
-    __syncthreads();
-    c.place = s.found[0];
-    c.weight = s.found[2];
-    __syncthreads();
-    return c;
-  }
   int shift = any == each ? -8 : (63 - __builtin_clzll(any ^ each)) & ~7;
   if (shift >= 0) c.place = shift == 56 ? 0 : each >> (shift + 8) << (shift + 8);   // what all share
   for (; shift >= 0; shift -= 8) {
@@ -671,9 +701,11 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
   if (done == 2) {
     const uint64_t cut = cut_row<DT>(s, rw, row, a.V, f);
     __syncthreads();
-    for (int q = 0; q < sp.pieces; ++q) {
-      const int64_t first = q * sp.size, end = first + sp.size < a.V ? first + sp.size : a.V;
-      uint64_t sum = 0, all;
+    s.unit[tid] = 0;
+    __syncthreads();
+    for (int q = 0; q < sp.units; ++q) {
+      const int64_t first = q * sp.unit, end = first + sp.unit < a.V ? first + sp.unit : a.V;
+      uint64_t sum = 0;
       for (int64_t i = first + 8 * tid; i < end; i += kBlock) {
         float v[8];
         load_logits<DT>(row, i, a.V, v);
@@ -683,8 +715,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
           sum += w >= f.least && place_of(v[j], i + j) <= cut ? w : 0;
         }
       }
-      block_scan64(s, sum, all);
-      if (tid == 0) s.piece[q] = all;
+      wave_add64(&s.unit[q], sum);
     }
     __syncthreads();
     draw<DT>(s, a, sp, p.row, f, cut);
@@ -695,28 +726,29 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
   const uint32_t above = p0 < (uint32_t)kBins ? p0 : bk, end = bk < (uint32_t)kBins ? bk + 1 : p1 + 1;
   const float above16 = (float)above, end16 = (float)end;
   if (tid == 0) s.pick[0] = 0;
+  s.unit[tid] = 0;
   __syncthreads();
-  uint64_t sum = 0;
-  for (int64_t i = p.first + 8 * tid; i < p.end; i += kBlock) {
-    float v[8];
-    load_logits<DT>(row, i, a.V, v);
+  for (int64_t from = p.first, q = 0; from < p.end; from += sp.unit, ++q) {
+    const int64_t to = from + sp.unit < p.end ? from + sp.unit : p.end;
+    uint64_t sum = 0;
+    for (int64_t i = from + 8 * tid; i < to; i += kBlock) {
+      float v[8];
+      load_logits<DT>(row, i, a.V, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float away = away_of(f, v[j]), t = away * 16.0f;
-      if (t < end16) {   // few tokens, and few waves that hold one
-        const uint32_t w = weight_at(away), b = (uint32_t)t;
-        if (t < above16) sum += w >= f.least ? w : 0;
-        else if (w && ((p0 <= b && b <= p1) || b == bk)) s.list[atomicAdd(&s.pick[0], 1u)] = place_of(v[j], i + j);
+      for (int j = 0; j < 8; ++j) {
+        const float away = away_of(f, v[j]), t = away * 16.0f;
+        if (t < end16) {   // few tokens, and few waves that hold one
+          const uint32_t w = weight_at(away), b = (uint32_t)t;
+          if (t < above16) sum += w >= f.least ? w : 0;
+          else if (w && ((p0 <= b && b <= p1) || b == bk)) s.list[atomicAdd(&s.pick[0], 1u)] = place_of(v[j], i + j);
+        }
       }
     }
+    wave_add64(&s.unit[q], sum);
   }
-  uint64_t kept;
-  block_scan64(s, sum, kept);
+  put_units(s, rw, p, sp);   // (the list is complete, too)
   const uint32_t mine = s.pick[0];
-  if (tid == 0) {
-    put(&rw.piece[p.piece], kept);
-    s.pick[1] = mine ? atomicAdd(&rw.listed, mine) : 0;
-  }
+  if (tid == 0) s.pick[1] = mine ? atomicAdd(&rw.listed, mine) : 0;
   __syncthreads();
   for (uint32_t i = tid; i < mine; i += kThreads) put(&rw.list[s.pick[1] + i], s.list[i]);
   if (!last_of_row(s, &rw.ticket[1], sp.pieces)) return;
@@ -737,27 +769,27 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
   if (with_p) cut = select_place<true>(s, n, f, 0, two ? p1 : kBins, mass_of(f.p, all) - rw.weight_p).place;
   const uint32_t per = (n + kThreads - 1) / kThreads, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
   __syncthreads();
-  s.piece[tid] = tid < sp.pieces ? get(&rw.piece[tid]) : 0;
+  s.unit[tid] = tid < sp.units ? get(&rw.unit[tid]) : 0;
   __syncthreads();
   for (uint32_t i = i0; i < i1; ++i)
     if (s.list[i] <= cut) {
       const uint32_t w = weight_of(f, logit_of(~(uint32_t)(s.list[i] >> 32)));
-      if (w >= f.least) atomicAdd((unsigned long long*)&s.piece[(uint32_t)s.list[i] / (uint32_t)sp.size], (unsigned long long)w);
+      if (w >= f.least) atomicAdd((unsigned long long*)&s.unit[(uint32_t)s.list[i] / (uint32_t)sp.unit], (unsigned long long)w);
     }
   __syncthreads();
   draw<DT>(s, a, sp, p.row, f, cut);
 }
 
-// Pieces of at least one 2,048-token block, so many that the rows together
+// Pieces of at least one unit, so many that the rows together
 // make about four workgroups a compute unit.
 static Split sample_split(int64_t batch, int64_t V) {
-  const int64_t blocks = (V + kBlock - 1) / kBlock;
+  const int64_t blocks = (V + kBlock - 1) / kBlock, unit = (blocks + kUnits - 1) / kUnits, all = (blocks + unit - 1) / unit;
   int64_t pieces = 1024 / (batch < 1024 ? batch : 1024);
   pieces = pieces < 1 ? 1 : pieces;
-  pieces = pieces < blocks ? pieces : blocks;
+  pieces = pieces < all ? pieces : all;
   pieces = pieces < kMaxSplits ? pieces : kMaxSplits;
-  const int64_t per = (blocks + pieces - 1) / pieces;
-  return Split{(int)((blocks + per - 1) / per), per * kBlock};
+  const int64_t per = (all + pieces - 1) / pieces;
+  return Split{(int)((all + per - 1) / per), per * unit * kBlock, (int)all, unit * kBlock};
 }
 
 template <int DT>
