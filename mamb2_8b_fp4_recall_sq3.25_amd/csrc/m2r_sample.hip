@@ -476,13 +476,14 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp
 struct Place { uint64_t place, weight; };   // a token's place and the weight of the list before it
 
 // The token of s.list, among those of bins b0..b1, at which the running count
-// (BY_WEIGHT: weight) in the order of the places reaches `target`: digit by
-// digit from the first that differs.  The target must be reached.
+// (BY_WEIGHT: weight) in the order of the places reaches `target`: up to 8
+// bits at a time from the first that differs.  The target must be reached.
 template <bool BY_WEIGHT>
 __device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, uint32_t b0, uint32_t b1, uint64_t target) {
   const int tid = threadIdx.x;
   uint64_t* sum = s.bins;   // 256 weights
   auto takes = [&](uint64_t c) {
+    if (b0 == 0 && b1 == (uint32_t)kBins) return true;
     const uint32_t b = bin_of(f, logit_of(~(uint32_t)(c >> 32)));
     return b >= b0 && b <= b1;
   };
@@ -539,19 +540,22 @@ __device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, u
   each = s.found[0] & s.found[1] & s.found[2] & s.found[3];
   Place c{each, 0};
   uint64_t count = 0;
-  int shift = any == each ? -8 : (63 - __builtin_clzll(any ^ each)) & ~7;
-  if (shift >= 0) c.place = shift == 56 ? 0 : each >> (shift + 8) << (shift + 8);   // what all share
-  for (; shift >= 0; shift -= 8) {
+  // from the highest bit that differs, up to 8 bits at a time
+  int top = any == each ? 0 : 64 - __builtin_clzll(any ^ each), shift;
+  if (top) c.place = top == 64 ? 0 : each >> top << top;   // what all share
+  for (; top; top = shift) {
+    shift = top > 8 ? top - 8 : 0;
+    const uint32_t mask = (1u << (top - shift)) - 1;
     __syncthreads();
     s.cnt[tid] = 0;
     sum[tid] = 0;
     __syncthreads();
     for (uint32_t i = tid; i < n; i += kThreads) {
       const uint64_t e = s.list[i];
-      if (takes(e) && (shift == 56 || (e >> (shift + 8)) == (c.place >> (shift + 8)))) {
-        atomicAdd(&s.cnt[(e >> shift) & 255], 1u);
-        atomicAdd((unsigned long long*)&sum[(e >> shift) & 255],
-                  (unsigned long long)weight_of(f, logit_of(~(uint32_t)(e >> 32))));
+      if (takes(e) && (top == 64 || (e >> top) == (c.place >> top))) {
+        const uint32_t digit = (uint32_t)(e >> shift) & mask;
+        atomicAdd(&s.cnt[digit], 1u);
+        atomicAdd((unsigned long long*)&sum[digit], (unsigned long long)weight_of(f, logit_of(~(uint32_t)(e >> 32))));
       }
     }
     __syncthreads();
