@@ -10,6 +10,13 @@
 // adds the slices up and multiplies by up.  The rows of a tile that share an
 // adapter are one product, whose other columns are computed and dropped: a
 // prompt's rows are mostly one such group, a decode step's rows one each.
+//
+// Bound by memory and by the latency of a short chain of loads (ids, weights
+// and rows, hidden values): 2 r (K + N) operations for 2 (K + 2 N) bytes a row.
+// 2,500 rows of rank 32 over K = 4,096, N = 18,560 (six adapters): 72 us, the
+// first launch 15 and the second 46 warm, 215 MB at 3.0 TB/s, where a copy of
+// base to out alone takes 38.  64 rows of 48 adapters of rank 16, K = 8,192,
+// N = 4,096: 14 us; one row, K = 4,096, N = 18,560: 8 us, two launches.
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 #include "m2r_tile.h"
@@ -38,8 +45,9 @@ struct AdapterArgs {
   int rank;             // r - 7 ... r: a hidden value past it counts as 0, whatever x holds
   int slices;           // of K, `slice` long each (a multiple of 64)
   int64_t slice;
-  int members;          // 16: a workgroup per row that leads its group; 1: a workgroup per tile
+  int members;          // workgroups (waves in the second launch) among which a tile's groups are dealt, a power of two to 16
   int64_t span;         // outputs of a wave in the second launch, a multiple of 64
+  uint32_t spans;
 };
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
@@ -73,33 +81,39 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int64_t m) {
   return id >= 0 && id < a.n ? id : -1;
 }
 
-// One wave per (tile, slice of K / 4): its four quarters meet in LDS.
+// Of 16 members each takes the group whose first row it is, without counting
+// the groups before it: leaves that group in `rows`, the tile's, or nothing.
+__device__ __forceinline__ int only_group(int id, int member, uint32_t& rows) {
+  const uint32_t group = (uint32_t)__ballot(id == __builtin_amdgcn_readlane(id, member)) & rows;
+  rows = (group >> member & 1) && !(group & ((1u << member) - 1)) ? group : 0;
+  return member;
+}
+
+// One wave per (tile, slice of K / 4): its four quarters meet in LDS.  (More
+// loads in flight at a time, three to six steps', changed nothing.)
 // RT: 16-rank tiles at a time.
 template <int RT>
 __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
   __shared__ f32x4 part[3][RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
-  int64_t w = blockIdx.x;
-  const int member = (int)(w % a.members);
-  w /= a.members;
-  const int slice = (int)(w % a.slices);
-  const int64_t m0 = w / a.slices * 16, m = m0 + lr;
+  uint32_t w = blockIdx.x;   // (64-bit divisions here would take a microsecond)
+  const int member = (int)(w % (uint32_t)a.members);
+  w /= (uint32_t)a.members;
+  const int slice = (int)(w % (uint32_t)a.slices);
+  const int64_t m0 = (int64_t)(w / (uint32_t)a.slices) * 16, m = m0 + lr;
   const int id = adapter_of(a, m);
   uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xffffu;
-  if (a.members > 1) {   // only this row's group, if it is the first of it
-    const int mine = __builtin_amdgcn_readlane(id, member);
-    const uint32_t group = (uint32_t)__ballot(id == mine) & 0xffffu;
-    if (mine < 0 || (group & ((1u << member) - 1))) return;
-    todo = group;
-  }
   const int64_t quarter = (a.slice / 64 + 3) / 4 * 64;
   const int64_t s1 = (slice + 1) * a.slice < a.Kp ? (slice + 1) * a.slice : a.Kp;
   const int64_t k0 = slice * a.slice + wave * quarter, k1 = k0 + quarter < s1 ? k0 + quarter : s1;
   const uint16_t* xr = a.x + (m < a.M ? m : a.M - 1) * a.xs;
-  while (todo) {
+  int group = 0;
+  if (a.members == 16) group = only_group(id, member, todo);
+  for (; todo; ++group) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
     const bool mine = id == cur;
     todo &= ~(uint32_t)__ballot(mine);
+    if ((group & (a.members - 1)) != member) continue;
     for (int r0 = 0; r0 < a.r; r0 += 16 * RT) {
       f32x4 acc[RT];
 #pragma unroll
@@ -219,18 +233,21 @@ __device__ __forceinline__ float hidden_fragments(const AdapterArgs& a, int64_t 
 
 // One wave per (MT tiles of 16 rows, span of outputs).  A lane holds row
 // 16 i + lr of each tile and 8 neighbouring outputs of 32: output tile T of
-// the pair takes outputs 8 q + 4 T + k of the 32 as its rows 4 q + k.  The
+// NT takes outputs 4 NT q + 4 T + k of the 16 NT as its rows 4 q + k.  The
 // hidden values go in as two binary16, scaled by each row's largest.
-// KS: 32-rank steps.
+// KS: 32-rank steps.  Two tiles of rows share the loads of `up` where rows are
+// many (one at a time: 81 us for 76), and take 64 outputs at a time, whole
+// 128-byte lines (32: 80 us for 76); few rows take 32, for more waves (64 rows:
+// 15.8 us for 17.9).  Turning the products in LDS for rows of full lines cost
+// more than the lines saved (82 us for 80).
 template <int MT, int KS, int NT>
 __global__ __launch_bounds__(256, KS == 1 ? 3 : 1) void k_adapter_up(AdapterArgs a) {
   const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-  const int64_t spans = (a.N + a.span - 1) / a.span;
-  int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t span = w % spans;
-  w /= spans;
-  const int member = (int)(w % a.members);
-  const int64_t m0 = w / a.members * (16 * MT);
+  uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t span = w % a.spans;
+  w /= a.spans;
+  const int member = (int)(w % (uint32_t)a.members);
+  const int64_t m0 = (int64_t)(w / (uint32_t)a.members) * (16 * MT);
   if (m0 >= a.M) return;
   const int64_t n0 = span * a.span, n1 = n0 + a.span < a.N ? n0 + a.span : a.N;
   int id[MT];
@@ -241,13 +258,13 @@ __global__ __launch_bounds__(256, KS == 1 ? 3 : 1) void k_adapter_up(AdapterArgs
     id[i] = adapter_of(a, m);
     todo |= (__ballot(m < a.M) & 0xffffull) << (16 * i);
   }
-  if (MT == 1 && a.members > 1) {
-    const int mine = __builtin_amdgcn_readlane(id[0], member);
-    const uint64_t group = __ballot(id[0] == mine) & todo;
-    if (!(todo >> member & 1) || (group & ((1ull << member) - 1))) return;
-    todo = group;
+  int group = 0;
+  if (MT == 1 && a.members == 16) {
+    uint32_t rows = (uint32_t)todo;
+    group = only_group(id[0], member, rows);
+    todo = rows;
   }
-  while (todo) {
+  for (; todo; ++group) {
     const int first = __builtin_ctzll(todo);
     int cur = 0;
 #pragma unroll
@@ -264,6 +281,7 @@ __global__ __launch_bounds__(256, KS == 1 ? 3 : 1) void k_adapter_up(AdapterArgs
       br[i] = a.base + (m < a.M ? m : 0) * a.bs;
       orow[i] = a.out + (m < a.M ? m : 0) * a.os;
     }
+    if (MT == 1 && (group & (a.members - 1)) != member) continue;
     if (cur < 0) {   // rows without an adapter
       for (int64_t n = n0 + 8 * lg; n < n1; n += 32)
 #pragma unroll
@@ -345,15 +363,27 @@ __global__ __launch_bounds__(256, KS == 1 ? 3 : 1) void k_adapter_up(AdapterArgs
   }
 }
 
-// Few rows: a workgroup for each row that leads its group, so that groups run
-// side by side; many: a workgroup walks through its tile's groups, mostly one.
 constexpr int64_t kMemberRows = 512;
-// Waves to aim for in the second launch.
+// Workgroups among which a tile's groups are dealt: few rows leave the chip idle
+// otherwise, and of many rows most find no group of theirs.  us a call at rank
+// 16, K = N = 4,096, 8 adapters, with 16 / 4 / 1 of them: 64 rows of 64 requests
+// 10.8 / 14.7 / -, of two 10.7 / 9.2 / -; 128 rows of 128 15.3 / 15.7 / -, of
+// two 14.2 / 9.5 / -; 256 rows of 256 19.8 / 18.9 / 49, of six 20.5 / 11.6 /
+// 16.7; 512 rows of 512 31 / 28 / 50, of six 34 / 15.4 / 20.3; 1,024 rows of
+// 1,024 54 / 41 / 57, of six 49 / 24.5 / 20.8.
+static int adapter_members(int64_t M) {
+  const int most = M <= 64 ? 16 : (M <= kMemberRows ? 4 : 1);
+  int members = 1;
+  while (members < most && members < M) members *= 2;
+  return members;
+}
+// Waves to aim for in the second launch (2,500 rows of rank 32, N = 18,560: 4,096
+// and 6,144 waves 1 to 2 us slower, 3,072 by 11).
 constexpr int64_t kSpanWaves = 8192;
 
 static void adapter_plan(AdapterArgs& a) {
   const int64_t tiles = (a.M + 15) / 16;
-  a.members = a.M <= kMemberRows ? (int)(a.M < 16 ? a.M : 16) : 1;
+  a.members = adapter_members(a.M);
   // Slices of K for about 512 workgroups, of at least 512 each and at most four,
   // since the second launch adds them up for each span.
   int64_t s = 512 / (tiles * a.members);
@@ -402,7 +432,8 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   else hipLaunchKernelGGL(k_adapter_down<4>, down_grid, block, 0, stream, a);
   int rc = m2r_check(hipGetLastError(), "adapters down launch");
   if (rc) return rc;
-  // two tiles share a pass over `up` where rows are many and the rank small
+  // Two tiles share a pass over `up` where rows are many and the rank leaves
+  // registers for both (2,048 rows of rank 128: 90 us with one, 107 with two).
   const bool wide = a.M > kMemberRows && rank <= 64;
   const int64_t groups = wide ? (M + 31) / 32 : tiles * a.members;
   int64_t spans = kSpanWaves / groups;
@@ -410,7 +441,8 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   spans = spans < 1 ? 1 : (spans < most ? spans : most);
   a.span = ((N + spans - 1) / spans + 63) / 64 * 64;
   spans = (N + a.span - 1) / a.span;
-  if ((groups * spans + 3) / 4 > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
+  if (groups * spans > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
+  a.spans = (uint32_t)spans;
   const dim3 up_grid((unsigned)((groups * spans + 3) / 4));
   if (wide) {
     if (rank <= 32) hipLaunchKernelGGL((k_adapter_up<2, 1, 4>), up_grid, block, 0, stream, a);

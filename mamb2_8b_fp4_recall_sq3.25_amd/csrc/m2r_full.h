@@ -1,5 +1,5 @@
 // Arguments and shared arithmetic of the scan with a full-precision
-// (binary32) carry: m2r_full.hip.
+// (binary32) carry: m2r_full.hip, m2r_full_chunks.hip.
 #pragma once
 #include "m2r_device.h"
 #include "m2r_tile.h"

@@ -4,6 +4,10 @@
 //   dt_t = softplus(dt[b, t, h] + dt_bias[h]),  a_t = exp(A[h] dt_t)
 //   S_t  = a_t S_{t-1} + dt_t x_t (x) B_t            (S: [P, 128])
 //   y_t  = half(S_t C_t + D[h] x_t)
+// Operands and readouts are binary16 as the model holds them; dt, decays,
+// carries and sums are binary32, and a readout is rounded once.  A few tokens
+// are stepped one by one (k_full_rows, here); more go through the matrix cores
+// in chunks (m2r_full_chunks.hip).
 #include "m2r_full.h"
 #include "m2r_abi_util.h"
 
@@ -16,6 +20,11 @@ typedef uint16_t h16x4 __attribute__((ext_vector_type(4)));
 // Token by token.  Half a wave holds one row of the carry (lane n holds
 // coordinates 4n .. 4n + 3, a 16-byte access), a wave 2 R rows, so that R
 // loads of 1 KiB are in flight; the readout is a butterfly over 32 lanes.
+// One token is bound by memory: it reads and writes 1 KiB of carry a row for
+// 640 operations.  At 128 heads of 64, 61 of 64 batch rows at work: 99 us for
+// 514 MB, 5.2 TB/s, where a copy of 2 GiB reaches 4.9 (R = 2: 108 us, fewer
+// loads in flight; R = 8: 104, fewer waves).  Batch 1, 8.4 MB: 5.3 us, a
+// launch and one way to memory and back (R = 2: 5.4, R = 8: 6.1).
 template <int R>
 __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, q = lane & 31;

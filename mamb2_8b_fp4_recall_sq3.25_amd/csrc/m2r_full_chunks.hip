@@ -3,6 +3,32 @@
 // of A dt inside a chunk, S the carry before it and S' the carry after it,
 //   y_t = sum_{s <= t} (C_t . B_s) exp(l_t - l_s) dt_s x_s + exp(l_t) S C_t + D x_t
 //   S'  = exp(l_63) S + sum_s exp(l_63 - l_s) dt_s x_s (x) B_s.
+// The products run on binary16 matrix instructions that sum in binary32.  B, C
+// and x are binary16 already; what is not (the carry, the weighted scores, the
+// weighted x) goes in as two of them, 22 bits, scaled by a power of two that
+// keeps the largest value near the top of the range.  The running sums l are
+// formed in 64 bits, since differences of them become exponents.
+//
+// Work: a chunk and head of 64 costs 3 products of 64 x 64 x 128, the last two
+// twice for the halves, and 64 x 64 weights; x, y, B, C and dt move once, the
+// carry stays in registers across a segment (64 values a thread, which is why
+// a workgroup is 512 threads of 256 registers).  What few rows lack in
+// workgroups is made up by cutting the tokens into segments: a first pass
+// forms what each adds to a zero carry (x and B only), k_full_join runs the
+// carries through, and the main pass starts every segment from its own.
+//
+// At 128 heads of 64 in 8 groups: 8,192 tokens of one row 212 us (first pass
+// 55, join 13, main pass 142), 1.5 TB/s and 204 TFLOP/s counted token by
+// token; 2,048 tokens 80 us; nine rows of up to 901 tokens 159 us in one pass;
+// five short prompts 29 us.  Neither memory (64 us at 8,192 tokens) nor the
+// matrix cores bound it: a chunk takes a workgroup 17,500 clocks, of which a
+// SIMD's vector instructions are about 8,700, the LDS 5,500 and the matrix
+// instructions 5,000, and they overlap little, as both waves of a SIMD are at
+// the same step.  Leaving parts out saves, of 218 us: S C 22, the update 40,
+// the stores 22, the loads 25, the weights 15, the scalars 10.  Not better:
+// scores formed by each wave for itself, with one barrier a chunk (222 us for
+// the main kernels' 177); 16 waves of 128 registers (219 for 221); S C behind
+// the barrier; waves that start their chunk's parts in another order.
 #include "m2r_full.h"
 #include "m2r_abi_util.h"
 
@@ -228,8 +254,11 @@ __device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
   return wave_max_bits(lo > hi ? lo : hi);
 }
 // A workgroup steps four blocks of 64 columns (a head's channels) of one
-// group, two waves each, over one segment of one batch row's tokens.  OUT:
-// readouts and the pool's carry; else what the segment adds to a zero carry.
+// group, two waves each, over one segment of one batch row's tokens: four
+// blocks share the loads of B and C and the scores.  OUT: readouts and the
+// pool's carry; else what the segment adds to a zero carry.
+// The next chunk's operands are on their way into LDS while one is in work
+// (two ahead without readouts, where a chunk is shorter).
 template <bool ALIGNED, bool OUT>
 __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg) {
   __shared__ ChunkShared<OUT> s;
@@ -674,8 +703,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 }
 
 // The carries before each segment, of rows of more than one: a running fma over
-// the segments' additions, four values a thread, all of a thread's loads in
-// flight.
+// the segments' additions, four values a thread, eight loads in flight.  Bound
+// by memory: 8 segments of 128 heads of 64 (67 MB) 12.7 us, 5.3 TB/s.
 __global__ __launch_bounds__(256) void k_full_join(FullArgs a, Segments sg) {
   const int64_t b = blockIdx.y, i = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = a.H * a.P * 32;
   if (i >= per_row) return;
@@ -712,11 +741,12 @@ using namespace m2r;
 
 namespace m2r {
 
-// How many segments a call's tokens are split into.
+// How many segments a call's tokens are split into: a workgroup on each of 256
+// compute units at most.
 Segments full_segments(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) {
   const int64_t hpg = H / G, blocks = (hpg * ((P + 63) / 64) + 3) / 4, chunks = (L + kChunk - 1) / kChunk;
   const int64_t groups = blocks * G * batch;
-  int64_t want = groups >= 192 ? 1 : 256 / groups;
+  int64_t want = groups < 256 ? 256 / groups : 1;
   want = want < chunks ? want : chunks;
   const int64_t per = (chunks + want - 1) / want;
   return Segments{per * kChunk, (int)((chunks + per - 1) / per), nullptr, nullptr};

@@ -208,8 +208,9 @@ struct Piece { int64_t row; int64_t first, end; int piece; };
 struct Split { int pieces; int64_t size; int units; int64_t unit; };   // `size` whole units
 __device__ __forceinline__ Piece my_piece(const Split& sp, int64_t V) {
   Piece p;
-  p.row = blockIdx.x / sp.pieces;
-  p.piece = (int)(blockIdx.x - p.row * sp.pieces);
+  const uint32_t row = blockIdx.x / (uint32_t)sp.pieces;   // (a 64-bit division would take longer than a short row)
+  p.row = row;
+  p.piece = (int)(blockIdx.x - row * (uint32_t)sp.pieces);
   p.first = p.piece * sp.size;
   p.end = p.first + sp.size < V ? p.first + sp.size : V;
   return p;
@@ -230,7 +231,8 @@ __device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATO
 
 // A piece's units, from the front of s.unit.
 __device__ __forceinline__ void put_units(SampleShared& s, RowWork& rw, const Piece& p, const Split& sp) {
-  const int first = (int)(p.first / sp.unit), n = (int)((p.end - p.first + sp.unit - 1) / sp.unit);
+  const uint32_t unit = (uint32_t)sp.unit, first = (uint32_t)p.first / unit;   // (V is below 2^31)
+  const int n = (int)(((uint32_t)(p.end - p.first) + unit - 1) / unit);
   __syncthreads();
   if ((int)threadIdx.x < n) put(&rw.unit[first + threadIdx.x], s.unit[threadIdx.x]);
 }
