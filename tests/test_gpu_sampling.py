@@ -104,6 +104,25 @@ def test_large_rows_with_filters_of_their_own(device, vocab):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("spread", [0.02, 1e-3, 1.0, 60.0])
+@pytest.mark.parametrize("masked", [None, "lowest", "inf", "far"])
+def test_close_and_distant_logits(device, dtype, spread, masked):
+    """Logits that nearly all weigh the same, or nearly nothing; a mask's
+    finite value tells nothing about the others' range."""
+    logits, u = _logits(device, 4, 100001, dtype, seed=7, spread=spread)
+    if masked:
+        value = {"lowest": torch.finfo(dtype).min, "inf": -math.inf, "far": float(logits.float().min()) - 25.0}[masked]
+        logits[:, ::3] = value
+        logits[0, :99000] = value
+    for kw in (dict(top_p=0.9), dict(top_k=50), dict(top_k=5000, top_p=0.9), dict(temperature=0.0),
+               dict(temperature=3.0, top_p=0.3)):
+        ids, lp = _sample(logits, u, **kw)
+        full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(kw)
+        _verify(logits, u, ids, lp, **full)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [5, 4096, 100001])
 def test_equal_logits_exactly(device, dtype, vocab):
     """All weights equal: the token is floor(u n) of the first n kept ones."""
