@@ -22,7 +22,7 @@
 // token; 2,048 tokens 80 us; nine rows of up to 901 tokens 159 us in one pass;
 // five short prompts 29 us.  Neither memory (64 us at 8,192 tokens) nor the
 // matrix cores bound it: a chunk takes a workgroup 17,500 clocks, of which a
-// SIMD's vector instructions are about 8,700, the LDS 5,500 and the matrix
+// SIMD's vector instructions are about 8,700, the LDS 4,500 and the matrix
 // instructions 5,000, and they overlap little, as both waves of a SIMD are at
 // the same step.  Leaving parts out saves, of 218 us: S C 22, the update 40,
 // the stores 22, the loads 25, the weights 15, the scalars 10.  Not better:
@@ -40,6 +40,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
 typedef __attribute__((address_space(3))) s16x4v lds_s16x4;
 
 constexpr int kChunk = 64;
@@ -452,6 +453,13 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       const uint16_t* r = m + 16 * tile * kRowB;
       return join(*(const f16x4*)(r + (row_at ^ (32 * kk))), *(const f16x4*)(r + (row_at ^ (32 * kk + 16))));
     };
+    // The same in reads of their own (volatile): paired by the compiler, the
+    // reads of two tiles meet on the same banks (1,000 of a chunk's LDS cycles).
+    auto row_fragment_alone = [&](const uint16_t* m, int tile, int kk) {
+      const uint16_t* r = m + 16 * tile * kRowB;
+      return join(*(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk))),
+                  *(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk + 16))));
+    };
     const bool odd = OUT && xm >= 0x7c00u;
     if constexpr (OUT) {
       // ---- C B^T, the same for all heads: two waves without scalars two tiles, the others one.
@@ -526,7 +534,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
           f16x8 cf[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) cf[i] = row_fragment(ct, i, kk);
+          for (int i = 0; i < 4; ++i) cf[i] = row_fragment_alone(ct, i, kk);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
