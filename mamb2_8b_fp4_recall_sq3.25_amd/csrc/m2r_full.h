@@ -49,15 +49,30 @@ __device__ __forceinline__ float full_dt(float v) {
   return v != v ? v : y;
 }
 
-// The carry of batch row b, or -1 for an idle row; and its token count.
-__device__ __forceinline__ int64_t full_slot(const FullArgs& a, int64_t b) {
-  const int64_t s = a.slots ? (int64_t)a.slots[b] : b;
-  return s >= 0 && s < a.pool ? s : -1;
+// The carry of batch row b, or -1 for an idle row, and its token count (0 for
+// an idle row).  Both loads are issued at once, whether they are needed or not.
+struct FullRow { int64_t slot, len; };
+__device__ __forceinline__ FullRow full_row(const FullArgs& a, int64_t b) {
+  const int32_t* any = (const int32_t*)a.A;   // readable, for what is not there
+  const int32_t sv = *(a.slots ? a.slots + b : any), lv = *(a.lengths ? a.lengths + b : any);
+  const int64_t s = a.slots ? sv : b, n = a.lengths ? lv : a.L;
+  FullRow r{s >= 0 && s < a.pool ? s : -1, n < 0 ? 0 : (n < a.L ? n : a.L)};
+  if (r.slot < 0) r.len = 0;
+  return r;
 }
-__device__ __forceinline__ int64_t full_length(const FullArgs& a, int64_t b) {
-  if (!a.lengths) return a.L;
-  const int64_t n = a.lengths[b];
-  return n < 0 ? 0 : (n < a.L ? n : a.L);
+
+// Element h of a binary16 or binary32 parameter: loaded without a branch, so
+// that other loads are issued before it is waited for.
+struct FullParam {
+  uint16_t low, high;
+  int f32;
+  __device__ __forceinline__ float value() const {
+    return f32 ? __builtin_bit_cast(float, ((uint32_t)high << 16) | low) : h2f(low);
+  }
+};
+__device__ __forceinline__ FullParam full_param(const void* p, int f32, int64_t h) {
+  const uint16_t* at = (const uint16_t*)p + (f32 ? 2 * h : h);
+  return FullParam{at[0], at[f32 ? 1 : 0], f32};
 }
 
 // Many tokens in chunks, on the matrix cores (m2r_full_chunks.hip).

@@ -35,8 +35,8 @@ __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
   w /= blocks;
   const int64_t h = w % a.H, b = w / a.H;
   const int64_t g = h / (a.H / a.G);
-  const int64_t slot = full_slot(a, b);
-  const int64_t len = slot < 0 ? 0 : full_length(a, b);
+  const FullRow fr = full_row(a, b);
+  const int64_t slot = fr.slot, len = fr.len;
   // the lane that stores row 2 q + half of the wave's rows
   const bool writer = q < R && p0 + 2 * q + half < a.P;
   uint16_t* y = a.y + (b * a.L * a.H + h) * a.P + p0 + 2 * q + half;
@@ -45,13 +45,14 @@ __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
     f32x4 s[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) s[r] = p0 + 2 * r + half < a.P ? *(const f32x4*)(srow + 256 * r) : f32x4{0.f, 0.f, 0.f, 0.f};
-    const float av = a.A[h], dh = load_param(a.D, a.d_f32, (int)h), bias = load_param(a.dt_bias, a.db_f32, (int)h);
+    const float av = a.A[h];
+    const FullParam skip = full_param(a.D, a.d_f32, h), bias = full_param(a.dt_bias, a.db_f32, h);
     const uint16_t* xp = a.x + b * a.xs_b + h * a.P + p0 + half;
     const uint16_t* dp = a.dt + b * a.ds_b + h;
     const uint16_t* bp = a.Bm + b * a.bs_b + g * 128 + 4 * q;
     const uint16_t* cp = a.Cm + b * a.cs_b + g * 128 + 4 * q;
     for (int64_t t = 0; t < len; ++t) {
-      const float dt = full_dt(h2f(dp[t * a.ds_l]) + bias);
+      const float dt = full_dt(h2f(dp[t * a.ds_l]) + bias.value());
       const float decay = expf(av * dt);
       const uint16_t *bt = bp + t * a.bs_l, *ct = cp + t * a.cs_l;
       float bv[4], cv[4];
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
           acc = __builtin_fmaf(s[r][j], cv[j], acc);
         }
         acc = butterfly_add<4>(butterfly_add<3>(butterfly_add<2>(butterfly_add<1>(butterfly_add<0>(acc)))));
-        if (q == r) mine = __builtin_fmaf(xv, dh, acc);
+        if (q == r) mine = __builtin_fmaf(xv, skip.value(), acc);
       }
       if (writer) y[t * a.H * a.P] = f2h(mine);
     }

@@ -19,8 +19,8 @@
 //
 // At 128 heads of 64 in 8 groups: 8,192 tokens of one row 212 us (first pass
 // 55, join 13, main pass 142), 1.5 TB/s and 204 TFLOP/s counted token by
-// token; 2,048 tokens 80 us; nine rows of up to 901 tokens 159 us in one pass;
-// five short prompts 29 us.  Neither memory (64 us at 8,192 tokens) nor the
+// token; 2,048 tokens 80 us; nine rows of 62 to 901 tokens 128 us in one pass;
+// five short prompts 28 us.  Neither memory (64 us at 8,192 tokens) nor the
 // matrix cores bound it: a chunk takes a workgroup 17,500 clocks, of which a
 // SIMD's vector instructions are about 8,700, the LDS 4,500 and the matrix
 // instructions 5,000, and they overlap little, as both waves of a SIMD are at
@@ -93,6 +93,7 @@ struct Segments {
   // segment q - 1.
   float* state;
   float* decay;       // [count, batch, H]
+  bool longest_first; // the grid's y is a row's place by length, not its number
 };
 
 // The largest over the wave.  Non-negative binary32 values order as their
@@ -254,6 +255,19 @@ __device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
   const uint32_t lo = m & 0xffffu, hi = m >> 16;
   return wave_max_bits(lo > hi ? lo : hi);
 }
+// The row of at most 64 whose token count has the given place among them,
+// largest first.
+__device__ __forceinline__ int64_t row_by_length(const FullArgs& a, uint32_t place) {
+  const int lane = threadIdx.x & 63, rows = (int)a.batch;
+  const int n = lane < rows ? (int)full_row(a, lane).len : -1;
+  uint32_t before = 0;
+  for (int j = 0; j < rows; ++j) {
+    const int o = __builtin_amdgcn_readlane(n, j);
+    before += o > n || (o == n && j < lane);
+  }
+  return __builtin_ctzll(__ballot(lane < rows && before == place));
+}
+
 // A workgroup steps four blocks of 64 columns (a head's channels) of one
 // group, two waves each, over one segment of one batch row's tokens: four
 // blocks share the loads of B and C and the scores.  OUT: readouts and the
@@ -266,12 +280,12 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   constexpr int kAhead = ChunkShared<OUT>::kAhead, kBuffers = ChunkShared<OUT>::kBuffers;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave >> 1, half = wave & 1;
   const int lr = lane & 15, lg = lane >> 4;
-  const int hpg = (int)(a.H / a.G), per_head = (int)((a.P + 63) / 64), blocks = (hpg * per_head + 3) / 4;
+  const int hpg = (int)((uint32_t)a.H / (uint32_t)a.G), per_head = (int)((a.P + 63) / 64), blocks = (hpg * per_head + 3) / 4;
   const int g = blockIdx.x / blocks, blk = blockIdx.x - g * blocks;
-  const int64_t b = blockIdx.y, seg = blockIdx.z;
+  const int64_t b = OUT && sg.longest_first ? row_by_length(a, blockIdx.y) : blockIdx.y, seg = blockIdx.z;
 
-  const int64_t slot = full_slot(a, b);
-  const int64_t len = slot < 0 ? 0 : full_length(a, b);
+  const FullRow fr = full_row(a, b);
+  const int64_t slot = fr.slot, len = fr.len;
   const int64_t t0 = seg * sg.tokens, t1 = t0 + sg.tokens < a.L ? t0 + sg.tokens : a.L;
   const int64_t n = len < t0 ? 0 : (len < t1 ? len : t1) - t0;   // the segment's tokens
   if (!OUT && len <= t1) return;                                   // no later segment reads this one
@@ -291,7 +305,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   }
   if (n == 0) return;
 
-  const float av = a.A[h], dh = load_param(a.D, a.d_f32, (int)h), bias = load_param(a.dt_bias, a.db_f32, (int)h);
+  const float av = a.A[h];
+  const FullParam skip = full_param(a.D, a.d_f32, h), shift = full_param(a.dt_bias, a.db_f32, h);
+  float bias = 0.f, dh = 0.f;
   double seg_log = 0.0;   // the segment's decay so far, as a power of two
 
   // the loads of a chunk: B and C two, x four 16-byte pieces a thread, dt.
@@ -374,16 +390,21 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   // the carry: S[16 nt + 4 lg + i][column] as st[nt][pt][i], 2^-eS times its value
   f32x4 st[8][2];
   int eS = 0;
-  {
+  if constexpr (OUT) {
     // the row's only segment: the pool's own carry
     const float* base = seg == 0 && len <= t1 ? a.state + slot * a.H * a.P * 128 : sg.state + (seg * a.batch + b) * a.H * a.P * 128;
+    const auto sb = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + (h * a.P + pc) * 128), 0, (int)cols * 512, 0x00020000);
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt) {
-      const float* src = base + (h * a.P + pc + pw + 16 * pt) * 128 + 4 * lg;
+    for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-        st[nt][pt] = OUT && pw + 16 * pt < cols ? *(const f32x4*)(src + 16 * nt) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+      for (int nt = 0; nt < 8; ++nt)   // (zeros past the last column)
+        st[nt][pt] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(sb, (pw + 16 * pt) * 512 + 16 * lg + 64 * nt, 0, 0));
+  } else {
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) st[nt][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   float sbound = 0.f;   // a bound of the carry's magnitudes
   const int turned_at = bc_at(4 * lg + (lr >> 2), 4 * (lr & 3));   // for transposing reads of B
@@ -421,9 +442,23 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     return m;
   };
 
-  wait_vmcnt<0>();   // the transfers have landed
+  // The first chunk has landed: behind its transfers are the carry's 16 loads,
+  // which go on while the scalars are formed, or the transfers of the next.
+  if constexpr (!ALIGNED) wait_vmcnt<0>();
+  else if constexpr (OUT) wait_vmcnt<16>();
+  else if (chunks < 2) wait_vmcnt<0>();
+  else if (scalars) wait_vmcnt<7>();
+  else wait_vmcnt<6>();
+  bias = shift.value();
+  dh = skip.value();
   if (scalars) prepare(0, 0, 0);
   __syncthreads();
+  if constexpr (OUT) {   // here, so that the loop waits for no load of before it
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) asm volatile("" : "+v"(st[nt][pt]));
+  }
 
   int buf = 0;
   for (int64_t ch = 0; ch < chunks; ++ch) {
@@ -716,7 +751,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 __global__ __launch_bounds__(256) void k_full_join(FullArgs a, Segments sg) {
   const int64_t b = blockIdx.y, i = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = a.H * a.P * 32;
   if (i >= per_row) return;
-  const int64_t slot = full_slot(a, b), len = slot < 0 ? 0 : full_length(a, b);
+  const FullRow fr = full_row(a, b);
+  const int64_t slot = fr.slot, len = fr.len;
   const int64_t started = (len + sg.tokens - 1) / sg.tokens;
   if (started < 2) return;
   const int64_t h = i / (a.P * 32);
@@ -757,7 +793,7 @@ Segments full_segments(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G
   int64_t want = groups < 256 ? 256 / groups : 1;
   want = want < chunks ? want : chunks;
   const int64_t per = (chunks + want - 1) / want;
-  return Segments{per * kChunk, (int)((chunks + per - 1) / per), nullptr, nullptr};
+  return Segments{per * kChunk, (int)((chunks + per - 1) / per), nullptr, nullptr, false};
 }
 
 int64_t full_chunks_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) {
@@ -779,6 +815,14 @@ hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t st
                        (((uintptr_t)a.x | (uintptr_t)a.Bm | (uintptr_t)a.Cm | (uintptr_t)a.y) & 15) == 0 &&
                        a.xs_l >= dense && a.bs_l >= a.G * 128 && a.cs_l >= a.G * 128 && a.ds_l >= a.H &&
                        a.xs_l < far && a.bs_l < far && a.cs_l < far && a.ds_l < far;
+  // Somewhat more workgroups than compute units: the rows that take longest
+  // start first.  us for ragged rows of 32 workgroups each, so / as they come:
+  // 9 of up to 901 tokens 128 / 154, 12 of up to 901 141 / 166, 20 of up to 600
+  // 173 / 182; more rows even out by themselves, and their short ones, which
+  // mostly move carries, run better among long ones: 40 of up to 300 218 / 209,
+  // 64 of up to 150 253 / 221.
+  const int64_t groups = blocks * a.G * a.batch;
+  sg.longest_first = a.lengths && a.batch <= 64 && groups > 256 && groups <= 768;
   const dim3 block(512);
   dim3 grid((unsigned)(blocks * a.G), (unsigned)a.batch, (unsigned)sg.count);
   if (sg.count > 1) {

@@ -150,6 +150,21 @@ def test_magnitudes(device, scale, dt_shift):
     _check(i, *_scan(i), _reference(i), 130)
 
 
+@pytest.mark.parametrize("batch", [17, 48, 64])
+def test_rows_out_of_order(device, batch):
+    """More workgroups than compute units with ragged, equal, absent and
+    impossible lengths and idle rows, in whatever order they are taken."""
+    tokens = 100
+    i = _inputs(device, batch, tokens, heads=64 if batch < 20 else 24, dim=64, groups=2, pool=batch + 3, seed=43)
+    gen = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, tokens + 1, (batch,), generator=gen)
+    lengths[:8] = torch.tensor([0, tokens, 64, 64, -5, tokens + 7, 1, tokens])
+    slots = torch.randperm(batch + 3, generator=gen)[:batch]
+    slots[3], slots[9] = -1, batch + 3
+    kw = dict(lengths=lengths.to(torch.int32).to(device), slots=slots.to(torch.int32).to(device))
+    _check(i, *_scan(i, **kw), _reference(i, **kw), tokens)
+
+
 @pytest.mark.parametrize("batch,tokens", [(200, 8256), (1, 20000)])
 def test_long_memory(device, batch, tokens):
     """Carries that hardly decay over many chunks, in one segment (many rows)
