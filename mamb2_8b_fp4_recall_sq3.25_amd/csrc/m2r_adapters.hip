@@ -91,33 +91,46 @@ __device__ __forceinline__ int only_group(int id, int member, uint32_t& rows) {
 
 // One wave per (tile, slice of K / 4): its four quarters meet in LDS.  (More
 // loads in flight at a time, three to six steps', changed nothing.)
-// RT: 16-rank tiles at a time.
-template <int RT>
+// RT: 16-rank tiles at a time.  MT: row tiles.
+template <int RT, int MT>
 __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
-  __shared__ f32x4 part[3][RT][64];
+  __shared__ f32x4 part[3][MT * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
   uint32_t w = blockIdx.x;   // (64-bit divisions here would take a microsecond)
   const int member = (int)(w % (uint32_t)a.members);
   w /= (uint32_t)a.members;
   const int slice = (int)(w % (uint32_t)a.slices);
-  const int64_t m0 = (int64_t)(w / (uint32_t)a.slices) * 16, m = m0 + lr;
-  const int id = adapter_of(a, m);
-  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xffffu;
+  const int64_t m0 = (int64_t)(w / (uint32_t)a.slices) * (16 * MT);
+  int id[MT];
+  uint32_t todo = 0;
+  const uint16_t* xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + 16 * i + lr;
+    id[i] = adapter_of(a, m);
+    todo |= ((uint32_t)__ballot(id[i] >= 0) & 0xffffu) << (16 * i);
+    xr[i] = a.x + (m < a.M ? m : a.M - 1) * a.xs;
+  }
+  int group = 0;
+  if (MT == 1 && a.members == 16) group = only_group(id[0], member, todo);
   const int64_t quarter = (a.slice / 64 + 3) / 4 * 64;
   const int64_t s1 = (slice + 1) * a.slice < a.Kp ? (slice + 1) * a.slice : a.Kp;
   const int64_t k0 = slice * a.slice + wave * quarter, k1 = k0 + quarter < s1 ? k0 + quarter : s1;
-  const uint16_t* xr = a.x + (m < a.M ? m : a.M - 1) * a.xs;
-  int group = 0;
-  if (a.members == 16) group = only_group(id, member, todo);
   for (; todo; ++group) {
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-    const bool mine = id == cur;
-    todo &= ~(uint32_t)__ballot(mine);
-    if ((group & (a.members - 1)) != member) continue;
-    for (int r0 = 0; r0 < a.r; r0 += 16 * RT) {
-      f32x4 acc[RT];
+    const int first = __builtin_ctz(todo);
+    int cur = 0;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT; ++i)
+      if (first >> 4 == i) cur = __builtin_amdgcn_readlane(id[i], first & 15);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) todo &= ~(((uint32_t)__ballot(id[i] == cur) & 0xffffu) << (16 * i));
+    if (MT == 1 && (group & (a.members - 1)) != member) continue;
+    for (int r0 = 0; r0 < a.r; r0 += 16 * RT) {
+      f32x4 acc[MT][RT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
       const uint16_t* dr[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {   // ranks past the last read its row and are not stored
@@ -128,12 +141,13 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
       // the pair of loads covers whole 128-byte lines of a row
 #pragma unroll 2
       for (int64_t kb = k0; kb < k1; kb += 64) {
-        f16x8 xv[2], dv[2][RT];
+        f16x8 xv[2][MT], dv[2][RT];
         if (kb + 64 <= k1 && kb + 64 <= a.K) {   // (one answer for the wave)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int64_t k = kb + 16 * lg + 8 * u;
-            xv[u] = __builtin_bit_cast(f16x8, load_h16x8(xr + k));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[u][i] = __builtin_bit_cast(f16x8, load_h16x8(xr[i] + k));
 #pragma unroll
             for (int t = 0; t < RT; ++t) dv[u][t] = __builtin_bit_cast(f16x8, load_h16x8(dr[t] + k));
           }
@@ -142,7 +156,8 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
           for (int u = 0; u < 2; ++u) {
             const int64_t k = kb + 16 * lg + 8 * u;
             const bool in = k < k1;
-            xv[u] = load_f16x8(xr + k, in ? a.K - k : 0);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[u][i] = load_f16x8(xr[i] + k, in ? a.K - k : 0);
 #pragma unroll
             for (int t = 0; t < RT; ++t) dv[u][t] = load_f16x8(dr[t] + k, in ? 8 : 0);
           }
@@ -150,22 +165,32 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int t = 0; t < RT; ++t) acc[t] = mfma16(dv[u][t], xv[u], acc[t]);
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[i][t] = mfma16(dv[u][t], xv[u][i], acc[i][t]);
       }
       __syncthreads();
       if (wave) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) part[wave - 1][t][lane] = acc[t];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) part[wave - 1][i * RT + t][lane] = acc[i][t];
       }
       __syncthreads();
-      if (wave == 0 && mine && m < a.M) {   // columns = rows m, rows = ranks 4 lg ...
+      if (wave == 0) {   // columns = rows m, rows = ranks 4 lg ...
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          f32x4 v = acc[t];
+        for (int i = 0; i < MT; ++i) {
+          const int64_t m = m0 + 16 * i + lr;
+          if (id[i] == cur && m < a.M) {
 #pragma unroll
-          for (int q = 0; q < 3; ++q) v += part[q][t][lane];
-          const int j = r0 + 16 * t + 4 * lg;
-          if (j < a.r) *(f32x4*)(a.hidden + (slice * a.M + m) * a.r + j) = v;
+            for (int t = 0; t < RT; ++t) {
+              f32x4 v = acc[i][t];
+#pragma unroll
+              for (int q = 0; q < 3; ++q) v += part[q][i * RT + t][lane];
+              const int j = r0 + 16 * t + 4 * lg;
+              if (j < a.r) *(f32x4*)(a.hidden + (slice * a.M + m) * a.r + j) = v;
+            }
+          }
         }
       }
     }
@@ -377,6 +402,10 @@ static int adapter_members(int64_t M) {
   while (members < most && members < M) members *= 2;
   return members;
 }
+// From here on two tiles share the loads of `down` in the first launch.  us a
+// call with one / two, K = N = 4,096: 2,500 rows of rank 32, N = 18,560, 72 /
+// 75; 8,000 rows of rank 16 60 / 57, of rank 128 199 / 169.
+constexpr int64_t kPairRows = 4096;
 // Waves to aim for in the second launch (2,500 rows of rank 32, N = 18,560: 4,096
 // and 6,144 waves 1 to 2 us slower, 3,072 by 11).
 constexpr int64_t kSpanWaves = 8192;
@@ -386,7 +415,7 @@ static void adapter_plan(AdapterArgs& a) {
   a.members = adapter_members(a.M);
   // Slices of K for about 512 workgroups, of at least 512 each and at most four,
   // since the second launch adds them up for each span.
-  int64_t s = 512 / (tiles * a.members);
+  int64_t s = 512 / (a.M > kPairRows ? (tiles + 1) / 2 : tiles * a.members);
   const int64_t most = (a.Kp + 511) / 512;
   s = s < most ? s : most;
   s = s < 1 ? 1 : (s > 4 ? 4 : s);
@@ -426,15 +455,22 @@ extern "C" int m2r_adapters_add(const void* x, int64_t x_stride, const void* bas
   adapter_plan(a);
   const int64_t tiles = (M + 15) / 16;
   if (tiles * a.members * a.slices > 0x7fffffff) return m2r_fail("adapters: grid limits exceeded");
-  const dim3 down_grid((unsigned)(tiles * a.members * a.slices)), block(256);
-  if (rank <= 16) hipLaunchKernelGGL(k_adapter_down<1>, down_grid, block, 0, stream, a);
-  else if (rank <= 32) hipLaunchKernelGGL(k_adapter_down<2>, down_grid, block, 0, stream, a);
-  else hipLaunchKernelGGL(k_adapter_down<4>, down_grid, block, 0, stream, a);
+  const bool pairs = M > kPairRows;
+  const dim3 down_grid((unsigned)((pairs ? (tiles + 1) / 2 : tiles * a.members) * a.slices)), block(256);
+  if (pairs) {
+    if (rank <= 16) hipLaunchKernelGGL((k_adapter_down<1, 2>), down_grid, block, 0, stream, a);
+    else if (rank <= 32) hipLaunchKernelGGL((k_adapter_down<2, 2>), down_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_down<4, 2>), down_grid, block, 0, stream, a);
+  } else {
+    if (rank <= 16) hipLaunchKernelGGL((k_adapter_down<1, 1>), down_grid, block, 0, stream, a);
+    else if (rank <= 32) hipLaunchKernelGGL((k_adapter_down<2, 1>), down_grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_adapter_down<4, 1>), down_grid, block, 0, stream, a);
+  }
   int rc = m2r_check(hipGetLastError(), "adapters down launch");
   if (rc) return rc;
   // Two tiles share a pass over `up` where rows are many and the rank leaves
   // registers for both (2,048 rows of rank 128: 90 us with one, 107 with two).
-  const bool wide = a.M > kMemberRows && rank <= 64;
+  const bool wide = M > kMemberRows && rank <= 64;
   const int64_t groups = wide ? (M + 31) / 32 : tiles * a.members;
   int64_t spans = kSpanWaves / groups;
   const int64_t most = (N + 63) / 64;

@@ -60,6 +60,16 @@ def test_sizes(device, rows, k, n, rank):
     _check(c, _add(c))
 
 
+@pytest.mark.parametrize("rank", [9, 32, 48])
+def test_many_rows(device, rank):
+    """More rows than one tile at a time is for, an odd number of tiles; every
+    row its own adapter, and runs of rows with one."""
+    c = _case(device, 4120, 200, 136, 7, rank, seed=rank)
+    _check(c, _add(c))
+    c["ids"] = (torch.arange(4120, device=device) // 311 % 9 - 1).to(torch.int32)
+    _check(c, _add(c))
+
+
 @pytest.mark.parametrize("rows", [1, 40, 500])
 def test_requests_side_by_side(device, rows):
     """Rows of a request next to each other, changes inside a tile."""
