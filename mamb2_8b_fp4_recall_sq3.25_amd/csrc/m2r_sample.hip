@@ -22,7 +22,9 @@
 // them and draw).  One row of binary16, filtered: 23 us, three launches of a
 // few dependent steps; 24 rows of 50,003 without filters: 13 us.  Logits that
 // are all close (normal, deviation 0.02 to 1; top-p 0.9): 64 rows 64 to 70 us,
-// where bins of a fixed 1/16 left lists that did not fit (1,350 us).
+// where bins of a fixed 1/16 left lists that did not fit (1,350 us).  All
+// logits equal, cut by a workgroup a row: one row 145 to 210 us, 64 rows 360 to
+// 470 (14,000 with a counter's atomics from every lane).
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
@@ -647,28 +649,88 @@ __device__ Place select_place(SampleShared& s, uint32_t n, const RowFilter& f, u
 
 struct Cut { uint32_t key; uint64_t count, weight; };   // tokens and weight before the key's first one
 
+// The bits that any and that all of the row's keys have, tokens of weight 0 aside.
+struct KeyBits { uint32_t any, each; };
+template <int DT>
+__device__ KeyBits key_bits(SampleShared& s, const void* row, int64_t V, const RowFilter& f) {
+  uint32_t any = 0, each = ~0u;
+#pragma unroll 4
+  for (int64_t i = 8 * threadIdx.x; i < V; i += kBlock) {
+    float v[8];
+    load_logits<DT>(row, i, V, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t key = order_key(v[j]);
+      const bool in = weight_of(f, v[j]) != 0;
+      any |= in ? key : 0;
+      each &= in ? key : ~0u;
+    }
+  }
+#pragma unroll
+  for (int by = 32; by; by >>= 1) {
+    any |= (uint32_t)__shfl_xor((int)any, by);
+    each &= (uint32_t)__shfl_xor((int)each, by);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = ((uint64_t)any << 32) | each;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    any |= (uint32_t)(s.part[i] >> 32);
+    each &= (uint32_t)s.part[i];
+  }
+  return KeyBits{any, each};
+}
+
 // The key at which the sorted row's running count (BY_WEIGHT: weight) reaches
-// `target`, digit by digit; tokens of weight 0 do not count.  The target must
-// be reached.
+// `target`, up to 8 bits at a time from the first that differs; tokens of
+// weight 0 do not count.  The target must be reached.
 template <int DT, bool BY_WEIGHT>
-__device__ Cut select_key(SampleShared& s, const void* row, int64_t V, const RowFilter& f, uint64_t target) {
-  Cut c{0, 0, 0};
+__device__ Cut select_key(SampleShared& s, const void* row, int64_t V, const RowFilter& f, KeyBits bits, uint64_t target) {
+  Cut c{bits.each, 0, 0};
   uint64_t* sum = s.list;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  int top = bits.any == bits.each ? 0 : 32 - __builtin_clz(bits.any ^ bits.each), shift;
+  if (top) c.key = top == 32 ? 0 : bits.each >> top << top;   // what all share
+  for (; top; top = shift) {
+    shift = top > 8 ? top - 8 : 0;
+    const uint32_t mask = (1u << (top - shift)) - 1;
     __syncthreads();
     s.cnt[threadIdx.x] = 0;
     sum[threadIdx.x] = 0;
     __syncthreads();
-    for (int64_t i = 8 * threadIdx.x; i < V; i += kBlock) {
+    // (whole waves step together: the last block's lanes past the row load nothing)
+    for (int64_t i0 = 0; i0 < V; i0 += kBlock) {
+      const int64_t i = i0 + 8 * threadIdx.x;
       float v[8];
       load_logits<DT>(row, i, V, v);
+      uint32_t w[8], digit[8];
+      int mine = -1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t key = order_key(v[j]), w = weight_of(f, v[j]);
-        if (w && (shift == 24 || (key >> (shift + 8)) == (c.key >> (shift + 8)))) {
-          atomicAdd(&s.cnt[(key >> shift) & 255], 1u);
-          atomicAdd((unsigned long long*)&sum[(key >> shift) & 255], (unsigned long long)w);
+      for (int j = 7; j >= 0; --j) {
+        const uint32_t key = order_key(v[j]);
+        w[j] = top == 32 || (key >> top) == (c.key >> top) ? weight_of(f, v[j]) : 0;
+        digit[j] = (key >> shift) & mask;
+        mine = w[j] ? (int)digit[j] : mine;
+      }
+      // equal logits would queue at one counter: the wave's tokens of one digit go together
+      const uint64_t with = __ballot(mine >= 0);
+      if (!with) continue;
+      const uint32_t lead = (uint32_t)__builtin_amdgcn_readlane(mine, __builtin_ctzll(with));
+      uint64_t together = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (w[j]) {
+          if (digit[j] == lead) {
+            together += (1ull << 46) | w[j];
+          } else {
+            atomicAdd(&s.cnt[digit[j]], 1u);
+            atomicAdd((unsigned long long*)&sum[digit[j]], (unsigned long long)w[j]);
+          }
         }
+      together = wave_scan64(together);
+      if ((threadIdx.x & 63) == 63) {
+        atomicAdd(&s.cnt[lead], (uint32_t)(together >> 46));
+        atomicAdd((unsigned long long*)&sum[lead], (unsigned long long)(together & ((1ull << 46) - 1)));
       }
     }
     __syncthreads();
@@ -704,15 +766,16 @@ template <int DT>
 __device__ uint64_t cut_row(SampleShared& s, const RowWork& rw, const void* row, int64_t V, const RowFilter& f) {
   uint32_t key = 0;
   uint64_t ties = 0, all = rw.all;
+  const KeyBits bits = key_bits<DT>(s, row, V, f);
   if (rw.bk < (uint32_t)kBins) {
-    const Cut c = select_key<DT, false>(s, row, V, f, f.k);
+    const Cut c = select_key<DT, false>(s, row, V, f, bits, f.k);
     key = c.key;
     ties = f.k - c.count;
     all = c.weight + ties * weight_of(f, logit_of(key));
   }
   if (f.p < 1.0) {   // at or above the top-k cut: the mass is at most all
     const uint64_t mass = mass_of(f.p, all);
-    const Cut c = select_key<DT, true>(s, row, V, f, mass);
+    const Cut c = select_key<DT, true>(s, row, V, f, bits, mass);
     const uint64_t each = weight_of(f, logit_of(c.key));
     key = c.key;
     ties = (mass - c.weight + each - 1) / each;
@@ -720,17 +783,22 @@ __device__ uint64_t cut_row(SampleShared& s, const RowWork& rw, const void* row,
   // the index of the last of the key's `ties` first tokens
   __syncthreads();
   if (threadIdx.x == 0) s.found[0] = 0xffffffffu;
-  for (int64_t i0 = 0; i0 < V; i0 += kBlock) {
-    const int64_t i = i0 + 8 * threadIdx.x;
-    float v[8];
-    load_logits<DT>(row, i, V, v);
+  constexpr int kWide = 2;   // blocks at a time
+  for (int64_t i0 = 0; i0 < V; i0 += kWide * kBlock) {
+    const int64_t i = i0 + 8 * kWide * threadIdx.x;
+    float v[8 * kWide];
+#pragma unroll
+    for (int q = 0; q < kWide; ++q) load_logits<DT>(row, i + 8 * q, V, v + 8 * q);
     uint64_t n = 0, block;
-    for (int j = 0; j < 8; ++j) n += i + j < V && order_key(v[j]) == key;
+#pragma unroll
+    for (int j = 0; j < 8 * kWide; ++j) n += i + j < V && order_key(v[j]) == key;
     uint64_t run = block_scan64(s, n, block);
     if (ties <= block) {
-      for (int j = 0; j < 8; ++j) {
-        run += i + j < V && order_key(v[j]) == key;
-        if (run == ties && i + j < V && order_key(v[j]) == key) s.found[0] = (uint32_t)(i + j);
+#pragma unroll
+      for (int j = 0; j < 8 * kWide; ++j) {
+        const bool in = i + j < V && order_key(v[j]) == key;
+        run += in;
+        if (in && run == ties) s.found[0] = (uint32_t)(i + j);
       }
       break;
     }
@@ -741,7 +809,7 @@ __device__ uint64_t cut_row(SampleShared& s, const RowWork& rw, const void* row,
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp, RowWork* work) {
+__global__ __launch_bounds__(kThreads, 4) void k_sample_draw(SampleArgs a, Split sp, RowWork* work) {
   __shared__ SampleShared s;
   const Piece p = my_piece(sp, a.V);
   RowWork& rw = work[p.row];
@@ -757,10 +825,11 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs a, Split sp
     __syncthreads();
     s.unit[tid] = 0;
     __syncthreads();
-    for (int q = 0; q < sp.units; ++q) {
+    for (int q = tid >> 6; q < sp.units; q += kThreads / 64) {   // a unit for each wave
       const int64_t first = q * sp.unit, end = first + sp.unit < a.V ? first + sp.unit : a.V;
       uint64_t sum = 0;
-      for (int64_t i = first + 8 * tid; i < end; i += kBlock) {
+#pragma unroll 4
+      for (int64_t i = first + 8 * (tid & 63); i < end; i += 512) {
         float v[8];
         load_logits<DT>(row, i, a.V, v);
 #pragma unroll

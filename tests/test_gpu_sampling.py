@@ -140,6 +140,23 @@ def test_equal_logits_exactly(device, dtype, vocab):
         assert torch.allclose(lp.double().cpu(), torch.full((5,), -math.log(n), dtype=torch.float64), atol=1e-6, rtol=1e-6)
 
 
+@pytest.mark.parametrize("values", [[0.5, 0.25], [0.0, -0.0, 3.0, -1.0], [1.0, 1.0009765625, 1.001953125, 0.5, -30.0]])
+@pytest.mark.parametrize("vocab", [30000, 100001])
+def test_few_values_among_many_tokens(device, values, vocab):
+    """Thousands of tokens of each logit: more than a list holds, cut inside
+    one value's tokens by count and by weight."""
+    gen = torch.Generator(device=device).manual_seed(vocab)
+    pick = torch.randint(0, len(values), (5, vocab), generator=gen, device=device)
+    logits = torch.tensor(values, device=device)[pick]
+    u = torch.rand(5, generator=gen, device=device)
+    for kw in (dict(top_k=7000), dict(top_k=vocab - 3), dict(top_p=0.37), dict(top_k=9999, top_p=0.8, min_p=0.3),
+               dict(temperature=0.0), dict(temperature=0.02, top_p=0.5)):
+        ids, lp = _sample(logits, u, **kw)
+        full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(kw)
+        _verify(logits, u, ids, lp, **full)
+
+
 def test_ties_go_to_the_lowest_index(device):
     logits = torch.full((3, 9000), -8.0, dtype=torch.float16, device=device)
     logits[:, [17, 4000, 8000, 8999]] = 4.0
