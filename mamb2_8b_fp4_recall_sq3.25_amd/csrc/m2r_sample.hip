@@ -20,7 +20,7 @@
 // first two read at 5.3 and 3.4 TB/s; the last ends with its heaviest row (19
 // us to gather thousands of listed tokens, then 11 in one workgroup to order
 // them and draw).  One row of binary16, filtered: 23 us, three launches of a
-// few dependent steps; 24 rows of 50,003 without filters: 13 us.  Logits that
+// few dependent steps; 24 rows of 50,003 without filters: 12 us.  Logits that
 // are all close (normal, deviation 0.02 to 1; top-p 0.9): 64 rows 64 to 70 us,
 // where bins of a fixed 1/16 left lists that did not fit (1,350 us).  All
 // logits equal, cut by a workgroup a row: one row 145 to 210 us, 64 rows 360 to
@@ -920,7 +920,10 @@ static void launch_sample(const SampleArgs& a, const Split& sp, RowWork* work, h
   const dim3 grid((unsigned)(a.batch * sp.pieces)), block(kThreads);
   hipLaunchKernelGGL(k_sample_top<DT>, grid, block, 0, stream, a, sp, work);
   hipLaunchKernelGGL(k_sample_bins<DT>, grid, block, 0, stream, a, sp, work);
-  hipLaunchKernelGGL(k_sample_draw<DT>, grid, block, 0, stream, a, sp, work);
+  // where no row can have top-k or top-p the second launch has drawn them all
+  const bool filtered = a.temperature || a.top_k || a.top_p || !(a.temperature_s > 0.f) ||
+                        (a.top_k_s > 0 && a.top_k_s < a.V) || a.top_p_s < 1.f;
+  if (filtered) hipLaunchKernelGGL(k_sample_draw<DT>, grid, block, 0, stream, a, sp, work);
 }
 
 }  // namespace m2r
