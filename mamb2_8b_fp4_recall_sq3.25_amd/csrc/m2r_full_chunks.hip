@@ -281,7 +281,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave >> 1, half = wave & 1;
   const int lr = lane & 15, lg = lane >> 4;
   const int hpg = (int)((uint32_t)a.H / (uint32_t)a.G), per_head = (int)((a.P + 63) / 64), blocks = (hpg * per_head + 3) / 4;
-  const int g = blockIdx.x / blocks, blk = blockIdx.x - g * blocks;
+  // A group's blocks G apart, on one XCD where G is a multiple of 8: B and C come
+  // into one L2 (8,192 tokens: 213 MB read for 322, in the same time).
+  const int blk = (int)(blockIdx.x / (uint32_t)a.G), g = (int)(blockIdx.x - blk * (uint32_t)a.G);
   const int64_t b = OUT && sg.longest_first ? row_by_length(a, blockIdx.y) : blockIdx.y, seg = blockIdx.z;
 
   const FullRow fr = full_row(a, b);
