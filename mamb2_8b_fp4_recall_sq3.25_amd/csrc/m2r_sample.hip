@@ -16,7 +16,7 @@
 // Each logit has to be read once; here it is read two or three times, mostly
 // from the caches, since a weight needs the row's largest logit and a cut the
 // row's whole weight.  64 rows of 256,000 binary32 logits (65 MB, 13 us for a
-// copy), with filters of all kinds: 63 us, the launches 12, 19 and 29.  The
+// copy), with filters of all kinds: 63 us, the launches 12, 19 and 32.  The
 // first two read at 5.3 and 3.4 TB/s; the last ends with its heaviest row (19
 // us to gather thousands of listed tokens, then 11 in one workgroup to order
 // them and draw).  One row of binary16, filtered: 23 us, three launches of a

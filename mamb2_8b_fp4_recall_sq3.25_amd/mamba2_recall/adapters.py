@@ -64,6 +64,22 @@ def _rows(t, features, what):
     return t, rows, stride if rows > 1 else features
 
 
+def _taken(base, x, ids, adapters):
+    """The rows of a call with dense operands, conditions checked at once (a
+    call of a few rows is bound by the host); 0 for any other call."""
+    k, n = adapters.features
+    try:
+        shape = ids.shape
+        if (base.dtype is torch.float16 and x.dtype is torch.float16 and ids.dtype is torch.int32
+                and base.shape == (*shape, n) and x.shape == (*shape, k)
+                and base.is_contiguous() and x.is_contiguous() and ids.is_contiguous()
+                and base.get_device() == x.get_device() == ids.get_device() == adapters.down.get_device()):
+            return ids.numel()
+    except AttributeError:
+        pass
+    return 0
+
+
 def add(base, x, adapters, ids, out=None):
     """base[..., N] plus each row's adapter update of x[..., K]; a new FP16
     tensor, or `out` (which may be `base`).  `ids` int32[...] names each row's
@@ -72,26 +88,29 @@ def add(base, x, adapters, ids, out=None):
     if not isinstance(adapters, AdapterSet):
         raise ValueError("adapters must be an AdapterSet")
     k, n = adapters.features
-    shape = tuple(base.shape) if isinstance(base, torch.Tensor) else None
-    b2, rows, bs = _rows(base, n, "base")
-    x2, xrows, xs = _rows(x, k, "x")
-    if rows != xrows or shape[:-1] != tuple(x.shape[:-1]):
-        raise ValueError("base and x must have the same rows")
-    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or tuple(ids.shape) != shape[:-1]:
-        raise ValueError("ids must be int32, one for each row")
-    if any(t.device != base.device for t in (x, ids, adapters.down)):
-        raise ValueError("Adapter operands must share one device")
+    rows = _taken(base, x, ids, adapters)
+    if rows:
+        b2, x2, bs, xs = base, x, n, k
+    else:
+        b2, rows, bs = _rows(base, n, "base")
+        x2, xrows, xs = _rows(x, k, "x")
+        if rows != xrows or base.shape[:-1] != x.shape[:-1]:
+            raise ValueError("base and x must have the same rows")
+        if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.shape != base.shape[:-1]:
+            raise ValueError("ids must be int32, one for each row")
+        if any(t.device != base.device for t in (x, ids, adapters.down)):
+            raise ValueError("Adapter operands must share one device")
+        ids = ids.contiguous()
     if out is None:
-        out = torch.empty(shape, dtype=torch.float16, device=base.device)
-    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or tuple(out.shape) != shape
+        out = torch.empty_like(base, memory_format=torch.contiguous_format)
+    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or out.shape != base.shape
           or out.device != base.device or not out.is_contiguous()):
         raise ValueError("out must be contiguous FP16 of base's shape")
     if rows == 0:
         return out
-    ids = ids.contiguous()
     rank = adapters.rank
     ws_bytes = int(_native.lib().m2r_adapters_workspace(rows, k, n, rank))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=base.device)
+    ws = base.new_empty(ws_bytes, dtype=torch.uint8)
     p = _native.ptr
     with _native.device_of(base):
         _native.call("m2r_adapters_add", p(x2), xs, p(b2), bs, p(adapters.down), p(adapters.up), p(adapters.scale),

@@ -112,7 +112,7 @@ def scan(x, dt, A, B, C, D, dt_bias, state, *, lengths=None, slots=None):
     A, D, dt_bias = A.contiguous(), D.contiguous(), dt_bias.contiguous()
     lengths = lengths.contiguous() if lengths is not None else None
     slots = slots.contiguous() if slots is not None else None
-    y = torch.empty((batch, length, heads, dim), dtype=torch.float16, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     ws, ws_bytes = None, 0
     if length > 1:
         ws_bytes = _native.lib().m2r_full_scan_workspace(batch, length, heads, dim, groups)

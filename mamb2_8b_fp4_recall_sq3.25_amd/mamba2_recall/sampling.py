@@ -53,15 +53,15 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     k, k_all = _filter(top_k, "top_k", torch.int32, logits, 0, 2 ** 31 - 1)
     tp, tp_all = _filter(top_p, "top_p", torch.float32, logits, 0.0, 1.0)
     mp, mp_all = _filter(min_p, "min_p", torch.float32, logits, 0.0, 1.0)
-    ids = torch.empty(batch, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(batch, dtype=torch.float32, device=logits.device)
+    ids = logits.new_empty(batch, dtype=torch.int64)
+    logprobs = torch.empty_like(uniforms, memory_format=torch.contiguous_format)
     if batch == 0:
         return ids, logprobs
     if vocab > 1 and logits.stride(1) != 1 or batch > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()
     ws_bytes = int(_native.lib().m2r_sample_workspace(batch, vocab))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
+    ws = logits.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     p = _native.ptr
     with _native.device_of(logits):
         _native.call("m2r_sample", p(logits), _DTYPES[logits.dtype], logits.stride(0) if batch > 1 else vocab,
