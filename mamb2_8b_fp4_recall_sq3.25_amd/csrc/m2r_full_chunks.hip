@@ -497,7 +497,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       return join(*(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk))),
                   *(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk + 16))));
     };
-    const bool odd = OUT && xm >= 0x7c00u;
+    const bool odd = OUT && (xm >= 0x7c00u || hs.tot > 1.0f);
     if constexpr (OUT) {
       // ---- C B^T, the same for all heads: two waves without scalars two tiles, the others one.
       // Tile (j, i): rows tokens 16 j + 4 lg + r (B), columns tokens 16 i + lr (C).
@@ -526,7 +526,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       const int kS = 13 - exponent_of(smax) > 100 ? 100 : 13 - exponent_of(smax);   // in units of st
       if (odd) {
         // A non-finite x must not reach earlier tokens, which the matrix
-        // products would let it do (0 * inf): this chunk token by token.
+        // products would let it do (0 * inf); and where the carry grows (a
+        // positive A) the last tokens' weights would set the first ones' scale:
+        // this chunk token by token.
         const float undo = pow2(-eS);
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
@@ -586,13 +588,12 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 
       if (!odd) {
         // ---- masked scores and their product with x.  Below the diagonal
-        // tiles the decay is 2^(l_t - r_j) 2^(r_j - l_s), no factor above 1
-        // for a negative A; D joins the diagonal.
+        // tiles the decay is 2^(l_t - r_j) 2^(r_j - l_s), no factor above 1;
+        // D joins the diagonal.
         float gmax = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) gmax = __builtin_fmaxf(gmax, s.gmax[k]);
-        const float tot = hs.tot;
-        float mb = gmax * hs.dtmax * (tot > 1.f ? tot : 1.f) + __builtin_fabsf(dh);   // bounds the weights
+        float mb = gmax * hs.dtmax + __builtin_fabsf(dh);   // bounds the weights
         // Weights below 2^15.  Below 2^-25 one times any x is nothing in the
         // readout; and without a finite bound there is no scale to choose.
         int km = mb < __builtin_inff() ? 13 - exponent_of(mb) : 0;

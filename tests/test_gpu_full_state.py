@@ -150,6 +150,21 @@ def test_magnitudes(device, scale, dt_shift):
     _check(i, *_scan(i), _reference(i), 130)
 
 
+@pytest.mark.parametrize("rate,tokens,scale", [(0.0, 130, 1.0), (0.4, 130, 1e-2), (1.5, 70, 1e-5), (1.5, 3, 1.0)])
+@pytest.mark.parametrize("batch", [1, 20])
+def test_carries_that_grow(device, rate, tokens, scale, batch):
+    """A of 0 and above on every other head, the carry e^20 times as large at the end."""
+    i = _inputs(device, batch, tokens, heads=4, seed=44, scale=scale)
+    i["A"][::2] = rate
+    y, state = _scan(i)
+    ry, ym, rs, sm = _reference(i)
+    beyond = ry.abs() >= 65520 * (1 + 2.0 ** -10)      # binary16's infinity, whatever the last bits
+    assert torch.equal(y[beyond].double(), ry[beyond].sign() * math.inf)
+    near = (ry.abs() > 65504 * (1 - 2.0 ** -10)) & ~beyond
+    y = torch.where(beyond | near, ry, y.double())
+    _check(i, y, state, (ry, ym, rs, sm), tokens)
+
+
 @pytest.mark.parametrize("batch", [17, 48, 64])
 def test_rows_out_of_order(device, batch):
     """More workgroups than compute units with ragged, equal, absent and
