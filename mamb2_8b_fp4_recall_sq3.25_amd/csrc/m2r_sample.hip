@@ -78,7 +78,9 @@ __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, int64_t row
   RowFilter f;
   f.top = -__builtin_inff();
   f.fine = 0.f;
-  f.rate = (1.0f / (greedy ? 1.0f : t)) * 0x1.715476p+0f;
+  // (2^126 stands for whatever lies above, infinity too: at a rate of 0 a masked
+  // token, and what is read past the row's end, would weigh as much as the likeliest)
+  f.rate = (1.0f / (greedy ? 1.0f : __builtin_fminf(t, 0x1p126f))) * 0x1.715476p+0f;
   f.k = greedy ? 1 : (k > 0 && k < a.V ? k : a.V);
   f.p = p < 1.f ? (double)p : 1.0;
   const double least = m > 0.f ? __builtin_ceil((m < 1.f ? (double)m : 1.0) * 0x1p31) : 1.0;

@@ -30,7 +30,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     logits[B,V] in FP16, BF16 or FP32 (unit column stride); uniforms FP32[B]
     in [0, 1).  Filters are numbers, or tensors with a value for each row
     (FP32; top_k int32), applied in this order: temperature (0: the likeliest
-    token, the lowest index of equal ones), top_k (0: off; equal logits in
+    token, the lowest index of equal ones; a tensor's may be infinite: all
+    tokens above -inf alike), top_k (0: off; equal logits in
     the order of their indices), top_p of what top_k left (the shortest
     prefix of the sorted row that holds it, at least one token), min_p
     relative to the likeliest token.  The token is found by the inverse of
