@@ -4,13 +4,17 @@
 //   y_t = sum_{s <= t} (C_t . B_s) exp(l_t - l_s) dt_s x_s + exp(l_t) S C_t + D x_t
 //   S'  = exp(l_63) S + sum_s exp(l_63 - l_s) dt_s x_s (x) B_s.
 // The products run on binary16 matrix instructions that sum in binary32.  B, C
-// and x are binary16 already; what is not (the carry, the weighted scores, the
-// weighted x) goes in as two of them, 22 bits, scaled by a power of two that
-// keeps the largest value near the top of the range.  The running sums l are
-// formed in 64 bits, since differences of them become exponents.
+// and x are binary16 already; what is not goes in as several of them, scaled by
+// a power of two that keeps the largest value near the top of the range.  The
+// carry and the weighted x take two, 22 bits and nothing below 2^-39 of the
+// largest, with a power of two for each channel, since channels do not meet in
+// any product.  The weighted scores take three, down to 2^-62: decays and inputs
+// that lie far apart spread them further.  The running sums l are formed in 64
+// bits, since differences of them become exponents.
 //
-// Work: a chunk and head of 64 costs 3 products of 64 x 64 x 128, the last two
-// twice for the halves, and 64 x 64 weights; x, y, B, C and dt move once, the
+// Work: a chunk and head of 64 costs 3 products of 64 x 64 x 128 (C B^T once for
+// all heads of a group), the last two twice for the halves, and 64 x 64 weights,
+// whose product with x runs three times; x, y, B, C and dt move once, the
 // carry stays in registers across a segment (64 values a thread, which is why
 // a workgroup is 512 threads of 256 registers).  What few rows lack in
 // workgroups is made up by cutting the tokens into segments: a first pass
@@ -67,7 +71,7 @@ struct ChunkScalars {
   float ws[kOut];                 // dt 2^(r_tile - l)
   float el[kOut];                 // 2^l
   alignas(16) float w[kChunk];    // dt 2^(l_63 - l)
-  float tot, wmax, dtmax, unused; // 2^l_63, the largest w and dt
+  float tot, dtmax, unused[2];    // 2^l_63, the largest dt
 };
 
 // `Ahead`: chunks on their way besides the one in work.
@@ -81,6 +85,7 @@ struct ChunkShared {
   f32x4 scores[OUT ? 10 : 1][64];        // (C B^T) tiles on and below the diagonal, by lane
   ChunkScalars<OUT> h[2][4];
   float gmax[8];                         // largest score, by wave
+  float undo[OUT ? 8 : 1][OUT ? 32 : 1]; // by wave and column: the carry's value to one unit of its halves
 };
 
 struct Segments {
@@ -118,31 +123,28 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 __device__ __forceinline__ float wave_max(float v) {
   return __builtin_bit_cast(float, wave_max_bits(__builtin_bit_cast(uint32_t, v)));
 }
+// The largest over the four lanes that hold the same column (lane % 16).
+__device__ __forceinline__ float column_max(float v) {
+  const int iv = __builtin_bit_cast(int, v);
+  const auto p = __builtin_amdgcn_permlane16_swap(iv, iv, false, false);
+  v = __builtin_fmaxf(__builtin_bit_cast(float, (int)p[0]), __builtin_bit_cast(float, (int)p[1]));
+  const int jv = __builtin_bit_cast(int, v);
+  const auto q = __builtin_amdgcn_permlane32_swap(jv, jv, false, false);
+  return __builtin_fmaxf(__builtin_bit_cast(float, (int)q[0]), __builtin_bit_cast(float, (int)q[1]));
+}
+__device__ __forceinline__ float finite_or_0(float v) { return __builtin_fabsf(v) < __builtin_inff() ? v : 0.f; }
 // floor(log2 v) of a positive normal v (-127 for zero and subnormals).
 __device__ __forceinline__ int exponent_of(float v) { return ((__builtin_bit_cast(int, v) >> 23) & 255) - 127; }
 __device__ __forceinline__ float pow2(int k) { return __builtin_ldexpf(1.0f, k); }
 
-// v as the sum of two binary16, in units in which the largest value has the
-// exponent 14: the first carries 11 bits, the second the next 11 (whatever is
-// left above 2^-25), so that a product of a binary16 factor with both keeps
-// 22 bits, and is summed in binary32 by the matrix instruction.  `scale`, a
-// power of two, comes with the conversions: v scale - high is one mixed fma.
+// v scale as the sum of two binary16, `scale` a power of two that takes the
+// largest value to the exponent 13: the first carries 11 bits, the second the
+// next 11 (whatever is left above 2^-25), so that a product of a binary16
+// factor with both keeps 22 bits, and nothing below 2^-39 of the largest; it is
+// summed in binary32 by the matrix instruction.  `scale` comes with the
+// conversions: v scale - high is one mixed fma.
 struct Split { f16x8 hi, lo; };
-__device__ __forceinline__ Split split8(const float* v, float one) {   // one: 1, not known to the compiler
-  Split s;
-#pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const f16x2 h = __builtin_convertvector((f32x2{v[j], v[j + 1]}), f16x2);
-    const f16x2 l = __builtin_convertvector(
-        (f32x2{__builtin_fmaf(v[j], one, -(float)h[0]), __builtin_fmaf(v[j + 1], one, -(float)h[1])}), f16x2);
-    s.hi[j] = h[0];
-    s.hi[j + 1] = h[1];
-    s.lo[j] = l[0];
-    s.lo[j + 1] = l[1];
-  }
-  return s;
-}
-__device__ __forceinline__ Split split8_scaled(const float* v, float scale) {
+__device__ __forceinline__ Split split8(const float* v, float scale) {
   Split s;
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
@@ -153,6 +155,30 @@ __device__ __forceinline__ Split split8_scaled(const float* v, float scale) {
     s.hi[j + 1] = h[1];
     s.lo[j] = l[0];
     s.lo[j + 1] = l[1];
+  }
+  return s;
+}
+// v as hi + lo + least 2^-kLeast, for |v| below 2^14: the third in units of its
+// own, so that nothing is left out above 2^-62 of the largest, for two sums that
+// meet in binary32.
+constexpr int kLeast = 24;
+struct Split3 { f16x8 hi, lo, least; };
+__device__ __forceinline__ Split3 split8_3(const float* v, float one) {   // one: 1, not known to the compiler
+  constexpr float kUp = 1 << kLeast;
+  Split3 s;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const f16x2 h = __builtin_convertvector((f32x2{v[j], v[j + 1]}), f16x2);
+    const float r0 = __builtin_fmaf(v[j], one, -(float)h[0]), r1 = __builtin_fmaf(v[j + 1], one, -(float)h[1]);
+    const f16x2 l = __builtin_convertvector((f32x2{r0, r1}), f16x2);
+    const f16x2 e = __builtin_convertvector(
+        (f32x2{__builtin_fmaf(r0, one, -(float)l[0]) * kUp, __builtin_fmaf(r1, one, -(float)l[1]) * kUp}), f16x2);
+    s.hi[j] = h[0];
+    s.hi[j + 1] = h[1];
+    s.lo[j] = l[0];
+    s.lo[j + 1] = l[1];
+    s.least[j] = e[0];
+    s.least[j + 1] = e[1];
   }
   return s;
 }
@@ -251,10 +277,8 @@ __device__ __forceinline__ uint32_t max_magnitudes(uint32_t m, u32x4 v) {   // p
 __device__ __forceinline__ uint32_t max_magnitudes(uint32_t m, u32x2 v) {
   return max_magnitudes(m, u32x4{v[0], v[1], 0u, 0u});
 }
-__device__ __forceinline__ uint32_t wave_max_half(uint32_t m) {
-  const uint32_t lo = m & 0xffffu, hi = m >> 16;
-  return wave_max_bits(lo > hi ? lo : hi);
-}
+// Whether a pair of binary16 magnitudes has a non-finite one.
+__device__ __forceinline__ bool non_finite_half(uint32_t m) { return (m & 0xffffu) >= 0x7c00u || m >= 0x7c000000u; }
 // The row of at most 64 whose token count has the given place among them,
 // largest first.
 __device__ __forceinline__ int64_t row_by_length(const FullArgs& a, uint32_t place) {
@@ -375,12 +399,11 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       hs.ws[lane] = dt * __builtin_amdgcn_exp2f((float)(tile - l));
       hs.el[lane] = __builtin_amdgcn_exp2f(lh);
     }
-    const float wm = wave_max(w), dm = wave_max(dt);
-    if (lane == 0) {
-      hs.tot = __builtin_amdgcn_exp2f((float)last);
-      hs.wmax = wm;
-      hs.dtmax = dm;
+    if constexpr (OUT) {
+      const float dm = wave_max(dt);
+      if (lane == 0) hs.dtmax = dm;
     }
+    if (lane == 0) hs.tot = __builtin_amdgcn_exp2f((float)last);
     seg_log += last;
   };
 
@@ -389,9 +412,11 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   for (int k = 0; k < kAhead; ++k)
     if (k < chunks) load_chunk(k * kChunk, k);
 
-  // the carry: S[16 nt + 4 lg + i][column] as st[nt][pt][i], 2^-eS times its value
+  // the carry: S[16 nt + 4 lg + i][column] as st[nt][pt][i], 2^eS times its value.
+  // Columns do not meet in any product, so each has powers of two of its own: a
+  // large channel takes no bits from its neighbours.
   f32x4 st[8][2];
-  int eS = 0;
+  int eS[2] = {0, 0};
   if constexpr (OUT) {
     // the row's only segment: the pool's own carry
     const float* base = seg == 0 && len <= t1 ? a.state + slot * a.H * a.P * 128 : sg.state + (seg * a.batch + b) * a.H * a.P * 128;
@@ -408,9 +433,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) st[nt][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  float sbound = 0.f;   // a bound of the carry's magnitudes
+  float sbound[2] = {0.f, 0.f};   // a bound of the carry's magnitudes, by column
   const int turned_at = bc_at(4 * lg + (lr >> 2), 4 * (lr & 3));   // for transposing reads of B
-  float one = 1.0f;   // keeps the halves' differences mixed-precision fmas
+  float one = 1.0f;   // keeps the parts' differences mixed-precision fmas
   asm volatile("" : "+s"(one));
   uint32_t yoff[2];
 #pragma unroll
@@ -418,30 +443,65 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     const int p = 32 * half + 16 * pt + 4 * lg;
     yoff[pt] = p < cols ? (uint32_t)(2 * (lr * a.H * a.P + p)) : kOutside;
   }
-  // the carry's largest magnitude; an infinite channel must set no scale
-  auto largest = [&]() {
-    float m = 0.f;
+  // a column's largest magnitude in units of st; an infinite coordinate must set
+  // no scale
+  auto largest = [&](float (&m)[2]) {
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(st[nt][pt][i]));
-    m = wave_max(m);
-    if (!(m < __builtin_inff())) {
-      m = 0.f;
+    for (int pt = 0; pt < 2; ++pt) {
+      m[pt] = 0.f;
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
+        for (int i = 0; i < 4; ++i) m[pt] = __builtin_fmaxf(m[pt], __builtin_fabsf(st[nt][pt][i]));
+      m[pt] = column_max(m[pt]);
+    }
+    if (__ballot(!(m[0] < __builtin_inff() && m[1] < __builtin_inff()))) {
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt) {
+        m[pt] = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m[pt] = __builtin_fmaxf(m[pt], __builtin_fabsf(finite_or_0(st[nt][pt][i])));
+        m[pt] = column_max(m[pt]);
+      }
+    }
+  };
+
+  // One chunk token by token, in binary32 throughout: the carry in its own units
+  // from here on.
+  auto by_token = [&](int64_t c0, const ChunkScalars<OUT>& hs, const uint16_t* xt, const uint16_t* bt, const uint16_t* ct) {
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt) {
+      const float undo = pow2(-eS[pt]);
+      eS[pt] = 0;
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) st[nt][pt] *= undo;
+    }
+    const int left = (int)(n - c0 < kChunk ? n - c0 : kChunk);
+    for (int t = 0; t < left; ++t) {
+      const float dt = hs.dt[t];
+      const float decay = __builtin_amdgcn_exp2f(t ? (hs.lh[t] - hs.lh[t - 1]) + (hs.ll[t] - hs.ll[t - 1]) : hs.lh[0]);
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt) {
+        const float xv = h2f(xt[x_at(t, pw + 16 * pt)]), in = xv * dt;
+        float acc = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float v = __builtin_fabsf(st[nt][pt][i]);
-            m = __builtin_fmaxf(m, v < __builtin_inff() ? v : 0.f);
+            const float bv = h2f(bt[bc_at(t, 16 * nt + 4 * lg + i)]);
+            st[nt][pt][i] = __builtin_fmaf(st[nt][pt][i], decay, in * bv);
+            if constexpr (OUT) acc = __builtin_fmaf(st[nt][pt][i], h2f(ct[bc_at(t, 16 * nt + 4 * lg + i)]), acc);
           }
-      m = wave_max(m);
+        if constexpr (OUT) {
+          acc = butterfly_add<5>(butterfly_add<4>(acc));
+          if (lg == 0 && pw + 16 * pt < cols)
+            a.y[((b * a.L + t0 + c0 + t) * a.H + h) * a.P + pc + pw + 16 * pt] = f2h(__builtin_fmaf(xv, dh, acc));
+        }
+      }
     }
-    return m;
+    wait_vmcnt<0>();   // the next chunk, before these stores
   };
 
   // The first chunk has landed: behind its transfers are the carry's 16 loads,
@@ -481,7 +541,6 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         xf[pt][T] = read_transposed(xt + 16 * T * kRowX + x_at(4 * lg + (lr >> 2), 32 * half + 16 * pt + 4 * (lr & 3)));
         xm = max_magnitudes(xm, __builtin_bit_cast(u32x2, xf[pt][T]));
       }
-    xm = wave_max_half(xm);
 
     // 8 coordinates of row 16 tile + lr of B or C in the order of the carry's
     // fragments: 32 kk + 4 lg + ..., and 16 further
@@ -497,7 +556,10 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       return join(*(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk))),
                   *(const volatile lds_f16x4*)(r + (row_at ^ (32 * kk + 16))));
     };
-    const bool odd = OUT && (xm >= 0x7c00u || hs.tot > 1.0f);
+    // A non-finite x must not reach earlier tokens, which the matrix products would
+    // let it do (0 * inf); and where the carry grows (a positive A) the last tokens'
+    // weights would set the first ones' scale: such a chunk token by token.
+    bool odd = OUT && (__ballot(non_finite_half(xm)) != 0 || hs.tot > 1.0f);
     if constexpr (OUT) {
       // ---- C B^T, the same for all heads: two waves without scalars two tiles, the others one.
       // Tile (j, i): rows tokens 16 j + 4 lg + r (B), columns tokens 16 i + lr (C).
@@ -521,46 +583,24 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt) acc[i][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const float smax = largest();
-      sbound = __builtin_ldexpf(smax, -eS);
-      const int kS = 13 - exponent_of(smax) > 100 ? 100 : 13 - exponent_of(smax);   // in units of st
-      if (odd) {
-        // A non-finite x must not reach earlier tokens, which the matrix
-        // products would let it do (0 * inf); and where the carry grows (a
-        // positive A) the last tokens' weights would set the first ones' scale:
-        // this chunk token by token.
-        const float undo = pow2(-eS);
+      float smax[2];
+      largest(smax);
+      int kS[2];   // in units of st
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int pt = 0; pt < 2; ++pt) st[nt][pt] *= undo;
-        const int left = (int)(n - c0 < kChunk ? n - c0 : kChunk);
-        for (int t = 0; t < left; ++t) {
-          const float dt = hs.dt[t];
-          const float decay = __builtin_amdgcn_exp2f(t ? (hs.lh[t] - hs.lh[t - 1]) + (hs.ll[t] - hs.ll[t - 1]) : hs.lh[0]);
-#pragma unroll
-          for (int pt = 0; pt < 2; ++pt) {
-            const float xv = h2f(xt[x_at(t, pw + 16 * pt)]), in = xv * dt;
-            float acc = 0.f;
-#pragma unroll
-            for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float bv = h2f(bt[bc_at(t, 16 * nt + 4 * lg + i)]);
-                const float cv = h2f(ct[bc_at(t, 16 * nt + 4 * lg + i)]);
-                st[nt][pt][i] = __builtin_fmaf(st[nt][pt][i], decay, in * bv);
-                acc = __builtin_fmaf(st[nt][pt][i], cv, acc);
-              }
-            acc = butterfly_add<5>(butterfly_add<4>(acc));
-            if (lg == 0 && pw + 16 * pt < cols)
-              a.y[((b * a.L + t0 + c0 + t) * a.H + h) * a.P + pc + pw + 16 * pt] = f2h(__builtin_fmaf(xv, dh, acc));
-          }
-        }
-        eS = 0;
-        wait_vmcnt<0>();   // the next chunk, before these stores
-      } else {
+      for (int pt = 0; pt < 2; ++pt) {
+        sbound[pt] = __builtin_ldexpf(smax[pt], -eS[pt]);
+        kS[pt] = 13 - exponent_of(smax[pt]) > 100 ? 100 : 13 - exponent_of(smax[pt]);
+      }
+      // (so would one of carries whose products leave binary32)
+      odd = odd || __ballot(sbound[0] > 0x1p40f || sbound[1] > 0x1p40f) != 0;
+      if (!odd) {
         // ---- S C_t: rows = columns of x, columns = tokens
-        const float ss = pow2(kS);
+        float ss[2];
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt) {
+          ss[pt] = pow2(kS[pt]);
+          s.undo[wave][16 * pt + lr] = __builtin_ldexpf(1.0f, -kS[pt] - eS[pt]);
+        }
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           Split f[2];
@@ -569,7 +609,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = st[2 * kk + (i >> 2)][pt][i & 3];
-            f[pt] = split8_scaled(v, ss);
+            f[pt] = split8(v, ss[pt]);
           }
           f16x8 cf[4];
 #pragma unroll
@@ -583,6 +623,17 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 #pragma unroll
             for (int pt = 0; pt < 2; ++pt) acc[i][pt] = mfma(f[pt].lo, cf[i], acc[i][pt]);
         }
+        // (written and read by this wave alone)
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt) {
+          const f32x4 u = *(const f32x4*)(s.undo[wave] + 16 * pt + 4 * lg);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][pt][r] *= u[r];
+        }
+      } else {
+        by_token(c0, hs, xt, bt, ct);
       }
       __syncthreads();   // the scores are there
 
@@ -593,19 +644,16 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         float gmax = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) gmax = __builtin_fmaxf(gmax, s.gmax[k]);
-        float mb = gmax * hs.dtmax + __builtin_fabsf(dh);   // bounds the weights
-        // Weights below 2^15.  Below 2^-25 one times any x is nothing in the
-        // readout; and without a finite bound there is no scale to choose.
+        const float mb = gmax * hs.dtmax + __builtin_fabsf(dh);   // bounds the weights
+        // Weights below 2^14; without a finite bound there is no scale to choose.
+        // (No power above 24: what that leaves out is nothing in a readout.)
         int km = mb < __builtin_inff() ? 13 - exponent_of(mb) : 0;
-        km = km > 40 ? 40 : km;
+        km = km > 24 ? 24 : km;
         km = __builtin_amdgcn_readfirstlane(km);
         const float scale = pow2(km), back = pow2(-km), fkm = (float)km;
         float dk[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) dk[k] = 4 * lg + k == lr ? dh * scale : 0.f;
-        const int left = (int)(n - c0 < kChunk ? n - c0 : kChunk);
-        uint16_t* yc = a.y + ((b * a.L + t0 + c0) * a.H + h) * a.P + pc;
-        const auto yb = rows_buffer(yc, a.H * a.P, left, (int)cols);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float th = hs.lh[16 * i + lr], tl = hs.ll[16 * i + lr] + fkm;
@@ -631,20 +679,31 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
 #pragma unroll
           for (int k = 4 * i + 4; k < 16; ++k) v[k] = 0.f;
-          const float f = __builtin_ldexpf(hs.el[16 * i + lr], km - kS - eS);
+          const float f = hs.el[16 * i + lr] * (scale * (1 << kLeast));
+          Split3 m[2];
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt)
+          for (int kk = 0; kk <= i / 2; ++kk) m[kk] = split8_3(v + 8 * kk, one);
+          auto add = [&](f16x8 Split3::*part) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][pt][r] *= f;
+            for (int kk = 0; kk <= i / 2; ++kk)
 #pragma unroll
-          for (int kk = 0; kk <= i / 2; ++kk) {
-            const Split m = split8(v + 8 * kk, one);
+              for (int pt = 0; pt < 2; ++pt) acc[i][pt] = mfma(join(xf[pt][2 * kk], xf[pt][2 * kk + 1]), m[kk].*part, acc[i][pt]);
+          };
+          auto rescale = [&](float by) {
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) acc[i][pt] = mfma(join(xf[pt][2 * kk], xf[pt][2 * kk + 1]), m.hi, acc[i][pt]);
+            for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-            for (int pt = 0; pt < 2; ++pt) acc[i][pt] = mfma(join(xf[pt][2 * kk], xf[pt][2 * kk + 1]), m.lo, acc[i][pt]);
-          }
+              for (int r = 0; r < 4; ++r) acc[i][pt][r] *= by;
+          };
+          rescale(f);
+          add(&Split3::least);
+          rescale(1.0f / (1 << kLeast));
+          add(&Split3::lo);
+          add(&Split3::hi);
         }
+        const int left = (int)(n - c0 < kChunk ? n - c0 : kChunk);
+        uint16_t* yc = a.y + ((b * a.L + t0 + c0) * a.H + h) * a.P + pc;
+        const auto yb = rows_buffer(yc, a.H * a.P, left, (int)cols);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -670,42 +729,57 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       }
     }
 
-    // ---- the carry after the chunk: x w 2^e1 below 2^15, unless a bound of
-    // the carry (the decayed one and 64 products) would leave binary32.
+    // ---- the carry after the chunk: a column's x w 2^e1 below 2^14, unless a
+    // bound of its carry (the decayed one and 64 products) would leave binary32.
     if (!odd) {
-      const float tot = hs.tot, wmax = hs.wmax;
-      const float xmax = xm >= 0x7c00u ? 65536.0f : h2f((uint16_t)xm);
-      sbound = __builtin_fmaf(sbound, tot, 64.0f * 65504.0f * xmax * wmax);
-      const int eb = sbound < 0x1p120f ? exponent_of(sbound) : 121;
-      int e1 = eS;
-      if (xm && wmax > 0.f && wmax < __builtin_inff()) {
-        e1 = 13 - exponent_of(xmax) - exponent_of(wmax);
-        e1 = e1 < 120 - eb ? e1 : 120 - eb;
+      const float tot = hs.tot;
+      float xw[2][16], mx[2], keep[2], sx[2];
+      int d[2];
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt) {
+        mx[pt] = 0.f;
+#pragma unroll
+        for (int T = 0; T < 4; ++T) {
+          const f32x4 w = *(const f32x4*)(hs.w + 16 * T + 4 * lg);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            xw[pt][4 * T + i] = (float)xf[pt][T][i] * w[i];
+            mx[pt] = __builtin_fmaxf(mx[pt], __builtin_fabsf(xw[pt][4 * T + i]));
+          }
+        }
+        mx[pt] = column_max(mx[pt]);
+        sbound[pt] = __builtin_fmaf(sbound[pt], tot, 64.0f * 65504.0f * mx[pt]);
+        const int most = 120 - (sbound[pt] < 0x1p120f ? exponent_of(sbound[pt]) : 121);
+        int e1 = 13 - exponent_of(mx[pt]);
+        e1 = e1 < most ? e1 : most;
         e1 = e1 < 110 ? (e1 > -110 ? e1 : -110) : 110;
+        e1 = mx[pt] > 0.f && mx[pt] < __builtin_inff() ? e1 : eS[pt];
+        d[pt] = e1 - eS[pt];
+        eS[pt] = e1;
+        keep[pt] = __builtin_ldexpf(tot, d[pt]);
+        sx[pt] = pow2(e1);
       }
-      e1 = __builtin_amdgcn_readfirstlane(e1);
-      const float keep = __builtin_ldexpf(tot, e1 - eS), sx = pow2(e1);
-      eS = e1;
+      // (a factor past binary32 would make a carry of zero a NaN)
+      if (__ballot(d[0] > 100 || d[1] > 100 || d[0] < -100 || d[1] < -100)) {
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[nt][pt][i] = __builtin_ldexpf(st[nt][pt][i] * tot, d[pt]);
+        keep[0] = keep[1] = 1.0f;
+      }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st[nt][pt][i] *= keep;
+          for (int i = 0; i < 4; ++i) st[nt][pt][i] *= keep[pt];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        const f32x4 w0 = *(const f32x4*)(hs.w + 32 * kk + 4 * lg) * sx, w1 = *(const f32x4*)(hs.w + 32 * kk + 16 + 4 * lg) * sx;
         Split f[2];
 #pragma unroll
-        for (int pt = 0; pt < 2; ++pt) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = (float)xf[pt][2 * kk][i] * w0[i];
-            v[4 + i] = (float)xf[pt][2 * kk + 1][i] * w1[i];
-          }
-          f[pt] = split8(v, one);
-        }
+        for (int pt = 0; pt < 2; ++pt) f[pt] = split8(xw[pt] + 8 * kk, sx[pt]);
         const uint16_t* r = bt + 32 * kk * kRowB;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
@@ -734,12 +808,12 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   }
 
   if (!OUT || len <= t1) {
-    const float undo = pow2(-eS);
     const int64_t base = OUT ? slot * a.H + h : ((seg + 1) * a.batch + b) * a.H + h;
     float* dst = OUT ? a.state : sg.state;
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt)
       if (pw + 16 * pt < cols) {
+        const float undo = pow2(-eS[pt]);
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
           *(f32x4*)(dst + (base * a.P + pc + pw + 16 * pt) * 128 + 16 * nt + 4 * lg) = st[nt][pt] * undo;
