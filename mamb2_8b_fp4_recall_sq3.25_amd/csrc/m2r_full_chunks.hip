@@ -71,7 +71,7 @@ struct ChunkScalars {
   float ws[kOut];                 // dt 2^(r_tile - l)
   float el[kOut];                 // 2^l
   alignas(16) float w[kChunk];    // dt 2^(l_63 - l)
-  float tot, dtmax, unused[2];    // 2^l_63, the largest dt
+  float tot, dtmax, unused[2];    // 2^l_63, the largest finite dt
 };
 
 // `Ahead`: chunks on their way besides the one in work.
@@ -84,7 +84,7 @@ struct ChunkShared {
   uint32_t dt[kBuffers][4][kChunk];      // as loaded, one value a word
   f32x4 scores[OUT ? 10 : 1][64];        // (C B^T) tiles on and below the diagonal, by lane
   ChunkScalars<OUT> h[2][4];
-  float gmax[8];                         // largest score, by wave
+  float gmax[8];                         // largest finite score, by wave
   float undo[OUT ? 8 : 1][OUT ? 32 : 1]; // by wave and column: the carry's value to one unit of its halves
 };
 
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       hs.el[lane] = __builtin_amdgcn_exp2f(lh);
     }
     if constexpr (OUT) {
-      const float dm = wave_max(dt);
+      const float dm = wave_max(finite_or_0(dt));
       if (lane == 0) hs.dtmax = dm;
     }
     if (lane == 0) hs.tot = __builtin_amdgcn_exp2f((float)last);
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         for (int kk = 0; kk < 4; ++kk) acc = mfma(row_fragment(bt, j, kk), row_fragment(ct, i, kk), acc);
         s.scores[at][lane] = acc;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) gm = __builtin_fmaxf(gm, __builtin_fabsf(acc[k]));
+        for (int k = 0; k < 4; ++k) gm = __builtin_fmaxf(gm, __builtin_fabsf(finite_or_0(acc[k])));
       };
       score_tile(wave);
       if (wave == 1 || wave == 3) score_tile(wave == 1 ? 8 : 9);
@@ -644,8 +644,9 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         float gmax = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) gmax = __builtin_fmaxf(gmax, s.gmax[k]);
-        const float mb = gmax * hs.dtmax + __builtin_fabsf(dh);   // bounds the weights
-        // Weights below 2^14; without a finite bound there is no scale to choose.
+        const float mb = gmax * hs.dtmax + __builtin_fabsf(dh);   // bounds the finite weights
+        // Those below 2^14, so that a non-finite score or step, which is in some
+        // tokens' weights only, leaves the others' bits (an infinite D is in all).
         // (No power above 24: what that leaves out is nothing in a readout.)
         int km = mb < __builtin_inff() ? 13 - exponent_of(mb) : 0;
         km = km > 24 ? 24 : km;
