@@ -70,8 +70,11 @@ struct ChunkScalars {
   float dt[kOut];
   float ws[kOut];                 // dt 2^(r_tile - l)
   float el[kOut];                 // 2^l
-  alignas(16) float w[kChunk];    // dt 2^(l_63 - l)
-  float tot, dtmax, unused[2];    // 2^l_63, the largest finite dt
+  // Where the carry grows, 2^(l_63 - l) may leave binary32 while what it multiplies
+  // does not: its whole powers of two are kept apart.
+  alignas(16) float w[kChunk];    // dt 2^(l_63 - up - l)
+  float tot, up;                  // 2^(l_63 - up), max(floor(l_63), 0)
+  float dtmax, unused;            // the largest finite dt
 };
 
 // `Ahead`: chunks on their way besides the one in work.
@@ -95,9 +98,9 @@ struct Segments {
   // 0 the row's first carry (the pool's own is overwritten by the last segment
   // while others still start), q > 0 first what segment q - 1 adds to a zero
   // carry, then (k_full_join) the carry before segment q; and the decay over
-  // segment q - 1.
+  // segment q - 1, as a factor below 2 and a power of two.
   float* state;
-  float* decay;       // [count, batch, H]
+  f32x2* decay;       // [count, batch, H]
   bool longest_first; // the grid's y is a row's place by length, not its number
 };
 
@@ -389,7 +392,8 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     const double last = lane64(l, 63), tile = dpp_row_last64(l);
     const double e0 = lane64(l, 15), e1 = lane64(l, 31), e2 = lane64(l, 47);
     const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e1 : e2));
-    const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - l));
+    const double up = last > 0.0 ? __builtin_floor(last < 1e6 ? last : 1e6) : 0.0;
+    const float lh = (float)l, w = dt * __builtin_amdgcn_exp2f((float)(last - up - l));
     hs.w[lane] = w;
     if constexpr (OUT) {
       hs.lh[lane] = lh;
@@ -403,7 +407,10 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
       const float dm = wave_max(finite_or_0(dt));
       if (lane == 0) hs.dtmax = dm;
     }
-    if (lane == 0) hs.tot = __builtin_amdgcn_exp2f((float)last);
+    if (lane == 0) {
+      hs.tot = __builtin_amdgcn_exp2f((float)(last - up));
+      hs.up = (float)up;
+    }
     seg_log += last;
   };
 
@@ -487,13 +494,15 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
         const float xv = h2f(xt[x_at(t, pw + 16 * pt)]), in = xv * dt;
         float acc = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
+        for (int nt = 0; nt < 8; ++nt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float bv = h2f(bt[bc_at(t, 16 * nt + 4 * lg + i)]);
             st[nt][pt][i] = __builtin_fmaf(st[nt][pt][i], decay, in * bv);
             if constexpr (OUT) acc = __builtin_fmaf(st[nt][pt][i], h2f(ct[bc_at(t, 16 * nt + 4 * lg + i)]), acc);
           }
+          __builtin_amdgcn_sched_barrier(0);   // few loads at a time: the registers are the chunks'
+        }
         if constexpr (OUT) {
           acc = butterfly_add<5>(butterfly_add<4>(acc));
           if (lg == 0 && pw + 16 * pt < cols)
@@ -559,7 +568,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     // A non-finite x must not reach earlier tokens, which the matrix products would
     // let it do (0 * inf); and where the carry grows (a positive A) the last tokens'
     // weights would set the first ones' scale: such a chunk token by token.
-    bool odd = OUT && (__ballot(non_finite_half(xm)) != 0 || hs.tot > 1.0f);
+    bool odd = OUT && (__ballot(non_finite_half(xm)) != 0 || hs.tot > 1.0f || hs.up > 0.f);
     if constexpr (OUT) {
       // ---- C B^T, the same for all heads: two waves without scalars two tiles, the others one.
       // Tile (j, i): rows tokens 16 j + 4 lg + r (B), columns tokens 16 i + lr (C).
@@ -734,6 +743,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
     // bound of its carry (the decayed one and 64 products) would leave binary32.
     if (!odd) {
       const float tot = hs.tot;
+      const int up = OUT ? 0 : (int)hs.up;   // (a growing chunk is an odd one with readouts)
       float xw[2][16], mx[2], keep[2], sx[2];
       int d[2];
 #pragma unroll
@@ -749,14 +759,14 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           }
         }
         mx[pt] = column_max(mx[pt]);
-        sbound[pt] = __builtin_fmaf(sbound[pt], tot, 64.0f * 65504.0f * mx[pt]);
+        sbound[pt] = __builtin_ldexpf(__builtin_fmaf(sbound[pt], tot, 64.0f * 65504.0f * mx[pt]), up);
         const int most = 120 - (sbound[pt] < 0x1p120f ? exponent_of(sbound[pt]) : 121);
         int e1 = 13 - exponent_of(mx[pt]);
         e1 = e1 < most ? e1 : most;
-        e1 = e1 < 110 ? (e1 > -110 ? e1 : -110) : 110;
         e1 = mx[pt] > 0.f && mx[pt] < __builtin_inff() ? e1 : eS[pt];
+        e1 = e1 < 110 ? (e1 > -110 ? e1 : -110) : 110;
         d[pt] = e1 - eS[pt];
-        eS[pt] = e1;
+        eS[pt] = e1 - up;
         keep[pt] = __builtin_ldexpf(tot, d[pt]);
         sx[pt] = pow2(e1);
       }
@@ -814,12 +824,18 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt)
       if (pw + 16 * pt < cols) {
-        const float undo = pow2(-eS[pt]);
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
-          *(f32x4*)(dst + (base * a.P + pc + pw + 16 * pt) * 128 + 16 * nt + 4 * lg) = st[nt][pt] * undo;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[nt][pt][i] = __builtin_ldexpf(st[nt][pt][i], -eS[pt]);
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+          *(f32x4*)(dst + (base * a.P + pc + pw + 16 * pt) * 128 + 16 * nt + 4 * lg) = st[nt][pt];
       }
-    if (!OUT && live && scalars && pc == 0 && lane == 0) sg.decay[base] = __builtin_amdgcn_exp2f((float)seg_log);
+    if (!OUT && live && scalars && pc == 0 && lane == 0) {
+      const double e = __builtin_fmin(__builtin_fmax(__builtin_floor(seg_log), -1000.0), 1000.0);
+      sg.decay[base] = f32x2{__builtin_amdgcn_exp2f((float)(seg_log - e)), (float)e};
+    }
   }
 }
 
@@ -840,7 +856,7 @@ __global__ __launch_bounds__(256) void k_full_join(FullArgs a, Segments sg) {
   at[0] = cur;
   for (int64_t q0 = 1; q0 < started; q0 += 8) {
     f32x4 v[8];
-    float d[8];
+    f32x2 d[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (q0 + k < started) {
@@ -851,7 +867,7 @@ __global__ __launch_bounds__(256) void k_full_join(FullArgs a, Segments sg) {
     for (int k = 0; k < 8; ++k)
       if (q0 + k < started) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) cur[e] = __builtin_fmaf(cur[e], d[k], v[k][e]);
+        for (int e = 0; e < 4; ++e) cur[e] = __builtin_fmaf(__builtin_ldexpf(cur[e], (int)d[k][1]), d[k][0], v[k][e]);
         at[(q0 + k) * step] = cur;
       }
   }
@@ -876,7 +892,7 @@ Segments full_segments(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G
 
 int64_t full_chunks_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, int64_t G) {
   const Segments sg = full_segments(batch, L, H, P, G);
-  return sg.count > 1 ? (int64_t)sg.count * batch * H * (P * 128 + 1) * 4 : 0;
+  return sg.count > 1 ? (int64_t)sg.count * batch * H * (P * 128 + 2) * 4 : 0;
 }
 
 hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t stream) {
@@ -884,7 +900,7 @@ hipError_t launch_full_chunks(const FullArgs& a, void* workspace, hipStream_t st
   const int64_t hpg = a.H / a.G, blocks = (hpg * ((a.P + 63) / 64) + 3) / 4;
   if (sg.count > 1) {
     sg.state = (float*)workspace;
-    sg.decay = sg.state + (int64_t)sg.count * a.batch * a.H * a.P * 128;
+    sg.decay = (f32x2*)(sg.state + (int64_t)sg.count * a.batch * a.H * a.P * 128);
   }
   // 16-byte pieces through buffers: rows that do not overlap, and 64 of them
   // within 31-bit offsets
