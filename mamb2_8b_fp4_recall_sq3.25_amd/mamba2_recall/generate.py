@@ -3,7 +3,16 @@ prompt in one backbone call, then one token at a time, each drawn on the
 device from given uniform numbers (reference: the greedy loop of
 scripts/infer_fp4_ridge_resurface_v1.py:100-110, which asks the host for every
 token).  Works with any controller; full_state.FullState takes prompts at
-matrix rate, and controller.use_adapters gives every request its own adapter.
+matrix rate, and controller.use_adapters gives every request its own adapter:
+
+    sets = [{"in_proj": adapters.AdapterSet(down, up, scale)}     # for each layer
+            for down, up, scale in weights]
+    with full_state.FullState(model) as controller:               # installed while it runs
+        controller.use_adapters(sets, ids)                        # int32[batch], -1 for none
+        new, logprobs = generate.generate(controller, lm_head, prompt, uniforms,
+                                          temperature=0.8, top_k=50, top_p=0.95)
+
+All prompts of a call have the same length.
 """
 from __future__ import annotations
 
