@@ -407,10 +407,11 @@ int64_t m2r_full_scan_workspace(int64_t batch, int64_t L, int64_t H, int64_t P, 
  * out[m] = base[m] where ids[m] is outside 0..adapters-1.  The reference has
  * one adapter for all requests (mamba2_recall/resurface_native.py:363-375).
  *   x f16 rows of K, base and out f16 rows of N (element row strides; out may
- *   be base); down f16[adapters,r,Kp], up f16[adapters,N,r], both 16-byte
- *   aligned, r = rank and Kp = K each rounded up to 8, zeros in between; rank
- *   at most 256; scale f32[adapters], ids i32[M]; workspace: 16-byte aligned
- *   device memory of m2r_adapters_workspace() bytes, used on `stream` only.
+ *   be base, and must not overlap it otherwise); down f16[adapters,r,Kp], up
+ *   f16[adapters,N,r], both 16-byte aligned, r = rank and Kp = K each rounded up
+ *   to 8, zeros in between; rank at most 256; scale f32[adapters], ids i32[M];
+ *   workspace: 16-byte aligned device memory of m2r_adapters_workspace() bytes,
+ *   used on `stream` only.
  */
 int m2r_adapters_add(const void* x, int64_t x_stride, const void* base, int64_t base_stride, const void* down,
                      const void* up, const float* scale, const int32_t* ids, void* out, int64_t out_stride, int64_t M,

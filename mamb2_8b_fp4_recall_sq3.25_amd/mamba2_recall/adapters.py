@@ -80,11 +80,19 @@ def _taken(base, x, ids, adapters):
     return 0
 
 
+def _meets(t, rows, features, stride, out):
+    """Whether a row of `t` shares memory with the dense rows of `out`."""
+    t0, o0 = t.data_ptr(), out.data_ptr()
+    row = max(0, (o0 - t0 - 2 * features) // (2 * stride) + 1)   # the first that ends behind out's start
+    return row < rows and t0 + 2 * stride * row < o0 + 2 * rows * features
+
+
 def add(base, x, adapters, ids, out=None):
     """base[..., N] plus each row's adapter update of x[..., K]; a new FP16
-    tensor, or `out` (which may be `base`).  `ids` int32[...] names each row's
-    adapter: negative, or not below the set's count, for none (the row is
-    copied).  Rows with the same adapter cost least side by side."""
+    tensor, or `out` (`base` itself, or memory that base does not overlap).
+    `ids` int32[...] names each row's adapter: negative, or not below the set's
+    count, for none (the row is copied).  Rows with the same adapter cost least
+    side by side."""
     if not isinstance(adapters, AdapterSet):
         raise ValueError("adapters must be an AdapterSet")
     k, n = adapters.features
@@ -106,6 +114,8 @@ def add(base, x, adapters, ids, out=None):
     elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or out.shape != base.shape
           or out.device != base.device or not out.is_contiguous()):
         raise ValueError("out must be contiguous FP16 of base's shape")
+    elif rows and (b2.data_ptr() != out.data_ptr() or bs != n) and _meets(b2, rows, n, bs, out):
+        raise ValueError("out must be base itself or not overlap it")   # (other rows still read theirs)
     if rows == 0:
         return out
     rank = adapters.rank
