@@ -427,14 +427,18 @@ int64_t m2r_adapters_workspace(int64_t M, int64_t K, int64_t N, int64_t rank);
  * 2^-31 of the likeliest token's; sums are exact.  ids i64[B] (-1 where a row
  * holds nothing above -inf), logprobs f32[B] of the filtered distribution.
  * The reference decodes greedily (scripts/infer_fp4_ridge_resurface_v1.py:102-109).
- *   workspace: 16-byte aligned device memory of m2r_sample_workspace() bytes
- *   (null where that is 0), used on `stream` only.
+ *   workspace: 16-byte aligned device memory, used on `stream` only, of
+ *   m2r_sample_workspace() bytes, which is enough for any filters, or of
+ *   m2r_sample_call_workspace() bytes, less where no row can have top-k or top-p
+ *   (per_row: whether temperature, top_k or top_p is an array).
  */
 int m2r_sample(const void* logits, int dtype, int64_t row_stride, const float* uniforms, const float* temperature,
                float temperature_all, const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
                const float* min_p, float min_p_all, int64_t* ids, float* logprobs, int64_t batch, int64_t V,
                void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int64_t m2r_sample_workspace(int64_t batch, int64_t V);
+int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float temperature_all, int32_t top_k_all,
+                                  float top_p_all);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,8 @@
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
+#include <cstddef>
+
 namespace m2r {
 
 enum { LOGITS_F16 = 0, LOGITS_BF16 = 1, LOGITS_F32 = 2 };
@@ -126,18 +128,25 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 // order of the list decides anything.
 constexpr int kThreads = 256, kBlock = 8 * kThreads, kMaxSplits = 256, kUnits = kThreads, kBins = 512, kList = 4096;
 
-struct alignas(16) RowWork {
-  uint64_t weight[kBins];
+struct alignas(128) RowWork {   // (whole lines)
   uint64_t unit[kUnits];         // weight kept for certain
-  uint64_t list[kList];          // (~key, index) of the tokens in the cut's bins
-  uint32_t count[kBins];
   float top[kMaxSplits], low[kMaxSplits];
   uint32_t ticket[2], listed, done;   // done: 1 drawn, 2 cut by one workgroup
   // bins of the list: p0..p1 (top-p) and bk (top-k); kBins where that filter is off
   uint32_t p0, p1, bk, unused;
   uint64_t all;                       // weight of the row
   uint64_t count_p, weight_p, count_k, weight_k;   // before bin p0 and before bin bk
+  // from here on only rows with top-k or top-p
+  alignas(128) uint64_t weight[kBins];
+  uint32_t count[kBins];
+  uint64_t list[kList];          // (~key, index) of the tokens in the cut's bins: no more than the row's
 };
+// Bytes of a row's work; `filtered`: it may have top-k or top-p.
+static int64_t row_work_bytes(int64_t V, bool filtered) {
+  const int64_t list = 8 * (V < kList ? V : kList);
+  const int64_t bytes = filtered ? (int64_t)offsetof(RowWork, list) + list : (int64_t)offsetof(RowWork, weight);
+  return (bytes + 127) / 128 * 128;
+}
 
 struct SampleShared {
   uint64_t bins[kBins];          // count << 46 | weight
@@ -244,7 +253,10 @@ __device__ __forceinline__ uint64_t place_of(float l, int64_t i) {   // ascendin
 }
 
 struct Piece { int64_t row; int64_t first, end; int piece; };
-struct Split { int pieces; int64_t size; int units; int64_t unit; };   // `size` whole units
+struct Split { int pieces; int64_t size; int units; int64_t unit, work; bool filtered; };   // `size` whole units; `work` bytes a row
+__device__ __forceinline__ RowWork& work_of(RowWork* work, const Split& sp, int64_t row) {
+  return *(RowWork*)((char*)work + row * sp.work);
+}
 __device__ __forceinline__ Piece my_piece(const Split& sp, int64_t V) {
   Piece p;
   const uint32_t row = blockIdx.x / (uint32_t)sp.pieces;   // (a 64-bit division would take longer than a short row)
@@ -344,11 +356,12 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs a, Split sp, RowWork* work) {
   __shared__ float part[2][kThreads / 64];
   const Piece p = my_piece(sp, a.V);
-  RowWork& rw = work[p.row];
-  for (int i = p.piece * kThreads + threadIdx.x; i < kBins; i += sp.pieces * kThreads) {
-    rw.weight[i] = 0;
-    rw.count[i] = 0;
-  }
+  RowWork& rw = work_of(work, sp, p.row);
+  if (sp.filtered)
+    for (int i = p.piece * kThreads + threadIdx.x; i < kBins; i += sp.pieces * kThreads) {
+      rw.weight[i] = 0;
+      rw.count[i] = 0;
+    }
   if (p.piece == 0 && threadIdx.x < 4) (&rw.ticket[0])[threadIdx.x] = 0;   // the tickets, listed and done
   const void* row = row_of<DT>(a, p.row);
   const RowFilter f = row_filter(a, p.row);
@@ -409,7 +422,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a, Split sp, RowWork* work) {
   __shared__ SampleShared s;
   const Piece p = my_piece(sp, a.V);
-  RowWork& rw = work[p.row];
+  RowWork& rw = work_of(work, sp, p.row);
   const int tid = threadIdx.x;
   const void* row = row_of<DT>(a, p.row);
   RowFilter f = row_filter(a, p.row);
@@ -814,7 +827,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads, 4) void k_sample_draw(SampleArgs a, Split sp, RowWork* work) {
   __shared__ SampleShared s;
   const Piece p = my_piece(sp, a.V);
-  RowWork& rw = work[p.row];
+  RowWork& rw = work_of(work, sp, p.row);
   const int tid = threadIdx.x;
   const uint32_t done = rw.done;
   if (done == 1 || (done == 2 && p.piece)) return;
@@ -914,7 +927,12 @@ static Split sample_split(int64_t batch, int64_t V) {
   pieces = pieces < all ? pieces : all;
   pieces = pieces < kMaxSplits ? pieces : kMaxSplits;
   const int64_t per = (all + pieces - 1) / pieces;
-  return Split{(int)((all + per - 1) / per), per * unit * kBlock, (int)all, unit * kBlock};
+  return Split{(int)((all + per - 1) / per), per * unit * kBlock, (int)all, unit * kBlock, 0, false};
+}
+
+// Whether a row can have top-k or top-p (a temperature of 0 is a top-k of 1).
+static bool sample_filtered(bool per_row, int64_t V, float temperature, int32_t top_k, float top_p) {
+  return per_row || !(temperature > 0.f) || (top_k > 0 && top_k < V) || top_p < 1.f;
 }
 
 template <int DT>
@@ -923,9 +941,7 @@ static void launch_sample(const SampleArgs& a, const Split& sp, RowWork* work, h
   hipLaunchKernelGGL(k_sample_top<DT>, grid, block, 0, stream, a, sp, work);
   hipLaunchKernelGGL(k_sample_bins<DT>, grid, block, 0, stream, a, sp, work);
   // where no row can have top-k or top-p the second launch has drawn them all
-  const bool filtered = a.temperature || a.top_k || a.top_p || !(a.temperature_s > 0.f) ||
-                        (a.top_k_s > 0 && a.top_k_s < a.V) || a.top_p_s < 1.f;
-  if (filtered) hipLaunchKernelGGL(k_sample_draw<DT>, grid, block, 0, stream, a, sp, work);
+  if (sp.filtered) hipLaunchKernelGGL(k_sample_draw<DT>, grid, block, 0, stream, a, sp, work);
 }
 
 }  // namespace m2r
@@ -933,7 +949,13 @@ static void launch_sample(const SampleArgs& a, const Split& sp, RowWork* work, h
 using namespace m2r;
 
 extern "C" int64_t m2r_sample_workspace(int64_t batch, int64_t V) {
-  return batch > 0 ? batch * (int64_t)sizeof(RowWork) : 0;
+  return batch > 0 && V > 0 ? batch * row_work_bytes(V, true) : 0;
+}
+
+extern "C" int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float temperature_all,
+                                             int32_t top_k_all, float top_p_all) {
+  if (batch <= 0 || V <= 0) return 0;
+  return batch * row_work_bytes(V, sample_filtered(per_row, V, temperature_all, top_k_all, top_p_all));
 }
 
 extern "C" int m2r_sample(const void* logits, int dtype, int64_t row_stride, const float* uniforms,
@@ -948,9 +970,12 @@ extern "C" int m2r_sample(const void* logits, int dtype, int64_t row_stride, con
   if (row_stride < V && batch > 1) return m2r_fail("sample: rows overlap");
   SampleArgs a{logits, row_stride, uniforms, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all,
                top_k_all, ids, logprobs, batch, V};
-  if (!workspace || workspace_bytes < m2r_sample_workspace(batch, V) || ((uintptr_t)workspace & 15))
+  const bool filtered = sample_filtered(temperature || top_k || top_p, V, temperature_all, top_k_all, top_p_all);
+  Split sp = sample_split(batch, V);
+  sp.work = row_work_bytes(V, filtered);
+  sp.filtered = filtered;
+  if (!workspace || workspace_bytes < batch * sp.work || ((uintptr_t)workspace & 15))
     return m2r_fail("sample: workspace too small or not 16-byte aligned");
-  const Split sp = sample_split(batch, V);
   if (batch * sp.pieces > 0x7fffffff) return m2r_fail("sample: grid limits exceeded");
   RowWork* work = (RowWork*)workspace;
   if (dtype == LOGITS_F16) launch_sample<LOGITS_F16>(a, sp, work, stream);

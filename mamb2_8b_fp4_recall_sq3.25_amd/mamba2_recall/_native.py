@@ -53,6 +53,7 @@ _SIGNATURES = {
     "m2r_adapters_workspace": ([I64] * 4, I64),
     "m2r_adapters_add": ([P, I64, P, I64] + [P] * 5 + [I64] * 6 + [P, I64, P], I),
     "m2r_sample_workspace": ([I64] * 2, I64),
+    "m2r_sample_call_workspace": ([I64, I64, I, F32, I, F32], I64),
     "m2r_sample": ([P, I, I64, P, P, F32, P, I, P, F32, P, F32, P, P, I64, I64, P, I64, P], I),
     "m2r_state_step_ridge_layers_workspace": ([I], I64),
     "m2r_state_step_ridge_layers": ([P, I, I64, I64, I64, I64, P, I64, P], I),

@@ -61,8 +61,9 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if vocab > 1 and logits.stride(1) != 1 or batch > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()
-    ws_bytes = int(_native.lib().m2r_sample_workspace(batch, vocab))
-    ws = logits.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    per_row = t is not None or k is not None or tp is not None
+    ws_bytes = int(_native.lib().m2r_sample_call_workspace(batch, vocab, per_row, float(t_all), k_all, float(tp_all)))
+    ws = logits.new_empty(ws_bytes, dtype=torch.uint8)
     p = _native.ptr
     with _native.device_of(logits):
         _native.call("m2r_sample", p(logits), _DTYPES[logits.dtype], logits.stride(0) if batch > 1 else vocab,
