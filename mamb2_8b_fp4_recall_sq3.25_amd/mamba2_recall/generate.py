@@ -33,6 +33,7 @@ def generate(controller, lm_head, prompt, uniforms, *, temperature=1.0, top_k=0,
         raise ValueError("uniforms must be FP32[batch,new] with at least one new token")
     if not isinstance(prompt, torch.Tensor) or prompt.ndim != 2 or prompt.shape[0] != uniforms.shape[0]:
         raise ValueError("prompt must be [batch,tokens] with a row for each row of uniforms")
+    sampling.filters(uniforms, temperature, top_k, top_p, min_p)   # refused before the request is reset
     hidden = controller.backbone(prompt, reset=True)
     columns = uniforms.t().contiguous()
     ids, logprobs = [], []

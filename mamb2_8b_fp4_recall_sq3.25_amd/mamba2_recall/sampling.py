@@ -11,17 +11,26 @@ from . import _native
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _filter(value, name, dtype, logits, low, high):
+def _filter(value, name, dtype, like, low, high):
     """(tensor or None, scalar) of one filter: a number for every row, or a
     tensor with a value for each."""
     if isinstance(value, torch.Tensor):
-        if value.dtype != dtype or tuple(value.shape) != (logits.shape[0],) or value.device != logits.device:
+        if value.dtype != dtype or tuple(value.shape) != (like.shape[0],) or value.device != like.device:
             raise ValueError(f"{name} must be a number or {str(dtype).split('.')[1]}[batch] on the logits' device")
         return value.contiguous(), 0
     if isinstance(value, bool) or not isinstance(value, (int, float) if dtype == torch.float32 else int) \
             or not low <= value <= high:
         raise ValueError(f"{name} must lie in [{low}, {high}]")
     return None, value
+
+
+def filters(like, temperature, top_k, top_p, min_p):
+    """The four filters as (tensor or None, scalar), checked for as many rows as
+    `like` has, on its device."""
+    return (_filter(temperature, "temperature", torch.float32, like, 0.0, 1e30),
+            _filter(top_k, "top_k", torch.int32, like, 0, 2 ** 31 - 1),
+            _filter(top_p, "top_p", torch.float32, like, 0.0, 1.0),
+            _filter(min_p, "min_p", torch.float32, like, 0.0, 1.0))
 
 
 def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -50,10 +59,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if (not isinstance(uniforms, torch.Tensor) or uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (batch,)
             or uniforms.device != logits.device):
         raise ValueError("uniforms must be FP32[batch] on the logits' device")
-    t, t_all = _filter(temperature, "temperature", torch.float32, logits, 0.0, 1e30)
-    k, k_all = _filter(top_k, "top_k", torch.int32, logits, 0, 2 ** 31 - 1)
-    tp, tp_all = _filter(top_p, "top_p", torch.float32, logits, 0.0, 1.0)
-    mp, mp_all = _filter(min_p, "min_p", torch.float32, logits, 0.0, 1.0)
+    (t, t_all), (k, k_all), (tp, tp_all), (mp, mp_all) = filters(logits, temperature, top_k, top_p, min_p)
     ids = logits.new_empty(batch, dtype=torch.int64)
     logprobs = torch.empty_like(uniforms, memory_format=torch.contiguous_format)
     if batch == 0:
