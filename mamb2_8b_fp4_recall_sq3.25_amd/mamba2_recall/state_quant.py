@@ -436,6 +436,8 @@ class _MixerController:
             raise ValueError("Input IDs must be CUDA int64 on the model device")
         if self._running:
             raise RuntimeError("Concurrent/reentrant backbone invocation is unsupported")
+        if self._adapters is not None and self._adapters[1].shape[0] != ids.shape[0]:
+            raise ValueError("Adapter ids and batch differ")
         if reset or self._request is None:
             self.reset(ids.shape[0])
         self._running = True
@@ -606,7 +608,7 @@ class _MixerController:
                     raise ValueError("Adapter entries are AdapterSets under in_proj and out_proj")
                 if item.features != tuple(reversed(getattr(mx, name).weight.shape)) or item.down.device != self.device:
                     raise ValueError(f"Adapters of {name} do not match the layer's projection")
-        self._adapters = (list(sets), ids.contiguous())
+        self._adapters = (list(sets), ids.contiguous()) if any(sets) else None
         return self
 
     def _adapt(self, index, name, out, value):
