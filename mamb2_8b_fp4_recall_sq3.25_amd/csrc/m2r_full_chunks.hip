@@ -754,7 +754,7 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
           const f32x4 w = *(const f32x4*)(hs.w + 16 * T + 4 * lg);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            xw[pt][4 * T + i] = (float)xf[pt][T][i] * w[i];
+            xw[pt][4 * T + i] = __builtin_fmaf((float)xf[pt][T][i], w[i], 0.f);   // (one mixed fma)
             mx[pt] = __builtin_fmaxf(mx[pt], __builtin_fabsf(xw[pt][4 * T + i]));
           }
         }
