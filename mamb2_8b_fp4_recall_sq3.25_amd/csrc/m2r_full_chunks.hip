@@ -387,8 +387,13 @@ __global__ __launch_bounds__(512, 2) void k_full_chunks(FullArgs a, Segments sg)
   // the scalars of a chunk whose dt this wave has loaded
   auto prepare = [&](int64_t c0, int buf, int par) {   // lane = token
     ChunkScalars<OUT>& hs = s.h[par][pair];
-    const float dt = c0 + lane < n ? full_dt(h2f((uint16_t)s.dt[buf][pair][lane]) + bias) : 0.f;
-    const double l = scan_add64((double)av * (double)dt * 1.4426950408889634);
+    const bool in = c0 + lane < n;
+    const float dt = in ? full_dt(h2f((uint16_t)s.dt[buf][pair][lane]) + bias) : 0.f;
+    // (below 2^-4096 a decay leaves nothing of a carry; sums of more, or of minus
+    // infinity, would leave differences without a value)
+    double step = (double)av * (double)dt * 1.4426950408889634;
+    step = in ? (step < -4096.0 ? -4096.0 : step) : 0.0;
+    const double l = scan_add64(step);
     const double last = lane64(l, 63), tile = dpp_row_last64(l);
     const double e0 = lane64(l, 15), e1 = lane64(l, 31), e2 = lane64(l, 47);
     const double before = lane < 16 ? 0.0 : (lane < 32 ? e0 : (lane < 48 ? e1 : e2));
