@@ -197,8 +197,9 @@ __global__ __launch_bounds__(256) void k_adapter_down(AdapterArgs a) {
   }
 }
 
-// v 2^k as the sum of two binary16: 22 bits of the product's operand, where one
-// alone would round the hidden values to 11.  An infinity's second part is 0.
+// v 2^k as the sum of two binary16: 22 bits of the product's operand (and nothing
+// below 2^-39 of the row's largest), where one alone would round the hidden
+// values to 11.  An infinity's second part is 0.
 __device__ __forceinline__ void split_f16(const float* v, float scale, f16x8& hi, f16x8& lo) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {

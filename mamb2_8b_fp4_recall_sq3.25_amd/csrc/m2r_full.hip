@@ -21,10 +21,11 @@ typedef uint16_t h16x4 __attribute__((ext_vector_type(4)));
 // coordinates 4n .. 4n + 3, a 16-byte access), a wave 2 R rows, so that R
 // loads of 1 KiB are in flight; the readout is a butterfly over 32 lanes.
 // One token is bound by memory: it reads and writes 1 KiB of carry a row for
-// 640 operations.  At 128 heads of 64, 61 of 64 batch rows at work: 99 us for
-// 514 MB, 5.2 TB/s, where a copy of 2 GiB reaches 4.9 (R = 2: 108 us, fewer
-// loads in flight; R = 8: 104, fewer waves).  Batch 1, 8.4 MB: 5.3 us, a
-// launch and one way to memory and back (R = 2: 5.4, R = 8: 6.1).
+// 640 operations.  At 128 heads of 64, 61 of 64 batch rows at work, 514 MB: 91
+// to 94 us among calls in one graph, 5.5 TB/s, where a copy of 2 GiB reaches
+// 4.9; a graph of one call 99 (R = 2: 108 us, fewer loads in flight; R = 8: 104,
+// fewer waves).  Batch 1, 8.4 MB: 4.3 us, a launch and one way to memory and
+// back; a graph of one call 5.3 (R = 2: 5.4, R = 8: 6.1).
 template <int R>
 __global__ __launch_bounds__(256) void k_full_rows(FullArgs a) {
   const int lane = threadIdx.x & 63, half = lane >> 5, q = lane & 31;
@@ -93,10 +94,10 @@ using namespace m2r;
 // depends on L up to 64, or steps token by token.  The step's time is its
 // carries' plus a chain per token; few rows leave the chain bare, so the
 // chunked kernel's fixed cost is made up later.  us per call, step / chunked,
-// at 128 heads of 64: batch 1 12 tokens 15.5 / 18.8, 16 tokens 19.0 / 18.8;
-// batch 4 8 tokens 18.5 / 20.6, 12 tokens 24.0 / 20.5; batch 16 4 tokens
-// 35.7 / 43.7, 6 tokens 44.6 / 43.6; batch 64 4 tokens 134 / 162, 6 tokens
-// 168 / 163, 64 tokens 1,253 / 196.
+// at 128 heads of 64: batch 1 12 tokens 15.5 / 18.8, 16 tokens 19.0 / 18.4;
+// batch 4 8 tokens 18.5 / 20.6, 12 tokens 24.0 / 20.2; batch 16 4 tokens
+// 35.7 / 43.7, 6 tokens 44.6 / 44.2; batch 64 4 tokens 134 / 162, 6 tokens
+// 168 / 157, 64 tokens 1,253 / 183.
 static bool full_chunked(int64_t batch, int64_t L, int64_t H, int64_t P) {
   const int64_t rows = batch * H * P;
   return L >= (rows <= 16384 ? 16 : (rows <= 65536 ? 10 : 6));

@@ -21,18 +21,23 @@
 // forms what each adds to a zero carry (x and B only), k_full_join runs the
 // carries through, and the main pass starts every segment from its own.
 //
-// At 128 heads of 64 in 8 groups: 8,192 tokens of one row 212 us (first pass
-// 55, join 13, main pass 142), 1.5 TB/s and 204 TFLOP/s counted token by
-// token; 2,048 tokens 80 us; nine rows of 62 to 901 tokens 128 us in one pass;
-// five short prompts 28 us.  Neither memory (64 us at 8,192 tokens) nor the
-// matrix cores bound it: a chunk takes a workgroup 17,500 clocks, of which a
-// SIMD's vector instructions are about 8,700, the LDS 4,500 and the matrix
-// instructions 5,000, and they overlap little, as both waves of a SIMD are at
-// the same step.  Leaving parts out saves, of 218 us: S C 22, the update 40,
-// the stores 22, the loads 25, the weights 15, the scalars 10.  Not better:
-// scores formed by each wave for itself, with one barrier a chunk (222 us for
-// the main kernels' 177); 16 waves of 128 registers (219 for 221); S C behind
-// the barrier; waves that start their chunk's parts in another order.
+// At 128 heads of 64 in 8 groups: 8,192 tokens of one row 214 us (the profiler
+// has first pass 55, join 13, main pass 165 at least), 1.5 TB/s and 201 TFLOP/s
+// counted token by token; 2,048 tokens 81 us; nine rows of 62 to 901 tokens 137
+// us in one pass; five short prompts 28 us.  Neither memory (64 us at 8,192
+// tokens) nor the matrix cores bound it: a chunk takes a workgroup 18,400 clocks,
+// of which a SIMD's vector instructions are about 10,600, the LDS 4,600 and the
+// matrix instructions 5,400, and they overlap little, as both waves of a SIMD are
+// at the same step.  The powers of two of each channel and the weights' third
+// part are 260 of a chunk's 1,320 vector instructions and 8 us of the 214.
+// Weights as two bfloat16 parts, which need no power of two, but x in two parts
+// as well: 250 us.  Conversions by mixed fmas that write binary16: 237 (they
+// issue at half the rate).  Before these, of 218 us, leaving parts out saved: S C
+// 22, the update 40, the stores 22, the loads 25, the weights 15, the scalars 10;
+// and not better were: scores formed by each wave for itself, with one barrier a
+// chunk (222 us for the main kernels' 177); 16 waves of 128 registers (219 for
+// 221); S C behind the barrier; waves that start their chunk's parts in another
+// order.
 #include "m2r_full.h"
 #include "m2r_abi_util.h"
 

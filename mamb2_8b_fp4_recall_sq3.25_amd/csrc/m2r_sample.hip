@@ -19,12 +19,12 @@
 // copy), with filters of all kinds: 63 us, the launches 12, 19 and 32.  The
 // first two read at 5.3 and 3.4 TB/s; the last ends with its heaviest row (19
 // us to gather thousands of listed tokens, then 11 in one workgroup to order
-// them and draw).  One row of binary16, filtered: 23 us, three launches of a
-// few dependent steps; 24 rows of 50,003 without filters: 12 us.  Logits that
+// them and draw).  One row of binary16, filtered: 22 us, three launches of a
+// few dependent steps; 24 rows of 50,003 without filters: 11 us.  Logits that
 // are all close (normal, deviation 0.02 to 1; top-p 0.9): 64 rows 64 to 70 us,
 // where bins of a fixed 1/16 left lists that did not fit (1,350 us).  All
-// logits equal, cut by a workgroup a row: one row 145 to 210 us, 64 rows 360 to
-// 470 (14,000 with a counter's atomics from every lane).
+// logits equal, cut by a workgroup a row: one row 143 to 210 us, 64 rows 360 to
+// 470 (7,000 with a counter's atomics from every lane).
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
