@@ -440,6 +440,55 @@ int64_t m2r_sample_workspace(int64_t batch, int64_t V);
 int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float temperature_all, int32_t top_k_all,
                                   float top_p_all);
 
+/*
+ * Penalties for repeated tokens, biases and grammar masks on logits (dtype 0
+ * binary16, 1 bfloat16, 2 binary32), before m2r_sample.  For a token that is c
+ * times in its row of `tokens` (the ids generated so far):
+ *   l <- l / repetition (l > 0) or l * repetition (else) where the token is in
+ *   `prompt` or `tokens`; l <- l - (frequency c + presence) where c > 0;
+ *   l <- l + the value of the row's last bias entry that names the token;
+ *   l <- -inf where the row's mask has its bit (word token / 32, bit token % 32) 0.
+ * In binary32, rounded once; a logit that nothing touches keeps its bits.  The
+ * reference decodes greedily (scripts/infer_fp4_ridge_resurface_v1.py:102-109).
+ *   prompt, tokens: ids i32 or i64 rows of prompt_n (tokens_n), or null with 0;
+ *   prompt_lengths, lengths i32[B] or null (all), clamped to 0..n; ids outside
+ *   0..V-1 count for nothing.  repetition, presence, frequency: f32[B], or null
+ *   and one value for all rows.  bias_ids i32 and bias_values f32 rows of `biases`
+ *   entries.  allowed: u32 rows of (V + 31) / 32 words, `masks` of them;
+ *   allowed_rows i32[B] names each row's, outside 0..masks-1 for none, or null
+ *   (mask b).  Row strides in elements; lists, biases and masks may have stride 0.
+ *   out: logits itself with their stride, or memory that does not overlap them.
+ */
+int m2r_adjust_logits(const void* logits, int dtype, int64_t row_stride, void* out, int64_t out_stride,
+                      const void* prompt, int prompt_is_i64, int64_t prompt_stride, int64_t prompt_n,
+                      const int32_t* prompt_lengths, const void* tokens, int tokens_are_i64, int64_t tokens_stride,
+                      int64_t tokens_n, const int32_t* lengths, const float* repetition, float repetition_all,
+                      const float* presence, float presence_all, const float* frequency, float frequency_all,
+                      const int32_t* bias_ids, int64_t bias_ids_stride, const float* bias_values,
+                      int64_t bias_values_stride, int64_t biases, const uint32_t* allowed, int64_t allowed_stride,
+                      int64_t masks, const int32_t* allowed_rows, int64_t batch, int64_t V, hipStream_t stream);
+
+/*
+ * The mixer's short causal convolution with SiLU over a pool of windows, for
+ * rows of different lengths, before m2r_full_scan:
+ *   o_t = half(silu(bias + sum_{j<4} w_j u_{t-3+j})),
+ * u before a row's first token being its window's last three inputs; the
+ * window then holds the row's last four.  The ragged form of the convolution of
+ * mamba2_recall/state_quant.py:283-317, with one rounding.
+ *   window f16 [pool, 4, C] by element strides ws_s, ws_t (channel stride 1),
+ *   changed in place; value f16 [B, L, C] with strides vs_b, vs_l (channel stride
+ *   1); weight f16 [C, 4] contiguous, 8-byte aligned; bias f16 [C] or NULL; slots
+ *   and lengths as in m2r_full_scan; x, bm, cm f16 [B, L, n_x | n_b | n_c]
+ *   contiguous, C = n_x + n_b + n_c, zero past a row's length; width must be 4;
+ *   silu 1 applies the SiLU.  window and value must not overlap an output or each
+ *   other.  16-byte aligned tensors of channel counts and strides that are whole
+ *   eights take the faster loads, with the same results.
+ */
+int m2r_conv_pool(void* window, int64_t pool, int64_t ws_s, int64_t ws_t, const void* value, int64_t vs_b,
+                  int64_t vs_l, const void* weight, const void* bias, const int32_t* slots, const int32_t* lengths,
+                  void* x, void* bm, void* cm, int64_t n_x, int64_t n_b, int64_t n_c, int64_t batch, int64_t tokens,
+                  int width, int silu, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,216 @@
+// Penalties for repeated tokens, biases and grammar masks on logits, for
+// gfx950, before a token is drawn from them (m2r_sample.hip).  For a row's
+// token v, c times among its generated tokens:
+//   l <- l / r (l > 0) or l r (else)   where v is in the prompt or c > 0
+//   l <- l - (f c + p)                 where c > 0
+//   l <- l + bias[v]                   the last entry of the row's list that names v
+//   l <- -inf                          where the row's mask does not allow v
+// in binary32, rounded once to the logits' type; a logit that none of this
+// touches keeps its bits.
+//
+// A workgroup takes a slice of a row's tokens.  It counts the row's ids that
+// lie in its slice in a table in LDS (whole numbers: the order does not
+// matter), then passes over its logits once; no counts are kept in memory.
+// Bound by memory: each logit read and written once.
+#include "m2r_device.h"
+#include "m2r_abi_util.h"
+
+#include <initializer_list>
+
+namespace m2r {
+
+struct IdList {
+  const void* ids;       // int32 or int64 rows, or null
+  int64_t stride, n;
+  const int32_t* lengths;
+  int wide;              // 1: int64
+};
+struct RowValue {
+  const float* row;      // a value for each row, or null
+  float all;
+};
+struct AdjustArgs {
+  const void* logits;
+  int64_t ls;
+  void* out;
+  int64_t os;
+  IdList prompt, tokens;
+  RowValue repetition, presence, frequency;
+  const int32_t* bias_ids;
+  const float* bias_values;
+  int64_t bias_ids_stride, bias_values_stride, biases;
+  const uint32_t* allowed;
+  int64_t allowed_stride, masks;
+  const int32_t* allowed_rows;
+  int64_t V;
+  uint32_t slices;
+  int slice;             // tokens of a workgroup, a multiple of 32
+  int in_place;
+};
+
+constexpr int kAdjustThreads = 512;
+constexpr uint32_t kInPrompt = 0x80000000u;   // of a table's word; the rest counts the generated tokens
+
+template <int DTYPE> struct LogitType { typedef uint16_t T; };
+template <> struct LogitType<2> { typedef float T; };
+template <int DTYPE>
+__device__ __forceinline__ float logit_value(typename LogitType<DTYPE>::T v) {
+  if constexpr (DTYPE == 0) return h2f(v);
+  else if constexpr (DTYPE == 1) return __builtin_bit_cast(float, (uint32_t)v << 16);
+  else return v;
+}
+template <int DTYPE>
+__device__ __forceinline__ typename LogitType<DTYPE>::T logit_rounded(float v) {
+  if constexpr (DTYPE == 0) return f2h(v);
+  else if constexpr (DTYPE == 1) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)(u >> 16 | 0x40);   // NaN stays one
+    return (uint16_t)((u + 0x7fffu + (u >> 16 & 1)) >> 16);
+  } else return v;
+}
+
+__device__ __forceinline__ float row_value(const RowValue& v, int64_t row) { return v.row ? v.row[row] : v.all; }
+
+// Calls f(token of the slice) for each id of the row's list in [v0, v0 + size).
+template <typename F>
+__device__ __forceinline__ void for_ids(const IdList& l, int64_t row, int64_t v0, int size, F f) {
+  if (!l.ids) return;
+  int64_t n = l.lengths ? l.lengths[row] : l.n;
+  n = n < l.n ? n : l.n;
+  if (l.wide) {
+    const int64_t* p = (const int64_t*)l.ids + row * l.stride;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += kAdjustThreads) {
+      const uint64_t at = (uint64_t)(p[i] - v0);
+      if (at < (uint64_t)size) f((int)at);
+    }
+  } else {
+    const int32_t* p = (const int32_t*)l.ids + row * l.stride;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += kAdjustThreads) {
+      const uint64_t at = (uint64_t)((int64_t)p[i] - v0);
+      if (at < (uint64_t)size) f((int)at);
+    }
+  }
+}
+
+template <int DTYPE>
+__global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustArgs a) {
+  typedef typename LogitType<DTYPE>::T T;
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ uint32_t table[];            // [slice], and [slice] places in the list of biases
+  const int64_t row = blockIdx.x / a.slices, v0 = (int64_t)(blockIdx.x % a.slices) * a.slice;
+  const int size = (int)(a.V - v0 < a.slice ? a.V - v0 : a.slice);
+  const T* src = (const T*)a.logits + row * a.ls + v0;
+  T* dst = (T*)a.out + row * a.os + v0;
+  const bool counted = a.prompt.ids || a.tokens.ids, biased = a.bias_ids != nullptr;
+  uint32_t* place = table + (counted ? a.slice : 0);
+  if (counted || biased) {
+    for (int i = threadIdx.x; i < a.slice * (counted + biased); i += kAdjustThreads) table[i] = 0;
+    __syncthreads();
+    for_ids(a.prompt, row, v0, size, [&](int at) { atomicOr(&table[at], kInPrompt); });
+    for_ids(a.tokens, row, v0, size, [&](int at) { atomicAdd(&table[at], 1u); });
+    if (biased)
+      for (int64_t i = threadIdx.x; i < a.biases; i += kAdjustThreads) {
+        const uint64_t at = (uint64_t)((int64_t)a.bias_ids[row * a.bias_ids_stride + i] - v0);
+        if (at < (uint64_t)size) atomicMax(&place[at], (uint32_t)i + 1u);   // the list's last entry for a token
+      }
+    __syncthreads();
+  }
+  const float repetition = row_value(a.repetition, row), presence = row_value(a.presence, row),
+              frequency = row_value(a.frequency, row);
+  const uint32_t* allowed = nullptr;
+  if (a.allowed) {
+    const int64_t m = a.allowed_rows ? a.allowed_rows[row] : row;
+    if (m >= 0 && m < a.masks) allowed = a.allowed + m * a.allowed_stride + (v0 >> 5);
+  }
+  for (int i = threadIdx.x * VEC; i < size; i += kAdjustThreads * VEC) {
+    uint32_t free = 0xffffffffu;
+    if (allowed) free = allowed[i >> 5] >> (i & 31);
+    uint32_t word[VEC], entry[VEC], touched = 0;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      word[k] = counted ? table[i + k] : 0;
+      entry[k] = biased ? place[i + k] : 0;
+      touched |= word[k] | entry[k];
+    }
+    const bool all_free = (free & ((1u << VEC) - 1)) == (1u << VEC) - 1;
+    if (a.in_place && all_free && !touched) continue;
+    T l[VEC];
+    const bool whole = i + VEC <= size;
+    if (whole) __builtin_memcpy(l, src + i, 16);
+    else
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) l[k] = i + k < size ? src[i + k] : T(0);
+    if (touched) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        if (!(word[k] | entry[k])) continue;
+        float v = logit_value<DTYPE>(l[k]);
+        if (word[k]) {
+          v = v > 0.f ? v / repetition : v * repetition;
+          const uint32_t c = word[k] & ~kInPrompt;
+          if (c) v = v - (frequency * (float)c + presence);
+        }
+        if (entry[k]) v = v + a.bias_values[row * a.bias_values_stride + entry[k] - 1];
+        l[k] = logit_rounded<DTYPE>(v);
+      }
+    }
+    if (!all_free) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (!(free >> k & 1)) l[k] = logit_rounded<DTYPE>(-__builtin_inff());
+    }
+    if (whole) __builtin_memcpy(dst + i, l, 16);
+    else
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (i + k < size) dst[i + k] = l[k];
+  }
+}
+
+}  // namespace m2r
+
+using namespace m2r;
+
+extern "C" int m2r_adjust_logits(const void* logits, int dtype, int64_t row_stride, void* out, int64_t out_stride,
+                                 const void* prompt, int prompt_is_i64, int64_t prompt_stride, int64_t prompt_n,
+                                 const int32_t* prompt_lengths, const void* tokens, int tokens_are_i64,
+                                 int64_t tokens_stride, int64_t tokens_n, const int32_t* lengths,
+                                 const float* repetition, float repetition_all, const float* presence,
+                                 float presence_all, const float* frequency, float frequency_all,
+                                 const int32_t* bias_ids, int64_t bias_ids_stride, const float* bias_values,
+                                 int64_t bias_values_stride, int64_t biases, const uint32_t* allowed,
+                                 int64_t allowed_stride, int64_t masks, const int32_t* allowed_rows, int64_t batch,
+                                 int64_t V, hipStream_t stream) {
+  if (batch <= 0 || V <= 0) return m2r_fail("adjust: non-positive shape");
+  if (batch > 0x7fffffff || V > 0x7ffffffe) return m2r_fail("adjust: size limits");
+  if (dtype < 0 || dtype > 2) return m2r_fail("adjust: logits must be binary16, bfloat16 or binary32");
+  if (!logits || !out) return m2r_fail("adjust: null pointer");
+  if (row_stride < V || out_stride < V) return m2r_fail("adjust: rows overlap");
+  const int64_t lim = (int64_t)1 << 30;
+  if (prompt_n < 0 || tokens_n < 0 || biases < 0 || prompt_n > lim || tokens_n > lim || biases > lim)
+    return m2r_fail("adjust: list limits");
+  if ((prompt_n && !prompt) || (tokens_n && !tokens) || (biases && (!bias_ids || !bias_values)))
+    return m2r_fail("adjust: null pointer");
+  if (prompt_stride < 0 || tokens_stride < 0 || bias_ids_stride < 0 || bias_values_stride < 0 || allowed_stride < 0)
+    return m2r_fail("adjust: negative strides");
+  if (allowed && masks <= 0) return m2r_fail("adjust: no masks");
+  if (allowed && !allowed_rows && masks < batch) return m2r_fail("adjust: more batch rows than masks");
+  AdjustArgs a{logits, row_stride, out, out_stride,
+               {prompt_n ? prompt : nullptr, prompt_stride, prompt_n, prompt_lengths, prompt_is_i64},
+               {tokens_n ? tokens : nullptr, tokens_stride, tokens_n, lengths, tokens_are_i64},
+               {repetition, repetition_all}, {presence, presence_all}, {frequency, frequency_all},
+               biases ? bias_ids : nullptr, bias_values, bias_ids_stride, bias_values_stride, biases,
+               allowed, allowed_stride, masks, allowed_rows, V, 0, 0, logits == out && row_stride == out_stride};
+  a.slice = 4096;
+  const int64_t slices = (V + a.slice - 1) / a.slice;
+  if (slices > 0x7fffffff / batch) return m2r_fail("adjust: grid limits exceeded");
+  a.slices = (uint32_t)slices;
+  const size_t lds = 4 * (size_t)a.slice * ((a.prompt.ids || a.tokens.ids) + (a.bias_ids != nullptr));
+  const dim3 grid((unsigned)(slices * batch)), block(kAdjustThreads);
+  if (dtype == 0) hipLaunchKernelGGL((k_adjust<0>), grid, block, lds, stream, a);
+  else if (dtype == 1) hipLaunchKernelGGL((k_adjust<1>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((k_adjust<2>), grid, block, lds, stream, a);
+  return m2r_check(hipGetLastError(), "adjust launch");
+}

@@ -55,6 +55,9 @@ _SIGNATURES = {
     "m2r_sample_workspace": ([I64] * 2, I64),
     "m2r_sample_call_workspace": ([I64, I64, I, F32, I, F32], I64),
     "m2r_sample": ([P, I, I64, P, P, F32, P, I, P, F32, P, F32, P, P, I64, I64, P, I64, P], I),
+    "m2r_adjust_logits": ([P, I, I64, P, I64] + [P, I, I64, I64, P] * 2 + [P, F32] * 3 + [P, I64, P, I64, I64]
+                          + [P, I64, I64, P] + [I64] * 2 + [P], I),
+    "m2r_conv_pool": ([P, I64, I64, I64, P, I64, I64] + [P] * 7 + [I64] * 5 + [I, I, P], I),
     "m2r_state_step_ridge_layers_workspace": ([I], I64),
     "m2r_state_step_ridge_layers": ([P, I, I64, I64, I64, I64, P, I64, P], I),
     "m2r_state_step_ridge_layers_noalloc": ([P, I, I64, I64, I64, I64, P], I),

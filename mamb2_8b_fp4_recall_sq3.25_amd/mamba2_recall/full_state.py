@@ -126,6 +126,68 @@ def scan(x, dt, A, B, C, D, dt_bias, state, *, lengths=None, slots=None):
     return y, None
 
 
+def allocate_windows(slots, channels, device):
+    """A zeroed pool of convolution windows, FP16 [slots, channels, 4] with the
+    channels next to each other in memory."""
+    if min(slots, channels) <= 0:
+        raise ValueError("Positive geometry required")
+    return torch.zeros((slots, 4, channels), dtype=torch.float16, device=device).permute(0, 2, 1)
+
+
+def convolve(value, weight, bias, window, sizes, *, lengths=None, slots=None, silu=True):
+    """The mixer's short causal convolution with SiLU over a pool of windows,
+    as scan takes its carries: the channels of `sizes` as three contiguous FP16
+    tensors [B,L,n].
+
+    value FP16[B,L,C] (a view with dense tokens is read in place), weight
+    FP16[C,4], bias FP16[C] or None; `window` FP16[S,C,4] (allocate_windows) is
+    the pool, changed in place: a row's last four inputs, of which the last
+    three precede its tokens; zeros for a new request.  `slots` and `lengths`
+    are scan's: outputs past a row's length, and an idle row's, are zero, and an
+    idle or empty row leaves its window alone.  The sum and the SiLU are formed
+    in FP32 and rounded once."""
+    if not isinstance(value, torch.Tensor) or value.dtype != torch.float16 or value.ndim != 3 or not value.is_cuda:
+        raise ValueError("value must be CUDA FP16[batch,tokens,channels]")
+    batch, tokens, channels = value.shape
+    if min(batch, tokens, channels) < 1:
+        raise ValueError("Positive geometry required")
+    if not isinstance(sizes, (tuple, list)) or len(sizes) != 3 \
+            or not all(isinstance(n, int) and n > 0 for n in sizes) or sum(sizes) != channels:
+        raise ValueError("sizes must be three positive channel counts that add up to value's")
+    for t, shape, name in ((weight, (channels, 4), "weight"), (bias, (channels,), "bias")):
+        if t is None and name == "bias":
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape \
+                or t.device != value.device:
+            raise ValueError(f"{name} must be FP16{list(shape)} on the device of value")
+    if (not isinstance(window, torch.Tensor) or window.dtype != torch.float16 or window.ndim != 3
+            or tuple(window.shape[1:]) != (channels, 4) or window.shape[0] < 1 or window.device != value.device
+            or channels > 1 and window.stride(1) != 1 or window.stride(2) < channels
+            or window.shape[0] > 1 and window.stride(0) < 3 * window.stride(2) + channels):
+        raise ValueError("window must be FP16[slots,channels,4] with channels next to each other (allocate_windows)")
+    if slots is None and window.shape[0] < batch:
+        raise ValueError("A window for every batch row, or slots, required")
+    for name, t in (("lengths", lengths), ("slots", slots)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (batch,)
+                              or t.device != value.device):
+            raise ValueError(f"{name} must be int32[batch] on the device of value")
+    if channels > 1 and value.stride(2) != 1:
+        value = value.contiguous()
+    weight = weight.contiguous()
+    if weight.data_ptr() % 8:
+        weight = weight.clone()
+    bias = bias.contiguous() if bias is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    slots = slots.contiguous() if slots is not None else None
+    parts = [value.new_empty((batch, tokens, n)) for n in sizes]
+    p = _native.ptr
+    with _native.device_of(value):
+        _native.call("m2r_conv_pool", p(window), window.shape[0], window.stride(0), window.stride(2), p(value),
+                     value.stride(0), value.stride(1), p(weight), p(bias), p(slots), p(lengths), *map(p, parts), *sizes,
+                     batch, tokens, 4, 1 if silu else 0, _native.stream_of(value))
+    return parts
+
+
 class FullState(_MixerController):
     """Controller with the full-precision carry: prompts in one scan call a
     layer, decode one token at a time, no table and no quantization."""
