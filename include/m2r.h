@@ -441,6 +441,31 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
                                   float top_p_all);
 
 /*
+ * Projection in 8-bit integers, a scale for each token and output channel:
+ *   s_m = max_k |x_mk| / 127, q_mk = rint(127 x_mk / max_k |x_mk|) (ties to even),
+ *   y_mn = (sum_k q_mk w_nk) s_m t_n, the sum exact, the rest binary32, rounded
+ *   once.  A row with a non-finite value gives NaN, a row of zeros zeros.  The
+ *   reference keeps decoded FP16 weights (mamba2_recall/fp4_checkpoint.py:345-405).
+ * m2r_int8_quantize writes rows (dtype 0 binary16, 1 bfloat16; x_stride in
+ * elements) as codes and scales: for weights a row is an output channel.
+ *   tiles: i8, 16-byte aligned, m2r_int8_tiles_bytes(rows, K) bytes, tiles of 16
+ *   rows by 64 inputs (inputs of a row tile after each other; K filled up with
+ *   zeros to a multiple of 128), byte 256 c + 16 r + i of a tile being row r,
+ *   input 16 c + i; rows past the last are left alone.  scale f32[rows].
+ * m2r_int8_linear: x rows as above, w_tiles and w_scale f32[N] the weights', y
+ *   rows of N (y_dtype 2 binary32, too; element row stride); K at most 131,072;
+ *   workspace: 16-byte aligned device memory of m2r_int8_linear_workspace()
+ *   bytes, used on `stream` only.
+ */
+int64_t m2r_int8_tiles_bytes(int64_t rows, int64_t K);
+int m2r_int8_quantize(const void* x, int dtype, int64_t x_stride, void* tiles, float* scale, int64_t rows, int64_t K,
+                      hipStream_t stream);
+int64_t m2r_int8_linear_workspace(int64_t M, int64_t N, int64_t K);
+int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, const void* w_tiles, const float* w_scale, void* y,
+                    int y_dtype, int64_t y_stride, int64_t M, int64_t N, int64_t K, void* workspace,
+                    int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Penalties for repeated tokens, biases and grammar masks on logits (dtype 0
  * binary16, 1 bfloat16, 2 binary32), before m2r_sample.  For a token that is c
  * times in its row of `tokens` (the ids generated so far):

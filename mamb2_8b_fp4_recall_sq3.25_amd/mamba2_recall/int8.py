@@ -1,0 +1,120 @@
+"""Projections in 8-bit integers, a scale for each token and each output channel.
+
+A server keeps a projection's weights in an Int8Weight, half the bytes of
+FP16; `linear` gives each token's row a scale of its own, from its largest
+value, and multiplies the whole numbers:
+
+    s[m] = max|x[m]| / 127,  q[m] = round(127 x[m] / max|x[m]|)
+    y[m] = s[m] * scale * (q[m] @ codes.T)
+
+The reference keeps decoded FP16 weights for all its projections
+(mamba2_recall/fp4_checkpoint.py:345-405); this is for prompts and batches,
+where fp4.gemv_g16 ends.  Runs the gfx950 HIP kernels of libm2r_hip.so
+(m2r_int8_quantize, m2r_int8_linear)."""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+
+MAX_INPUTS = 131072          # sums of that many products fit 32 bits
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _tiles(rows, k):
+    """(tiles of rows, tiles of inputs): 16 rows by 64 inputs each, inputs filled up to a multiple of 128."""
+    return (rows + 15) // 16, (k + 127) // 128 * 2
+
+
+class Int8Weight:
+    """The weights of one projection: `codes` int8[N,K] and `scale` FP32[N],
+    the value of a weight being its code times its channel's scale.  Kept in
+    the order in which the kernels read them; call it, or `linear`, with rows
+    of K."""
+
+    def __init__(self, codes, scale):
+        if not isinstance(codes, torch.Tensor) or codes.dtype != torch.int8 or codes.ndim != 2 or not codes.is_cuda:
+            raise ValueError("codes must be CUDA int8[N,K]")
+        n, k = codes.shape
+        if min(n, k) < 1 or k > MAX_INPUTS:
+            raise ValueError(f"Positive geometry and at most {MAX_INPUTS} inputs required")
+        if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (n,)
+                or scale.device != codes.device):
+            raise ValueError("scale must be FP32[N] on the device of codes")
+        nt, kt = _tiles(n, k)
+        filled = torch.nn.functional.pad(codes, (0, 64 * kt - k, 0, 16 * nt - n))
+        self.features = k, n
+        self.tiles = filled.view(nt, 16, kt, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
+        self.scale = scale.clone(memory_format=torch.contiguous_format)
+
+    @classmethod
+    def quantize(cls, weight):
+        """FP16 or BF16 weights [N,K], each channel by its largest value."""
+        if (not isinstance(weight, torch.Tensor) or weight.dtype not in (torch.float16, torch.bfloat16)
+                or weight.ndim != 2 or not weight.is_cuda):
+            raise ValueError("weight must be CUDA FP16 or BF16 [N,K]")
+        n, k = weight.shape
+        if min(n, k) < 1 or k > MAX_INPUTS:
+            raise ValueError(f"Positive geometry and at most {MAX_INPUTS} inputs required")
+        self = cls.__new__(cls)
+        self.features = k, n
+        weight, stride = _rows(weight.detach(), k)
+        self.tiles = torch.zeros((*_tiles(n, k), 4, 16, 16), dtype=torch.int8, device=weight.device)
+        self.scale = torch.empty(n, dtype=torch.float32, device=weight.device)
+        with _native.device_of(weight):
+            _native.call("m2r_int8_quantize", _native.ptr(weight), _TYPES[weight.dtype], stride, _native.ptr(self.tiles),
+                         _native.ptr(self.scale), n, k, _native.stream_of(weight))
+        return self
+
+    @property
+    def codes(self):
+        """int8[N,K]."""
+        k, n = self.features
+        nt, kt = _tiles(n, k)
+        return self.tiles.permute(0, 3, 1, 2, 4).reshape(16 * nt, 64 * kt)[:n, :k]
+
+    def decode(self, dtype=torch.float16):
+        """The weights' values [N,K], rounded once."""
+        return (self.codes.float() * self.scale[:, None]).to(dtype)
+
+    def __call__(self, x, dtype=None):
+        return linear(x, self, dtype)
+
+
+def _rows(t, features):
+    """`t` [rows, features] with unit column stride, and its row stride."""
+    stride, column = t.stride()
+    if column != 1 and features > 1 or t.shape[0] > 1 and stride < features:
+        t, stride = t.contiguous(), features
+    return t, stride if t.shape[0] > 1 else features
+
+
+def linear(x, weight, dtype=None):
+    """x[..., K] in FP16 or BF16 times an Int8Weight: a new tensor [..., N] of
+    x's type, or of `dtype` (FP16, BF16 or FP32).
+
+    The sum of a row's products is exact, its product with the two scales is
+    formed in FP32 and rounded once, so a row's result depends on the row
+    alone.  A row with a value that is not finite gives NaN.  Forward only."""
+    if not isinstance(weight, Int8Weight):
+        raise ValueError("weight must be an Int8Weight")
+    k, n = weight.features
+    if (not isinstance(x, torch.Tensor) or x.dtype not in (torch.float16, torch.bfloat16) or not x.is_cuda or x.ndim < 1
+            or x.shape[-1] != k or x.device != weight.tiles.device):
+        raise ValueError(f"x must be FP16 or BF16 [..., {k}] on the weights' device")
+    dtype = x.dtype if dtype is None else dtype
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be FP16, BF16 or FP32")
+    rows, stride = _rows(x if x.ndim == 2 else x.reshape(-1, k), k)
+    m = rows.shape[0]
+    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    if m == 0:
+        return y
+    ws_bytes = int(_native.lib().m2r_int8_linear_workspace(m, n, k))
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    p = _native.ptr
+    with _native.device_of(x):
+        _native.call("m2r_int8_linear", p(rows), _TYPES[x.dtype], stride, p(weight.tiles), p(weight.scale), p(y),
+                     _TYPES[dtype], n, m, n, k, p(ws), ws_bytes, _native.stream_of(x))
+    return y
