@@ -446,19 +446,21 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   y_mn = (sum_k q_mk w_nk) s_m t_n, the sum exact, the rest binary32, rounded
  *   once.  A row with a non-finite value gives NaN, a row of zeros zeros.  The
  *   reference keeps decoded FP16 weights (mamba2_recall/fp4_checkpoint.py:345-405).
- * m2r_int8_quantize writes rows (dtype 0 binary16, 1 bfloat16; x_stride in
- * elements) as codes and scales: for weights a row is an output channel.
- *   tiles: i8, 16-byte aligned, m2r_int8_tiles_bytes(rows, K) bytes, tiles of 16
- *   rows by 64 inputs (inputs of a row tile after each other; K filled up with
- *   zeros to a multiple of 128), byte 256 c + 16 r + i of a tile being row r,
- *   input 16 c + i; rows past the last are left alone.  scale f32[rows].
- * m2r_int8_linear: x rows as above, w_tiles and w_scale f32[N] the weights', y
- *   rows of N (y_dtype 2 binary32, too; element row stride); K at most 131,072;
- *   workspace: 16-byte aligned device memory of m2r_int8_linear_workspace()
- *   bytes, used on `stream` only.
+ * m2r_int8_quantize writes weights (N rows of K, dtype 0 binary16, 1 bfloat16;
+ * w_stride in elements) as codes and scales f32[N].
+ *   tiles: i8, 16-byte aligned, m2r_int8_weight_bytes(N, K) bytes: tiles of 16
+ *   channels by 64 inputs, those of one row of tiles after each other, K filled up
+ *   with zeros to a multiple of 128 and N to one of 32 (the bytes of channels past
+ *   N may hold anything).  Channel 32 a + 8 g + 4 t + r lies in row 4 g + r of tile
+ *   row 2 a + t, and byte 256 c + 16 r + i of a tile is row r, input 16 c + i.
+ * m2r_int8_linear: x rows of K (x_dtype as above, element row stride), y rows of N
+ *   (y_dtype 2 binary32, too; element row stride of at most 2^25); K at most
+ *   131,072; workspace: 16-byte aligned device memory of
+ *   m2r_int8_linear_workspace() bytes, used on `stream` only.  Scales whose product
+ *   is below binary32's normal numbers cost digits.
  */
-int64_t m2r_int8_tiles_bytes(int64_t rows, int64_t K);
-int m2r_int8_quantize(const void* x, int dtype, int64_t x_stride, void* tiles, float* scale, int64_t rows, int64_t K,
+int64_t m2r_int8_weight_bytes(int64_t N, int64_t K);
+int m2r_int8_quantize(const void* w, int dtype, int64_t w_stride, void* tiles, float* scale, int64_t N, int64_t K,
                       hipStream_t stream);
 int64_t m2r_int8_linear_workspace(int64_t M, int64_t N, int64_t K);
 int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, const void* w_tiles, const float* w_scale, void* y,

@@ -9,8 +9,11 @@
 // are row l % 16, inputs 16 (l / 16) ... + 15.  A wave's load of a tile is one
 // run of 1 KiB, a copy of it to LDS needs no rearranging, and a read from LDS
 // meets no bank twice.  Inputs are filled up to a multiple of 128 by zeros.
+// Of 32 channels the two tiles of weights take four each in turn, so that the
+// lane that holds rows 4 g ... + 3 of both products holds channels 8 g ... + 7.
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
+#include "m2r_tile.h"
 
 #include <initializer_list>
 
@@ -18,23 +21,30 @@ namespace m2r {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int64_t kTile = 1024;
+constexpr int kTile = 1024;
 static int64_t padded_inputs(int64_t K) { return (K + 127) / 128 * 128; }
 static int64_t row_tiles(int64_t rows) { return (rows + 15) / 16; }
+static int64_t channel_tiles(int64_t channels) { return (channels + 31) / 32 * 2; }
 
 // ---------------------------------------------------------------- codes of rows
 // The code of x is rint(127 x / top), ties to even, as in exact arithmetic.
 // With 11 significant bits in x and top (8 in bfloat16), 127 x / top is either
 // half of an odd number up to 253 or at least 2^-19 of its value away from any
 // such number: |254 x - (2 k + 1) top| is 0 or a unit of a number below 2^19
-// units.  x / top in two roundings is within 2^-23 of its value; rounded to 21
-// bits it is the tie where there is one, and on the right side of it otherwise.
+// units.  x (127 / top) in two roundings is within 2^-23 of its value; rounded
+// to 21 bits it is the tie where there is one, and on the right side of it
+// otherwise.
 struct RowArgs {
   const uint16_t* x;
   int64_t stride, rows, K, Kp;
   uint8_t* tiles;
   float* scale;
+  uint32_t* clear;       // words to set to 0 for the product that follows
+  int64_t clears;
+  int channels;          // 1: rows are output channels of weights
+  int aligned;           // 1: rows start at 16-byte boundaries
 };
 
 template <bool BF16>
@@ -51,39 +61,88 @@ __device__ __forceinline__ uint32_t code_of(uint32_t bits, float factor, int shi
   return __builtin_bit_cast(uint32_t, snapped + 0x1.8p23f);   // the low byte
 }
 
-// A wave a row; 16 inputs of a lane are 16 bytes of a tile.
+struct Chunk { u16x8 h[2]; };   // 16 inputs of a row
+
+// Inputs 16 c ... + 15 of a row, zeros from K on.
+__device__ __forceinline__ Chunk load_chunk(const RowArgs& a, const uint16_t* x, int64_t c) {
+  Chunk v;
+  if (16 * c + 16 <= a.K) {
+    if (a.aligned) {
+      v.h[0] = *(const u16x8*)(x + 16 * c);
+      v.h[1] = *(const u16x8*)(x + 16 * c + 8);
+    } else __builtin_memcpy(&v, x + 16 * c, 32);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v.h[j >> 3][j & 7] = 16 * c + j < a.K ? x[16 * c + j] : (uint16_t)0;
+  }
+  return v;
+}
+
+// A workgroup a row, 16 inputs a thread at a time; the first kHeld of a thread
+// stay in registers between the two passes over the row.  The 16 rows of a tile
+// are workgroups of one XCD, whose L2 puts their pieces of a line together.
+constexpr int kHeld = 4;
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_int8_rows(RowArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ uint32_t tops[4];
+  const int tid = threadIdx.x;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < a.clears; i += (int64_t)gridDim.x * 256) a.clear[i] = 0;
+  const uint32_t turn = blockIdx.x >> 3;
+  const int64_t row = ((int64_t)(turn >> 4) * 8 + (blockIdx.x & 7)) * 16 + (turn & 15);
   if (row >= a.rows) return;
   const uint16_t* x = a.x + row * a.stride;
+  const int64_t chunks = a.Kp / 16;
+  Chunk held[kHeld] = {};
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (tid + 256 * i < chunks) held[i] = load_chunk(a, x, tid + 256 * i);
   uint32_t top = 0;
-  for (int64_t k = lane; k < a.K; k += 64) {
-    const uint32_t v = x[k] & 0x7fffu;
-    top = top > v ? top : v;
-  }
+  auto largest_of = [&](const Chunk& v) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t m = v.h[j >> 3][j & 7] & 0x7fffu;
+      top = top > m ? top : m;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) largest_of(held[i]);
+  for (int64_t c = tid + 256 * kHeld; c < chunks; c += 256) largest_of(load_chunk(a, x, c));
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const uint32_t v = (uint32_t)__shfl_xor((int)top, d);
     top = top > v ? top : v;
   }
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = tops[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = top > tops[w] ? top : tops[w];
   const bool finite = top < (BF16 ? 0x7f80u : 0x7c00u);
   const float largest = half_value<BF16>(top);
   int shift = 0;
   if (BF16 && finite && top) shift = -__builtin_amdgcn_frexp_expf(largest);
   const float factor = finite && top ? 127.f / (BF16 ? __builtin_ldexpf(largest, shift) : largest) : 0.f;
-  if (lane == 0) a.scale[row] = finite ? largest / 127.f : __builtin_nanf("");
-  uint8_t* out = a.tiles + (row >> 4) * 16 * a.Kp + (row & 15) * 16;
-  for (int64_t k0 = lane * 16; k0 < a.Kp; k0 += 1024) {
+  if (tid == 0) a.scale[row] = finite ? largest / 127.f : __builtin_nanf("");
+  int64_t tile = row >> 4;
+  int r = (int)(row & 15);
+  if (a.channels) {
+    tile = 2 * (row >> 5) + (row >> 2 & 1);
+    r = (int)(4 * (row >> 3 & 3) + (row & 3));
+  }
+  uint8_t* out = a.tiles + tile * 16 * a.Kp + r * 16;
+  auto write = [&](const Chunk& v, int64_t c) {
     uint32_t word[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const uint32_t bits = finite && k0 + j < a.K ? x[k0 + j] : 0u;
+      const uint32_t bits = finite ? v.h[j >> 3][j & 7] : 0u;
       word[j >> 2] |= (code_of<BF16>(bits, factor, shift) & 0xffu) << (8 * (j & 3));
     }
-    *(u32x4*)(out + (k0 >> 6) * kTile + (k0 >> 4 & 3) * 256) = u32x4{word[0], word[1], word[2], word[3]};
-  }
+    *(u32x4*)(out + (c >> 2) * kTile + (c & 3) * 256) = u32x4{word[0], word[1], word[2], word[3]};
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (tid + 256 * i < chunks) write(held[i], tid + 256 * i);
+  for (int64_t c = tid + 256 * kHeld; c < chunks; c += 256) write(load_chunk(a, x, c), c);
 }
 
 // ---------------------------------------------------------------- the product
@@ -91,45 +150,491 @@ struct ProductArgs {
   const uint8_t *x, *w;          // tiles
   const float *xs, *ws;          // scales of rows and channels
   void* y;
-  int64_t ys, M, N, Kp;
-  int64_t channel_groups;
+  int64_t ys, M, N;
+  int32_t MT, NT, KT;            // tiles of rows, channels and inputs (even)
+  int32_t splits;                // of the inputs among workgroups
+  uint32_t* tickets;             // a word for each block of outputs, 0
+  uint64_t* parts;               // its splits' sums
+  uint32_t row_blocks, channel_blocks;   // of large tiles
+  uint32_t whole;                // workgroups with a large tile; the others have parts of one
 };
 
-// sum * token * channel in binary32: the smaller scale first, so that no
-// product on the way leaves binary32's range unless the value does (an integer
-// times a subnormal scale is exact).  A NaN scale gives NaN.
-__device__ __forceinline__ float scaled(int sum, float token, float channel) {
-  const bool less = token < channel;
-  return (float)sum * (less ? token : channel) * (less ? channel : token);
-}
-
-template <int DTYPE>
-__device__ __forceinline__ void store_value(void* y, int64_t at, float v) {
-  if constexpr (DTYPE == 0) ((uint16_t*)y)[at] = f2h(v);
-  else if constexpr (DTYPE == 1) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    ((uint16_t*)y)[at] = v != v ? (uint16_t)(u >> 16 | 0x40) : (uint16_t)((u + 0x7fffu + (u >> 16 & 1)) >> 16);
-  } else ((float*)y)[at] = v;
-}
-
-// A wave takes 16 rows by 16 channels.
-template <int DTYPE>
-__global__ __launch_bounds__(256) void k_int8_product(ProductArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t nt = (blockIdx.x % a.channel_groups) * 4 + wave, mt = blockIdx.x / a.channel_groups;
-  if (nt * 16 >= a.N) return;
-  const uint8_t* w = a.w + nt * 16 * a.Kp + lane * 16;
-  const uint8_t* x = a.x + mt * 16 * a.Kp + lane * 16;
-  i32x4 acc = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int64_t k = 0; k < a.Kp / 64; ++k)
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(w + k * kTile), *(const i32x4*)(x + k * kTile), acc, 0, 0,
-                                                0);
-  const int64_t m = mt * 16 + (lane & 15), n = nt * 16 + 4 * (lane >> 4);
-  if (m >= a.M) return;
+// Eight sums of a row and eight channels, scaled and stored.  The scales'
+// product first: it is the same in either order, and while it is a normal
+// number the result is within two roundings of the formula.  Held as binary32
+// before it is rounded to the output's type, in every kernel alike.
+struct Row8 { int v[8]; };
+template <int DTYPE, bool WIDE>
+__device__ __forceinline__ void store_row8(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, int valid, const Row8& sum,
+                                           float token, const float* channel) {
+  float v[8];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (n + r < a.N) store_value<DTYPE>(a.y, m * a.ys + n + r, scaled(acc[r], a.xs[m], a.ws[n + r]));
+  for (int r = 0; r < 8; ++r) {
+    v[r] = (float)sum.v[r] * (token * channel[r]);
+    asm("" : "+v"(v[r]));
+  }
+  constexpr uint32_t kOutside = 0x80000000u;   // past every resource: not stored
+  if constexpr (DTYPE == 2) {
+    u32x4 o[2];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) o[r >> 2][r & 3] = __builtin_bit_cast(uint32_t, v[r]);
+    if constexpr (WIDE) {
+      const uint32_t cell = valid > 0 ? at : kOutside;
+      __builtin_amdgcn_raw_buffer_store_b128(o[0], rsrc, cell, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(o[1], rsrc, cell + 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(o[r >> 2][r & 3], rsrc, r < valid ? at + 4 * r : kOutside, 0, 0);
+    }
+  } else {
+    u16x8 o;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if constexpr (DTYPE == 0) o[r] = f2h(v[r]);
+      else o[r] = __builtin_bit_cast(uint16_t, (__bf16)v[r]);
+    }
+    if constexpr (WIDE) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rsrc, valid > 0 ? at : kOutside, 0, 0);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        __builtin_amdgcn_raw_buffer_store_b16(o[r], rsrc, r < valid ? at + 2 * r : kOutside, 0, 0);
+    }
+  }
+}
+
+// Rows m0 ... + 15 of y from channel n0 on, as far as there are any.  (16 rows of
+// at most 2^25 values stay below 2^31 bytes.)
+template <int DTYPE>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of_y(const ProductArgs& a, int64_t m0, int64_t n0) {
+  constexpr int kSize = DTYPE == 2 ? 4 : 2;
+  const int64_t rows = a.M - m0 < 16 ? a.M - m0 : 16;
+  const int64_t bytes = rows > 0 && n0 < a.N ? ((rows - 1) * a.ys + a.N - n0) * kSize : 0;
+  return __builtin_amdgcn_make_buffer_rsrc((uint8_t*)a.y + (bytes ? (m0 * a.ys + n0) * kSize : 0), 0, (int)bytes,
+                                           0x00027000);
+}
+
+// Sums of splits meet in memory that all XCDs see at one place (stores and
+// loads that are not kept in an XCD's L2), the workgroup that comes last adds
+// them: whole numbers, so the order does not matter.
+__device__ __forceinline__ void put(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get(const uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether the workgroup is the last of its block's splits.  Its stores have
+// completed: each wave waits for its own before the barrier.
+__device__ __forceinline__ bool comes_last(const ProductArgs& a, uint32_t block, uint32_t* shared) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *shared = __hip_atomic_fetch_add(a.tickets + block, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return *shared == (uint32_t)a.splits - 1;
+}
+
+__device__ __forceinline__ void tile_to_lds(const uint8_t* tile, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(tile),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory"); }
+
+// A block of 16 BM rows by 16 BN channels over input tiles k0 ... k1 - 1 by
+// WM x WN waves.  The operands of STAGES stages of KS input tiles lie in LDS,
+// brought by direct transfers STAGES - 1 ahead; a wave reads the next tile's
+// operands while the matrix cores have this one's, and meets the others once a
+// stage.
+template <int DTYPE, bool WIDE, int BM, int BN, int WM, int WN, int STAGES, int KS>
+__device__ __forceinline__ void tile_block(const ProductArgs& a, uint8_t* lds, int m0, int n0, int k0, int k1, int split,
+                                           uint32_t block, uint32_t* shared) {
+  constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, ALL = BM + BN, L = ALL / NW;
+  static_assert(ALL % NW == 0 && TN % 2 == 0 && (KS == 1 || KS == 2) && STAGES > 2, "");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const uint8_t* src[L];      // tiles past the last read the last, for outputs that are not stored
+#pragma unroll
+  for (int j = 0; j < L; ++j) {
+    const int t = wave * L + j;
+    const bool weights = t < BN;
+    int64_t tile = weights ? n0 + t : m0 + t - BN;
+    const int64_t most = (weights ? a.NT : a.MT) - 1;
+    tile = tile < most ? tile : most;
+    src[j] = (weights ? a.w : a.x) + (tile * a.KT + k0) * kTile;
+  }
+  const uint32_t base = lds_address(lds) + wave * L * kTile, off = lane * 16;
+  auto issue = [&](int stage) {
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) tile_to_lds(src[j] + k * kTile, off, base + ((stage * KS + k) * ALL + j) * kTile);
+  };
+  int issued = k0;
+  auto advance = [&]() {      // past the end the last stage again, which nobody reads
+    issued += KS;
+    const int step = issued < k1 ? KS * kTile : 0;
+#pragma unroll
+    for (int j = 0; j < L; ++j) src[j] += step;
+  };
+  i32x4 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  i32x4 wf[2][TN], xf[2][TM];
+  auto fetch = [&](int slot, int step) {
+    const uint8_t* s = lds + step * ALL * kTile + off;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wf[slot][i] = *(const i32x4*)(s + (wn * TN + i) * kTile);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) xf[slot][j] = *(const i32x4*)(s + (BN + wm * TM + j) * kTile);
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    issue(s);
+    advance();
+  }
+  wait_loads<(STAGES - 2) * L * KS>();
+  meet();
+  fetch(0, 0);
+  int write = STAGES - 1, read = 1;
+  for (int kt = k0; kt < k1; kt += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (KS == 1 || u == 1) {
+        // the next stage is here, and nobody reads the one before this any more
+        wait_loads<(STAGES - 3) * L * KS>();
+        meet();
+        issue(write);
+        advance();
+        write = write + 1 < STAGES ? write + 1 : 0;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(1 - u, read);
+      read = read + 1 < STAGES * KS ? read + 1 : 0;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i], xf[u][j], acc[i][j], 0, 0, 0);
+      // reads between the products, not in front of them
+      constexpr int PER = TN * TM / (TN + TM);
+#pragma unroll
+      for (int q = 0; q < TN + TM; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, TN * TM - PER * (TN + TM), 0);
+    }
+  }
+  if (a.splits > 1) {
+    constexpr int kPart = NW * TN * TM * 128;   // 8-byte words of a block's sums
+    uint64_t* mine = a.parts + ((int64_t)block * a.splits) * kPart + wave * TN * TM * 128 + lane;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          put(mine + (int64_t)split * kPart + ((i * TM + j) * 2 + h) * 64,
+              (uint64_t)(uint32_t)acc[i][j][2 * h] | (uint64_t)(uint32_t)acc[i][j][2 * h + 1] << 32);
+    if (!comes_last(a, block, shared)) return;
+    for (int s = 0; s < a.splits; ++s) {
+      if (s == split) continue;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t v = get(mine + (int64_t)s * kPart + ((i * TM + j) * 2 + h) * 64);
+            acc[i][j][2 * h] += (int)(uint32_t)v;
+            acc[i][j][2 * h + 1] += (int)(uint32_t)(v >> 32);
+          }
+    }
+  }
+  // every scale of the wave's block in one go, then its outputs
+  float ts[TM], cs[TN / 2][8];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const int64_t m = (int64_t)(m0 + wm * TM + j) * 16 + (lane & 15);
+    ts[j] = a.xs[m < a.M ? m : a.M - 1];
+  }
+  const int64_t first = (int64_t)(n0 + wn * TN) * 16 + 8 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < TN / 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int64_t n = first + 32 * i + r;
+      cs[i][r] = a.ws[n < a.N ? n : a.N - 1];
+    }
+  wait_loads<0>();            // the transfers that nobody read, too
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const __amdgpu_buffer_rsrc_t y = rows_of_y<DTYPE>(a, (int64_t)(m0 + wm * TM + j) * 16, (int64_t)(n0 + wn * TN) * 16);
+#pragma unroll
+    for (int i = 0; i < TN / 2; ++i) {
+      Row8 s;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s.v[r] = acc[2 * i][j][r];
+        s.v[r + 4] = acc[2 * i + 1][j][r];
+      }
+      const int64_t left = a.N - (first + 32 * i);
+      const uint32_t at = (uint32_t)(((lane & 15) * a.ys + 32 * i + 8 * (lane >> 4)) * (DTYPE == 2 ? 4 : 2));
+      store_row8<DTYPE, WIDE>(y, at, left < 8 ? (int)left : 8, s, ts[j], cs[i]);
+    }
+  }
+}
+
+// Workgroups take consecutive blocks within an XCD, eight row blocks before the
+// next channel block, so that the 32 of an XCD share operands in its L2.
+__device__ __forceinline__ void block_place(uint32_t linear, uint32_t rows, uint32_t channels, uint32_t& rb, uint32_t& cb) {
+  const uint32_t group = linear / (8 * channels), in = linear - group * 8 * channels;
+  const uint32_t here = rows - group * 8 < 8 ? rows - group * 8 : 8;
+  rb = group * 8 + in % here;
+  cb = in / here;
+}
+__device__ __forceinline__ uint32_t on_one_xcd(uint32_t index, uint32_t count) {
+  const uint32_t per = count >> 3, more = count & 7, xcd = index & 7;
+  return xcd * per + (xcd < more ? xcd : more) + (index >> 3);
+}
+
+constexpr int kBig = 16;      // tiles a side of a large block
+constexpr int kTileLds = 128 * 1024;
+
+// PART: what the workgroups past `whole` take.  0: there are none; 1: halves of a
+// large block's channels; 2: its quarters; 3: blocks of a quarter's size, of
+// which row_blocks and channel_blocks then count, and splits of their inputs.
+template <int DTYPE, bool WIDE, int PART>
+__global__ __launch_bounds__(512, 2) void k_int8_tiles(ProductArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  uint32_t* shared = (uint32_t*)(lds + kTileLds);
+  const uint32_t blocks = a.row_blocks * a.channel_blocks;
+  uint32_t rb, cb;
+  if constexpr (PART == 3) {
+    const uint32_t index = on_one_xcd(blockIdx.x, blocks * a.splits), block = index / a.splits,
+                   split = index - block * a.splits;
+    block_place(block, a.row_blocks, a.channel_blocks, rb, cb);
+    const int pairs = a.KT / 2;
+    const int k0 = 2 * (int)((int64_t)pairs * split / a.splits), k1 = 2 * (int)((int64_t)pairs * (split + 1) / a.splits);
+    tile_block<DTYPE, WIDE, 8, 8, 4, 2, 4, 2>(a, lds, rb * 8, cb * 8, k0, k1, split, block, shared);
+    return;
+  }
+  if (blockIdx.x < a.whole) {
+    block_place(on_one_xcd(blockIdx.x, a.whole), a.row_blocks, a.channel_blocks, rb, cb);
+    tile_block<DTYPE, WIDE, kBig, kBig, 4, 2, 4, 1>(a, lds, rb * kBig, cb * kBig, 0, a.KT, 0, 0, shared);
+  } else if constexpr (PART == 1 || PART == 2) {
+    const uint32_t index = on_one_xcd(blockIdx.x - a.whole, (blocks - a.whole) * 2 * PART);
+    block_place(a.whole + index / (2 * PART), a.row_blocks, a.channel_blocks, rb, cb);
+    const int m0 = rb * kBig + (PART == 2 && (index & 2) ? 8 : 0), n0 = cb * kBig + (index & 1) * 8;
+    if (m0 >= a.MT || n0 >= a.NT) return;
+    if constexpr (PART == 1) tile_block<DTYPE, WIDE, kBig, 8, 4, 2, 4, 1>(a, lds, m0, n0, 0, a.KT, 0, 0, shared);
+    else tile_block<DTYPE, WIDE, 8, 8, 4, 2, 4, 2>(a, lds, m0, n0, 0, a.KT, 0, 0, shared);
+  }
+}
+
+// A few rows: bound by the weights' bytes.  A workgroup takes 64 channels, its
+// waves (and `splits` workgroups) a range of inputs each; operands go straight
+// to registers, kDeep input tiles ahead.
+constexpr int kFewWaves = 4, kDeep = 4;
+template <int DTYPE, bool WIDE, int BM>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void k_int8_few(ProductArgs a) {
+  __shared__ i32x4 sums[kFewWaves][4 * BM][64];
+  __shared__ uint32_t shared;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t groups = (uint32_t)(a.NT + 3) / 4, group = blockIdx.x % groups, split = blockIdx.x / groups;
+  const int pieces = a.splits * kFewWaves, piece = split * kFewWaves + wave;
+  const int k0 = (int)((int64_t)a.KT * piece / pieces), n = (int)((int64_t)a.KT * (piece + 1) / pieces) - k0;
+  const uint8_t *wp[4], *xp[BM];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t t = 4 * group + i < (uint32_t)a.NT ? 4 * group + i : a.NT - 1;
+    wp[i] = a.w + (t * a.KT + k0) * kTile;
+  }
+#pragma unroll
+  for (int j = 0; j < BM; ++j) xp[j] = a.x + ((int64_t)(j < a.MT ? j : a.MT - 1) * a.KT + k0) * kTile;
+  i32x4 acc[4][BM];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < BM; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  i32x4 wf[kDeep][4], xf[kDeep][BM];
+  auto load = [&](int slot, int k) {
+    const int at = (k < n ? k : n - 1) * kTile + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wf[slot][i] = *(const i32x4*)(wp[i] + at);
+#pragma unroll
+    for (int j = 0; j < BM; ++j) xf[slot][j] = *(const i32x4*)(xp[j] + at);
+  };
+  if (n > 0) {
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) load(d, d);
+    for (int k = 0; k < n; k += kDeep) {
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        if (k + d < n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < BM; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[d][i], xf[d][j], acc[i][j], 0, 0, 0);
+        }
+        load(d, k + d + kDeep);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < BM; ++j) sums[wave][i * BM + j][lane] = acc[i][j];
+  __syncthreads();
+  // 32 channels of 16 rows a wave at a time
+  constexpr int kUnits = (2 * BM + kFewWaves - 1) / kFewWaves;
+  Row8 total[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int unit = wave + u * kFewWaves, i = unit & 1, j = unit >> 1;
+    if (unit >= 2 * BM) break;
+    i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      lo += sums[w][2 * i * BM + j][lane];
+      hi += sums[w][(2 * i + 1) * BM + j][lane];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      total[u].v[r] = lo[r];
+      total[u].v[r + 4] = hi[r];
+    }
+  }
+  if (a.splits > 1) {
+    constexpr int kPart = 2 * BM * 256;
+    uint64_t* mine = a.parts + (int64_t)group * a.splits * kPart + lane;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int unit = wave + u * kFewWaves;
+      if (unit >= 2 * BM) break;
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        put(mine + (int64_t)split * kPart + (unit * 4 + h) * 64,
+            (uint64_t)(uint32_t)total[u].v[2 * h] | (uint64_t)(uint32_t)total[u].v[2 * h + 1] << 32);
+    }
+    if (!comes_last(a, group, &shared)) return;
+    for (uint32_t s = 0; s < (uint32_t)a.splits; ++s) {
+      if (s == split) continue;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int unit = wave + u * kFewWaves;
+        if (unit >= 2 * BM) break;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint64_t v = get(mine + (int64_t)s * kPart + (unit * 4 + h) * 64);
+          total[u].v[2 * h] += (int)(uint32_t)v;
+          total[u].v[2 * h + 1] += (int)(uint32_t)(v >> 32);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int unit = wave + u * kFewWaves, i = unit & 1, j = unit >> 1;
+    if (unit >= 2 * BM) break;
+    const int64_t m = 16 * j + (lane & 15), n0 = (int64_t)group * 64 + 32 * i, first = n0 + 8 * (lane >> 4);
+    float cs[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) cs[r] = a.ws[first + r < a.N ? first + r : a.N - 1];
+    const int64_t left = a.N - first;
+    store_row8<DTYPE, WIDE>(rows_of_y<DTYPE>(a, 16 * j, n0),
+                            (uint32_t)(((lane & 15) * a.ys + 8 * (lane >> 4)) * (DTYPE == 2 ? 4 : 2)),
+                            left < 8 ? (int)left : 8, total[u], a.xs[m < a.M ? m : a.M - 1], cs);
+  }
+}
+
+// ---------------------------------------------------------------- which kernel
+constexpr int64_t kFewRows = 64;
+
+struct Plan {
+  int few;                 // row tiles of k_int8_few, or 0
+  int part;                // how blocks past `whole` are cut
+  int splits;
+  uint32_t rb, cb, whole, grid;
+  int64_t tickets, parts;  // words of 4 and of 8 bytes
+};
+
+static Plan int8_plan(int64_t M, int64_t N, int64_t K) {
+  Plan p{};
+  const int64_t MT = row_tiles(M), NT = channel_tiles(N), KT = padded_inputs(K) / 64;
+  p.splits = 1;
+  if (M <= kFewRows) {
+    p.few = MT == 1 ? 1 : (MT == 2 ? 2 : 4);
+    const int64_t groups = (NT + 3) / 4;
+    int64_t s = 512 / groups;
+    const int64_t most = KT / (4 * kFewWaves);
+    s = s < most ? s : most;
+    p.splits = (int)(s < 1 ? 1 : (s < 8 ? s : 8));
+    p.grid = (uint32_t)(groups * p.splits);
+    if (p.splits > 1) {
+      p.tickets = groups;
+      p.parts = groups * p.splits * 2 * p.few * 256;
+    }
+    return p;
+  }
+  const int64_t rb = (MT + kBig - 1) / kBig, cb = (NT + kBig - 1) / kBig, all = rb * cb, rest = all % 256;
+  const int64_t rs = (MT + 7) / 8, cs = (NT + 7) / 8, small = rs * cs;
+  // Rounds of 256 workgroups, in large blocks: the last round's blocks whole, in
+  // halves, in quarters, or everything in blocks of a quarter's size.
+  const double full = (double)(all / 256), rounds[4] = {full + (rest ? 1 : 0), full + 0.62 * ((2 * rest + 255) / 256),
+                                                        full + 0.42 * ((4 * rest + 255) / 256),
+                                                        0.42 * ((small + 255) / 256)};
+  for (int i = 1; i < 4; ++i)
+    if (rounds[i] < rounds[p.part]) p.part = i;
+  p.rb = (uint32_t)(p.part == 3 ? rs : rb);
+  p.cb = (uint32_t)(p.part == 3 ? cs : cb);
+  p.whole = (uint32_t)(p.part == 0 ? all : (p.part == 3 ? 0 : all - rest));
+  if (p.part == 3) {
+    int64_t s = 256 / small;
+    const int64_t most = KT / 16;
+    s = s < most ? s : most;
+    p.splits = (int)(s < 1 ? 1 : (s < 8 ? s : 8));
+    if (p.splits > 1) {
+      p.tickets = small;
+      p.parts = small * p.splits * 8192;
+    }
+    p.grid = (uint32_t)(small * p.splits);
+  } else p.grid = (uint32_t)(p.whole + 2 * p.part * (all - p.whole));
+  return p;
+}
+
+template <int DTYPE, bool WIDE, int PART>
+static int tiles_launch(const Plan& p, const ProductArgs& a, hipStream_t stream) {
+  static const hipError_t allowed = hipFuncSetAttribute((const void*)k_int8_tiles<DTYPE, WIDE, PART>,
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds + 16);
+  if (int rc = m2r_check(allowed, "int8 shared memory")) return rc;
+  hipLaunchKernelGGL((k_int8_tiles<DTYPE, WIDE, PART>), dim3(p.grid), dim3(512), kTileLds + 16, stream, a);
+  return 0;
+}
+template <int DTYPE, bool WIDE>
+static int int8_product(const Plan& p, const ProductArgs& a, hipStream_t stream) {
+  if (p.few) {
+    const dim3 grid(p.grid), block(64 * kFewWaves);
+    if (p.few == 1) hipLaunchKernelGGL((k_int8_few<DTYPE, WIDE, 1>), grid, block, 0, stream, a);
+    else if (p.few == 2) hipLaunchKernelGGL((k_int8_few<DTYPE, WIDE, 2>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_int8_few<DTYPE, WIDE, 4>), grid, block, 0, stream, a);
+  } else {
+    int rc;
+    if (p.part == 0) rc = tiles_launch<DTYPE, WIDE, 0>(p, a, stream);
+    else if (p.part == 1) rc = tiles_launch<DTYPE, WIDE, 1>(p, a, stream);
+    else if (p.part == 2) rc = tiles_launch<DTYPE, WIDE, 2>(p, a, stream);
+    else rc = tiles_launch<DTYPE, WIDE, 3>(p, a, stream);
+    if (rc) return rc;
+  }
+  return m2r_check(hipGetLastError(), "int8 product launch");
 }
 
 }  // namespace m2r
@@ -137,9 +642,10 @@ __global__ __launch_bounds__(256) void k_int8_product(ProductArgs a) {
 using namespace m2r;
 
 static int int8_rows(const void* x, int dtype, int64_t stride, int64_t rows, int64_t K, uint8_t* tiles, float* scale,
-                     hipStream_t stream) {
-  const RowArgs a{(const uint16_t*)x, stride, rows, K, padded_inputs(K), tiles, scale};
-  const dim3 grid((unsigned)((rows + 3) / 4)), block(256);
+                     int channels, uint32_t* clear, int64_t clears, hipStream_t stream) {
+  const RowArgs a{(const uint16_t*)x, stride, rows, K, padded_inputs(K), tiles, scale, clear, clears, channels,
+                  !((uintptr_t)x & 15) && !(stride & 7)};
+  const dim3 grid((unsigned)((rows + 127) / 128 * 128)), block(256);
   if (dtype == 0) hipLaunchKernelGGL((k_int8_rows<false>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((k_int8_rows<true>), grid, block, 0, stream, a);
   return m2r_check(hipGetLastError(), "int8 rows launch");
@@ -151,24 +657,29 @@ static int int8_limits(int64_t rows, int64_t K) {
   return 0;
 }
 
-extern "C" int64_t m2r_int8_tiles_bytes(int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0) return 0;
-  return row_tiles(rows) * 16 * padded_inputs(K);
+extern "C" int64_t m2r_int8_weight_bytes(int64_t N, int64_t K) {
+  if (N <= 0 || K <= 0) return 0;
+  return channel_tiles(N) * 16 * padded_inputs(K);
 }
 
-extern "C" int m2r_int8_quantize(const void* x, int dtype, int64_t x_stride, void* tiles, float* scale, int64_t rows,
+extern "C" int m2r_int8_quantize(const void* w, int dtype, int64_t w_stride, void* tiles, float* scale, int64_t N,
                                  int64_t K, hipStream_t stream) {
-  if (int rc = int8_limits(rows, K)) return rc;
-  if (dtype < 0 || dtype > 1) return m2r_fail("int8: x must be binary16 or bfloat16");
-  if (!x || !tiles || !scale) return m2r_fail("int8: null pointer");
-  if (x_stride < 0) return m2r_fail("int8: negative stride");
+  if (int rc = int8_limits(N, K)) return rc;
+  if (dtype < 0 || dtype > 1) return m2r_fail("int8: weights must be binary16 or bfloat16");
+  if (!w || !tiles || !scale) return m2r_fail("int8: null pointer");
+  if (w_stride < 0) return m2r_fail("int8: negative stride");
   if ((uintptr_t)tiles & 15) return m2r_fail("int8: tiles must be 16-byte aligned");
-  return int8_rows(x, dtype, x_stride, rows, K, (uint8_t*)tiles, scale, stream);
+  return int8_rows(w, dtype, w_stride, N, K, (uint8_t*)tiles, scale, 1, nullptr, 0, stream);
 }
+
+// Codes, scales, then the tickets and sums of splits, each from 256 bytes on.
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+static int64_t int8_codes_bytes(int64_t M, int64_t K) { return up256(row_tiles(M) * 16 * padded_inputs(K)); }
 
 extern "C" int64_t m2r_int8_linear_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return m2r_int8_tiles_bytes(M, K) + 4 * M;
+  const Plan p = int8_plan(M, N, K);
+  return int8_codes_bytes(M, K) + up256(4 * M) + up256(4 * p.tickets) + 8 * p.parts;
 }
 
 extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, const void* w_tiles, const float* w_scale,
@@ -176,7 +687,7 @@ extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, con
                                int64_t workspace_bytes, hipStream_t stream) {
   if (N <= 0) return m2r_fail("int8: non-positive shape");
   if (int rc = int8_limits(M, K)) return rc;
-  if (N > (int64_t)1 << 24) return m2r_fail("int8: size limits");
+  if (N > (int64_t)1 << 24 || y_stride > (int64_t)1 << 25) return m2r_fail("int8: size limits");
   if (x_dtype < 0 || x_dtype > 1) return m2r_fail("int8: x must be binary16 or bfloat16");
   if (y_dtype < 0 || y_dtype > 2) return m2r_fail("int8: y must be binary16, bfloat16 or binary32");
   for (const void* p : {x, w_tiles, (const void*)w_scale, (const void*)y, (const void*)workspace})
@@ -186,15 +697,19 @@ extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, con
   if ((uintptr_t)w_tiles & 15) return m2r_fail("int8: tiles must be 16-byte aligned");
   if ((uintptr_t)workspace & 15 || workspace_bytes < m2r_int8_linear_workspace(M, N, K))
     return m2r_fail("int8: workspace too small or not 16-byte aligned");
+  const int64_t MT = row_tiles(M), NT = channel_tiles(N);
+  if ((MT + kBig - 1) / kBig * ((NT + kBig - 1) / kBig) > 0x7fffffff / 64) return m2r_fail("int8: grid limits exceeded");
+  const Plan p = int8_plan(M, N, K);
   uint8_t* codes = (uint8_t*)workspace;
-  float* scale = (float*)(codes + m2r_int8_tiles_bytes(M, K));
-  if (int rc = int8_rows(x, x_dtype, x_stride, M, K, codes, scale, stream)) return rc;
-  const int64_t groups = (N + 63) / 64;
-  if (groups * row_tiles(M) > 0x7fffffff) return m2r_fail("int8: grid limits exceeded");
-  const ProductArgs a{codes, (const uint8_t*)w_tiles, scale, w_scale, y, y_stride, M, N, padded_inputs(K), groups};
-  const dim3 grid((unsigned)(groups * row_tiles(M))), block(256);
-  if (y_dtype == 0) hipLaunchKernelGGL((k_int8_product<0>), grid, block, 0, stream, a);
-  else if (y_dtype == 1) hipLaunchKernelGGL((k_int8_product<1>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((k_int8_product<2>), grid, block, 0, stream, a);
-  return m2r_check(hipGetLastError(), "int8 product launch");
+  float* scale = (float*)(codes + int8_codes_bytes(M, K));
+  uint32_t* tickets = (uint32_t*)((uint8_t*)scale + up256(4 * M));
+  uint64_t* parts = (uint64_t*)((uint8_t*)tickets + up256(4 * p.tickets));
+  if (int rc = int8_rows(x, x_dtype, x_stride, M, K, codes, scale, 0, tickets, p.tickets, stream)) return rc;
+  const ProductArgs a{codes, (const uint8_t*)w_tiles, scale, w_scale, y, y_stride, M, N, (int32_t)MT, (int32_t)NT,
+                      (int32_t)(padded_inputs(K) / 64), p.splits, tickets, parts, p.rb, p.cb, p.whole};
+  // whole eights of channels, dword-aligned: stores of 16 bytes
+  const bool wide = !(N & 7) && !(y_stride & 1) && !((uintptr_t)y & 3);
+  if (y_dtype == 0) return wide ? int8_product<0, true>(p, a, stream) : int8_product<0, false>(p, a, stream);
+  if (y_dtype == 1) return wide ? int8_product<1, true>(p, a, stream) : int8_product<1, false>(p, a, stream);
+  return wide ? int8_product<2, true>(p, a, stream) : int8_product<2, false>(p, a, stream);
 }

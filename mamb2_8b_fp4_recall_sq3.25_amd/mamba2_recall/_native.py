@@ -57,7 +57,7 @@ _SIGNATURES = {
     "m2r_sample": ([P, I, I64, P, P, F32, P, I, P, F32, P, F32, P, P, I64, I64, P, I64, P], I),
     "m2r_adjust_logits": ([P, I, I64, P, I64] + [P, I, I64, I64, P] * 2 + [P, F32] * 3 + [P, I64, P, I64, I64]
                           + [P, I64, I64, P] + [I64] * 2 + [P], I),
-    "m2r_int8_tiles_bytes": ([I64] * 2, I64),
+    "m2r_int8_weight_bytes": ([I64] * 2, I64),
     "m2r_int8_quantize": ([P, I, I64, P, P, I64, I64, P], I),
     "m2r_int8_linear_workspace": ([I64] * 3, I64),
     "m2r_int8_linear": ([P, I, I64, P, P, P, I, I64] + [I64] * 3 + [P, I64, P], I),

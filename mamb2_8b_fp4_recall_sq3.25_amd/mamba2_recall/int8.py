@@ -22,9 +22,11 @@ MAX_INPUTS = 131072          # sums of that many products fit 32 bits
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _tiles(rows, k):
-    """(tiles of rows, tiles of inputs): 16 rows by 64 inputs each, inputs filled up to a multiple of 128."""
-    return (rows + 15) // 16, (k + 127) // 128 * 2
+# The kernels read weights in tiles of 16 channels by 64 inputs.  Of 32 channels
+# the first tile has the first four
+# of every eight; N is filled up to a multiple of 32, K to one of 128.
+def _groups(n, k):
+    return (n + 31) // 32, (k + 127) // 128 * 2
 
 
 class Int8Weight:
@@ -42,10 +44,10 @@ class Int8Weight:
         if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (n,)
                 or scale.device != codes.device):
             raise ValueError("scale must be FP32[N] on the device of codes")
-        nt, kt = _tiles(n, k)
-        filled = torch.nn.functional.pad(codes, (0, 64 * kt - k, 0, 16 * nt - n))
+        groups, steps = _groups(n, k)
+        filled = torch.nn.functional.pad(codes, (0, 64 * steps - k, 0, 32 * groups - n))
         self.features = k, n
-        self.tiles = filled.view(nt, 16, kt, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
+        self.tiles = filled.view(groups, 4, 2, 4, steps, 4, 16).permute(0, 2, 4, 5, 1, 3, 6).contiguous()
         self.scale = scale.clone(memory_format=torch.contiguous_format)
 
     @classmethod
@@ -60,7 +62,8 @@ class Int8Weight:
         self = cls.__new__(cls)
         self.features = k, n
         weight, stride = _rows(weight.detach(), k)
-        self.tiles = torch.zeros((*_tiles(n, k), 4, 16, 16), dtype=torch.int8, device=weight.device)
+        groups, steps = _groups(n, k)
+        self.tiles = torch.zeros((groups, 2, steps, 4, 4, 4, 16), dtype=torch.int8, device=weight.device)
         self.scale = torch.empty(n, dtype=torch.float32, device=weight.device)
         with _native.device_of(weight):
             _native.call("m2r_int8_quantize", _native.ptr(weight), _TYPES[weight.dtype], stride, _native.ptr(self.tiles),
@@ -71,8 +74,8 @@ class Int8Weight:
     def codes(self):
         """int8[N,K]."""
         k, n = self.features
-        nt, kt = _tiles(n, k)
-        return self.tiles.permute(0, 3, 1, 2, 4).reshape(16 * nt, 64 * kt)[:n, :k]
+        groups, steps = _groups(n, k)
+        return self.tiles.permute(0, 4, 1, 5, 2, 3, 6).reshape(32 * groups, 64 * steps)[:n, :k]
 
     def decode(self, dtype=torch.float16):
         """The weights' values [N,K], rounded once."""
