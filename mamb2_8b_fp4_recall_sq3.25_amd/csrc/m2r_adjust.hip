@@ -10,8 +10,13 @@
 //
 // A workgroup takes a slice of a row's tokens.  It counts the row's ids that
 // lie in its slice in a table in LDS (whole numbers: the order does not
-// matter), then passes over its logits once; no counts are kept in memory.
-// Bound by memory: each logit read and written once.
+// matter), then passes over its logits once, which were on their way meanwhile;
+// no counts are kept in memory.  Bound by memory: each logit read and written
+// once.  64 rows of 256,000 in binary32 with lists, biases and masks 32 us, 4.2
+// TB/s; one row of binary16 4.3 us.  With long lists every slice reads all ids
+// of its row (8 rows with up to 104,000 ids: 17 us, a thread's 100 ids and their
+// counting; plain stores of the prompt's flags in place of atomics, twice as many
+// loads in flight and other slices changed nothing).
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
@@ -25,6 +30,7 @@ struct IdList {
   const int32_t* lengths;
   int wide;              // 1: int64
 };
+struct alignas(16) Word4 { uint32_t w[4]; };
 struct RowValue {
   const float* row;      // a value for each row, or null
   float all;
@@ -44,11 +50,9 @@ struct AdjustArgs {
   const int32_t* allowed_rows;
   int64_t V;
   uint32_t slices;
-  int slice;             // tokens of a workgroup, a multiple of 32
   int in_place;
 };
 
-constexpr int kAdjustThreads = 512;
 constexpr uint32_t kInPrompt = 0x80000000u;   // of a table's word; the rest counts the generated tokens
 
 template <int DTYPE> struct LogitType { typedef uint16_t T; };
@@ -72,51 +76,74 @@ __device__ __forceinline__ typename LogitType<DTYPE>::T logit_rounded(float v) {
 __device__ __forceinline__ float row_value(const RowValue& v, int64_t row) { return v.row ? v.row[row] : v.all; }
 
 // Calls f(token of the slice) for each id of the row's list in [v0, v0 + size).
-template <typename F>
+// Sixteen bytes of ids a thread, four such loads at a time.
+template <int THREADS, int kLoads, typename F>
 __device__ __forceinline__ void for_ids(const IdList& l, int64_t row, int64_t v0, int size, F f) {
   if (!l.ids) return;
   int64_t n = l.lengths ? l.lengths[row] : l.n;
   n = n < l.n ? n : l.n;
+  const uint32_t from = (uint32_t)v0;
   if (l.wide) {
     const int64_t* p = (const int64_t*)l.ids + row * l.stride;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < n; i += kAdjustThreads) {
-      const uint64_t at = (uint64_t)(p[i] - v0);
-      if (at < (uint64_t)size) f((int)at);
+    for (int64_t i0 = 0; i0 < n; i0 += THREADS * 2 * kLoads) {
+      uint64_t id[kLoads][2];
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        if (i0 + j * THREADS * 2 >= n) break;
+        const int64_t i = i0 + (j * THREADS + threadIdx.x) * 2;
+        if (i + 2 <= n) __builtin_memcpy(id[j], p + i, 16);
+        else {
+          id[j][0] = i < n ? (uint64_t)p[i] : ~0ull;
+          id[j][1] = ~0ull;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        if (i0 + j * THREADS * 2 >= n) break;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t at = (uint32_t)id[j][k] - from;
+          if (at < (uint32_t)size && !(id[j][k] >> 32)) f((int)at);
+        }
+      }
     }
   } else {
-    const int32_t* p = (const int32_t*)l.ids + row * l.stride;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < n; i += kAdjustThreads) {
-      const uint64_t at = (uint64_t)((int64_t)p[i] - v0);
-      if (at < (uint64_t)size) f((int)at);
+    const uint32_t* p = (const uint32_t*)l.ids + row * l.stride;
+    for (int64_t i0 = 0; i0 < n; i0 += THREADS * 4 * kLoads) {
+      uint32_t id[kLoads][4];
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        if (i0 + j * THREADS * 4 >= n) break;
+        const int64_t i = i0 + (j * THREADS + threadIdx.x) * 4;
+        if (i + 4 <= n) __builtin_memcpy(id[j], p + i, 16);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) id[j][k] = i + k < n ? p[i + k] : ~0u;
+      }
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        if (i0 + j * THREADS * 4 >= n) break;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = id[j][k] - from;   // (a negative id is above every token)
+          if (at < (uint32_t)size) f((int)at);
+        }
+      }
     }
   }
 }
 
-template <int DTYPE>
-__global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustArgs a) {
+template <int DTYPE, int THREADS, int SLICE, int LOADS>
+__global__ __launch_bounds__(THREADS) void k_adjust(AdjustArgs a) {
   typedef typename LogitType<DTYPE>::T T;
-  constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ uint32_t table[];            // [slice], and [slice] places in the list of biases
-  const int64_t row = blockIdx.x / a.slices, v0 = (int64_t)(blockIdx.x % a.slices) * a.slice;
-  const int size = (int)(a.V - v0 < a.slice ? a.V - v0 : a.slice);
+  constexpr int VEC = 16 / sizeof(T), ROUNDS = (SLICE + THREADS * VEC - 1) / (THREADS * VEC);
+  extern __shared__ __attribute__((aligned(16))) uint32_t table[];   // [SLICE], and [SLICE] places in the list of biases
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.slices, v0 = (int64_t)(blockIdx.x % a.slices) * SLICE;
+  const int size = (int)(a.V - v0 < SLICE ? a.V - v0 : SLICE);
   const T* src = (const T*)a.logits + row * a.ls + v0;
   T* dst = (T*)a.out + row * a.os + v0;
-  const bool counted = a.prompt.ids || a.tokens.ids, biased = a.bias_ids != nullptr;
-  uint32_t* place = table + (counted ? a.slice : 0);
-  if (counted || biased) {
-    for (int i = threadIdx.x; i < a.slice * (counted + biased); i += kAdjustThreads) table[i] = 0;
-    __syncthreads();
-    for_ids(a.prompt, row, v0, size, [&](int at) { atomicOr(&table[at], kInPrompt); });
-    for_ids(a.tokens, row, v0, size, [&](int at) { atomicAdd(&table[at], 1u); });
-    if (biased)
-      for (int64_t i = threadIdx.x; i < a.biases; i += kAdjustThreads) {
-        const uint64_t at = (uint64_t)((int64_t)a.bias_ids[row * a.bias_ids_stride + i] - v0);
-        if (at < (uint64_t)size) atomicMax(&place[at], (uint32_t)i + 1u);   // the list's last entry for a token
-      }
-    __syncthreads();
-  }
+  // what the pass over the logits needs is on its way while the ids are counted
   const float repetition = row_value(a.repetition, row), presence = row_value(a.presence, row),
               frequency = row_value(a.frequency, row);
   const uint32_t* allowed = nullptr;
@@ -124,9 +151,36 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustArgs a) {
     const int64_t m = a.allowed_rows ? a.allowed_rows[row] : row;
     if (m >= 0 && m < a.masks) allowed = a.allowed + m * a.allowed_stride + (v0 >> 5);
   }
-  for (int i = threadIdx.x * VEC; i < size; i += kAdjustThreads * VEC) {
-    uint32_t free = 0xffffffffu;
-    if (allowed) free = allowed[i >> 5] >> (i & 31);
+  T l[ROUNDS][VEC];
+  uint32_t free[ROUNDS];
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const int i = (u * THREADS + tid) * VEC;
+    free[u] = allowed && i < size ? allowed[i >> 5] >> (i & 31) : 0xffffffffu;
+    if (i + VEC <= size) {
+      if (!a.in_place) __builtin_memcpy(l[u], src + i, 16);
+    } else
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) l[u][k] = i + k < size ? src[i + k] : T(0);
+  }
+  const bool counted = a.prompt.ids || a.tokens.ids, biased = a.bias_ids != nullptr;
+  uint32_t* place = table + (counted ? SLICE : 0);
+  if (counted || biased) {
+    for (int i = 4 * tid; i < SLICE * (counted + biased); i += 4 * THREADS) *(Word4*)(table + i) = Word4{};
+    __syncthreads();
+    for_ids<THREADS, LOADS>(a.prompt, row, v0, size, [&](int at) { atomicOr(&table[at], kInPrompt); });
+    for_ids<THREADS, LOADS>(a.tokens, row, v0, size, [&](int at) { atomicAdd(&table[at], 1u); });
+    if (biased)
+      for (int64_t i = tid; i < a.biases; i += THREADS) {
+        const uint64_t at = (uint64_t)((int64_t)a.bias_ids[row * a.bias_ids_stride + i] - v0);
+        if (at < (uint64_t)size) atomicMax(&place[at], (uint32_t)i + 1u);   // the list's last entry for a token
+      }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const int i = (u * THREADS + tid) * VEC;
+    if (i >= size) continue;
     uint32_t word[VEC], entry[VEC], touched = 0;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
@@ -134,39 +188,65 @@ __global__ __launch_bounds__(kAdjustThreads) void k_adjust(AdjustArgs a) {
       entry[k] = biased ? place[i + k] : 0;
       touched |= word[k] | entry[k];
     }
-    const bool all_free = (free & ((1u << VEC) - 1)) == (1u << VEC) - 1;
-    if (a.in_place && all_free && !touched) continue;
-    T l[VEC];
-    const bool whole = i + VEC <= size;
-    if (whole) __builtin_memcpy(l, src + i, 16);
-    else
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) l[k] = i + k < size ? src[i + k] : T(0);
+    const bool all_free = (free[u] & ((1u << VEC) - 1)) == (1u << VEC) - 1, whole = i + VEC <= size;
+    if (a.in_place) {
+      if (all_free && !touched) continue;
+      if (whole) __builtin_memcpy(l[u], src + i, 16);
+    }
     if (touched) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         if (!(word[k] | entry[k])) continue;
-        float v = logit_value<DTYPE>(l[k]);
+        float v = logit_value<DTYPE>(l[u][k]);
         if (word[k]) {
           v = v > 0.f ? v / repetition : v * repetition;
           const uint32_t c = word[k] & ~kInPrompt;
           if (c) v = v - (frequency * (float)c + presence);
         }
         if (entry[k]) v = v + a.bias_values[row * a.bias_values_stride + entry[k] - 1];
-        l[k] = logit_rounded<DTYPE>(v);
+        l[u][k] = logit_rounded<DTYPE>(v);
       }
     }
     if (!all_free) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (!(free >> k & 1)) l[k] = logit_rounded<DTYPE>(-__builtin_inff());
+        if (!(free[u] >> k & 1)) l[u][k] = logit_rounded<DTYPE>(-__builtin_inff());
     }
-    if (whole) __builtin_memcpy(dst + i, l, 16);
+    if (whole) __builtin_memcpy(dst + i, l[u], 16);
     else
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (i + k < size) dst[i + k] = l[k];
+        if (i + k < size) dst[i + k] = l[u][k];
   }
+}
+
+template <int DTYPE, int THREADS, int SLICE, int LOADS>
+static int adjust_launch(AdjustArgs& a, int64_t batch, hipStream_t stream) {
+  const int64_t slices = (a.V + SLICE - 1) / SLICE;
+  if (slices > 0x7fffffff / batch) return m2r_fail("adjust: grid limits exceeded");
+  a.slices = (uint32_t)slices;
+  const size_t lds = 4 * (size_t)SLICE * ((a.prompt.ids || a.tokens.ids) + (a.bias_ids != nullptr));
+  static const hipError_t allowed = hipFuncSetAttribute((const void*)k_adjust<DTYPE, THREADS, SLICE, LOADS>,
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 8 * SLICE);
+  if (int rc = m2r_check(allowed, "adjust shared memory")) return rc;
+  hipLaunchKernelGGL((k_adjust<DTYPE, THREADS, SLICE, LOADS>), dim3((unsigned)(slices * batch)), dim3(THREADS), lds, stream,
+                     a);
+  return m2r_check(hipGetLastError(), "adjust launch");
+}
+template <int DTYPE>
+static int adjust_dtype(AdjustArgs& a, int64_t batch, hipStream_t stream) {
+  // Threads and slice by the lists' length and the number of workgroups.  us, 256 x 1,024 / 512 x 4,096 /
+  // 1,024 x 4,096 / 1,024 x 16,384:
+  //   1 row of 256,000, 1,000 ids     4.4 / 4.4 / 4.9 / 6.5      64 such rows (binary32)     28 / 26 / 45 / 31
+  //   1 row, 50,000 ids                20 / 13 / 9.7 / 12        64 rows, 16,000 ids         98 / 46 / 73 / 45
+  //   16 rows of 256,000, 8,000 ids    19 / 12 / 17 / 12         64 rows, 50,000 ids        289 / 104 / 137 / 67
+  const int64_t ids = a.prompt.n + a.tokens.n;
+  if (ids >= 8192) {
+    if (batch * ((a.V + 16383) / 16384) >= 128) return adjust_launch<DTYPE, 1024, 16384, 4>(a, batch, stream);
+    return adjust_launch<DTYPE, 1024, 4096, 4>(a, batch, stream);
+  }
+  if (ids >= 4096 || batch * ((a.V + 4095) / 4096) >= 256) return adjust_launch<DTYPE, 512, 4096, 2>(a, batch, stream);
+  return adjust_launch<DTYPE, 256, 1024, 2>(a, batch, stream);
 }
 
 }  // namespace m2r
@@ -202,15 +282,8 @@ extern "C" int m2r_adjust_logits(const void* logits, int dtype, int64_t row_stri
                {tokens_n ? tokens : nullptr, tokens_stride, tokens_n, lengths, tokens_are_i64},
                {repetition, repetition_all}, {presence, presence_all}, {frequency, frequency_all},
                biases ? bias_ids : nullptr, bias_values, bias_ids_stride, bias_values_stride, biases,
-               allowed, allowed_stride, masks, allowed_rows, V, 0, 0, logits == out && row_stride == out_stride};
-  a.slice = 4096;
-  const int64_t slices = (V + a.slice - 1) / a.slice;
-  if (slices > 0x7fffffff / batch) return m2r_fail("adjust: grid limits exceeded");
-  a.slices = (uint32_t)slices;
-  const size_t lds = 4 * (size_t)a.slice * ((a.prompt.ids || a.tokens.ids) + (a.bias_ids != nullptr));
-  const dim3 grid((unsigned)(slices * batch)), block(kAdjustThreads);
-  if (dtype == 0) hipLaunchKernelGGL((k_adjust<0>), grid, block, lds, stream, a);
-  else if (dtype == 1) hipLaunchKernelGGL((k_adjust<1>), grid, block, lds, stream, a);
-  else hipLaunchKernelGGL((k_adjust<2>), grid, block, lds, stream, a);
-  return m2r_check(hipGetLastError(), "adjust launch");
+               allowed, allowed_stride, masks, allowed_rows, V, 0, logits == out && row_stride == out_stride};
+  if (dtype == 0) return adjust_dtype<0>(a, batch, stream);
+  if (dtype == 1) return adjust_dtype<1>(a, batch, stream);
+  return adjust_dtype<2>(a, batch, stream);
 }

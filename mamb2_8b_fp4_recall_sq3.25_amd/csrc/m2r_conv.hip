@@ -4,9 +4,12 @@
 // u before a row's first token being its window's last three inputs; the
 // window then holds the row's last four inputs.
 //
-// A thread takes 8 channels (16 bytes of a token's row) and kTokens tokens in
-// a row, so that an input is read once from memory and its three neighbours
-// stay in registers.  Bound by memory: 4 bytes a channel and token.
+// A thread takes 8 channels (16 bytes of a token's row) and up to 32 tokens in
+// a row, eight at a time with the next eight on their way; the three before
+// them stay in registers.  Bound by memory: 4 bytes a channel and token.
+// 10,240 channels: 8,192 tokens of one row 76 us, 4.4 TB/s, where a large copy
+// has 5.0; nine rows of 62 to 901 tokens, padded to 901, 49 us; one token of 64
+// rows 6 us.
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
@@ -37,7 +40,8 @@ __device__ __forceinline__ float silu(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
 
-template <int VEC, int TOKENS>
+// TOKENS: of a thread, STEP of them at a time.
+template <int VEC, int TOKENS, int STEP>
 __global__ __launch_bounds__(256) void k_conv_pool(ConvArgs a) {
   typedef Halves<VEC> V;
   uint32_t w = blockIdx.x;
@@ -52,13 +56,19 @@ __global__ __launch_bounds__(256) void k_conv_pool(ConvArgs a) {
   int part = 0;
   int64_t at = c;
   while (part < 2 && at >= a.n[part]) at -= a.n[part++];
-  uint16_t* out = a.out[part] + (b * a.tokens + t0) * a.n[part] + at;
   const int64_t os = a.n[part];
-
-  float y[TOKENS][VEC] = {};
+  uint16_t* out = a.out[part] + (b * a.tokens + t0) * os + at;
+  const int64_t end = a.tokens - t0 < TOKENS ? a.tokens - t0 : TOKENS;   // of the outputs
+  int64_t done = 0;
   if (t0 < live) {
     const uint16_t* value = a.value + b * a.vs_b + c;
-    V u[TOKENS + 3];
+    const int64_t last = live - 1 - t0;      // of this thread's tokens
+    V u[STEP + 3], next[STEP];
+    auto load = [&](int64_t from) {          // past the end the last token again, not used
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) next[i] = *(const V*)(value + (t0 + (from + i < last ? from + i : last)) * a.vs_l);
+    };
+    load(0);
     if (t0 == 0) {
       // this thread alone reads and writes its channels of the row's window
       uint16_t* window = a.window + slot * a.ws_s + c;
@@ -66,52 +76,56 @@ __global__ __launch_bounds__(256) void k_conv_pool(ConvArgs a) {
       for (int j = 0; j < 3; ++j) u[j] = *(const V*)(window + (j + 1) * a.ws_t);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t s = live - 4 + j;   // -1 ... -3: the window's last three
-        V last = *(const V*)(value + (s > 0 ? s : 0) * a.vs_l);
-        if (s == -1) last = u[2];
-        if (s == -2) last = u[1];
-        if (s == -3) last = u[0];
-        *(V*)(window + j * a.ws_t) = last;
+        const int64_t s = live - 4 + j;      // -1 ... -3: the window's last three
+        V v = *(const V*)(value + (s > 0 ? s : 0) * a.vs_l);
+        if (s == -1) v = u[2];
+        if (s == -2) v = u[1];
+        if (s == -3) v = u[0];
+        *(V*)(window + j * a.ws_t) = v;
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 3; ++j) u[j] = *(const V*)(value + (t0 - 3 + j) * a.vs_l);
     }
-#pragma unroll
-    for (int i = 0; i < TOKENS; ++i) {   // past the end the last row's token again, not stored
-      const int64_t t = t0 + i < live ? t0 + i : live - 1;
-      u[3 + i] = *(const V*)(value + t * a.vs_l);
-    }
+    Halves<4> wk[VEC];
+    float bk[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const Halves<4> wk = *(const Halves<4>*)(a.weight + 4 * (c + k));
-      const float bk = a.bias ? h2f(a.bias[c + k]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < TOKENS; ++i) {
-        float s = bk;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s = __builtin_fmaf(h2f(wk.v[j]), h2f(u[i + j].v[k]), s);
-        y[i][k] = a.silu ? silu(s) : s;
-      }
+      wk[k] = *(const Halves<4>*)(a.weight + 4 * (c + k));
+      bk[k] = a.bias ? h2f(a.bias[c + k]) : 0.f;
     }
-  }
+    const int64_t mine = last + 1 < end ? last + 1 : end;
+    for (; done < mine; done += STEP) {
 #pragma unroll
-  for (int i = 0; i < TOKENS; ++i) {
-    if (t0 + i >= a.tokens) break;
-    V o;
+      for (int i = 0; i < STEP; ++i) u[3 + i] = next[i];
+      if (TOKENS > STEP && done + STEP < mine) load(done + STEP);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) o.v[k] = t0 + i < live ? f2h(y[i][k]) : 0;
-    *(V*)(out + i * os) = o;
+      for (int i = 0; i < STEP; ++i) {
+        V o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          float s = bk[k];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s = __builtin_fmaf(h2f(wk[k].v[j]), h2f(u[i + j].v[k]), s);
+          o.v[k] = f2h(a.silu ? silu(s) : s);
+        }
+        if (done + i < mine) *(V*)(out + (done + i) * os) = o;
+      }
+#pragma unroll
+      for (int j = 0; j < 3; ++j) u[j] = u[STEP + j];
+    }
+    done = mine;
   }
+  for (; done < end; ++done) *(V*)(out + done * os) = V{};
 }
 
-template <int VEC, int TOKENS>
+template <int VEC, int TOKENS, int STEP>
 static int conv_launch(ConvArgs& a, hipStream_t stream) {
   const int64_t cb = (a.C + 256 * VEC - 1) / (256 * VEC), tb = (a.tokens + TOKENS - 1) / TOKENS;
   if (cb * tb > 0x7fffffff / a.batch) return m2r_fail("conv pool: grid limits exceeded");
   a.channel_blocks = (uint32_t)cb;
   a.token_blocks = (uint32_t)tb;
-  hipLaunchKernelGGL((k_conv_pool<VEC, TOKENS>), dim3((unsigned)(cb * tb * a.batch)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((k_conv_pool<VEC, TOKENS, STEP>), dim3((unsigned)(cb * tb * a.batch)), dim3(256), 0, stream, a);
   return m2r_check(hipGetLastError(), "conv pool launch");
 }
 
@@ -140,6 +154,11 @@ extern "C" int m2r_conv_pool(void* window, int64_t pool, int64_t ws_s, int64_t w
              batch, tokens, 0, 0, silu};
   const uint64_t bases = (uintptr_t)window | (uintptr_t)value | (uintptr_t)x | (uintptr_t)bm | (uintptr_t)cm;
   const bool wide = !(bases & 15) && !((ws_s | ws_t | vs_b | vs_l | n_x | n_b | n_c) & 7);
-  if (tokens == 1) return wide ? conv_launch<8, 1>(a, stream) : conv_launch<1, 1>(a, stream);
-  return wide ? conv_launch<8, 8>(a, stream) : conv_launch<1, 8>(a, stream);
+  if (tokens == 1) return wide ? conv_launch<8, 1, 1>(a, stream) : conv_launch<1, 1, 1>(a, stream);
+  if (!wide) return conv_launch<1, 8, 8>(a, stream);
+  // 32 tokens a thread once that leaves a workgroup a CU.  us with 8 a thread (11 loads for 8 outputs) / 32, 10,240
+  // channels: 8,192 tokens of one row 100 / 76, 1,000 of three 40 / 30, 128 of 16 28 / 24, 200 of four 14 / 16, 500 of
+  // one 12 / 15, 77 of one 6 / 13
+  const int64_t blocks = (C + 2047) / 2048 * batch * ((tokens + 31) / 32);
+  return blocks >= 256 ? conv_launch<8, 32, 8>(a, stream) : conv_launch<8, 8, 8>(a, stream);
 }
