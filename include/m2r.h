@@ -455,14 +455,15 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   row 2 a + t, and byte 256 c + 16 r + i of a tile is row r, input 16 c + i.
  * m2r_int8_linear: x rows of K (x_dtype as above, element row stride), y rows of N
  *   (y_dtype 2 binary32, too; element row stride of at most 2^25); K at most
- *   131,072; workspace: 16-byte aligned device memory of
- *   m2r_int8_linear_workspace() bytes, used on `stream` only.  Scales whose product
+ *   131,072; workspace: 16-byte aligned device memory of the bytes that
+ *   m2r_int8_linear_workspace() names for this call (x is not read; null where that
+ *   is 0), used on `stream` only.  Scales whose product
  *   is below binary32's normal numbers cost digits.
  */
 int64_t m2r_int8_weight_bytes(int64_t N, int64_t K);
 int m2r_int8_quantize(const void* w, int dtype, int64_t w_stride, void* tiles, float* scale, int64_t N, int64_t K,
                       hipStream_t stream);
-int64_t m2r_int8_linear_workspace(int64_t M, int64_t N, int64_t K);
+int64_t m2r_int8_linear_workspace(const void* x, int64_t x_stride, int64_t M, int64_t N, int64_t K);
 int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, const void* w_tiles, const float* w_scale, void* y,
                     int y_dtype, int64_t y_stride, int64_t M, int64_t N, int64_t K, void* workspace,
                     int64_t workspace_bytes, hipStream_t stream);

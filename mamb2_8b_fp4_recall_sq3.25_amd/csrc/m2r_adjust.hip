@@ -226,9 +226,8 @@ static int adjust_launch(AdjustArgs& a, int64_t batch, hipStream_t stream) {
   if (slices > 0x7fffffff / batch) return m2r_fail("adjust: grid limits exceeded");
   a.slices = (uint32_t)slices;
   const size_t lds = 4 * (size_t)SLICE * ((a.prompt.ids || a.tokens.ids) + (a.bias_ids != nullptr));
-  static const hipError_t allowed = hipFuncSetAttribute((const void*)k_adjust<DTYPE, THREADS, SLICE, LOADS>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 8 * SLICE);
-  if (int rc = m2r_check(allowed, "adjust shared memory")) return rc;
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = m2r_allow_lds((const void*)k_adjust<DTYPE, THREADS, SLICE, LOADS>, 8 * SLICE, allowed)) return rc;
   hipLaunchKernelGGL((k_adjust<DTYPE, THREADS, SLICE, LOADS>), dim3((unsigned)(slices * batch)), dim3(THREADS), lds, stream,
                      a);
   return m2r_check(hipGetLastError(), "adjust launch");

@@ -59,7 +59,7 @@ _SIGNATURES = {
                           + [P, I64, I64, P] + [I64] * 2 + [P], I),
     "m2r_int8_weight_bytes": ([I64] * 2, I64),
     "m2r_int8_quantize": ([P, I, I64, P, P, I64, I64, P], I),
-    "m2r_int8_linear_workspace": ([I64] * 3, I64),
+    "m2r_int8_linear_workspace": ([P] + [I64] * 4, I64),
     "m2r_int8_linear": ([P, I, I64, P, P, P, I, I64] + [I64] * 3 + [P, I64, P], I),
     "m2r_conv_pool": ([P, I64, I64, I64, P, I64, I64] + [P] * 7 + [I64] * 5 + [I, I, P], I),
     "m2r_state_step_ridge_layers_workspace": ([I], I64),

@@ -111,13 +111,13 @@ def linear(x, weight, dtype=None):
         raise ValueError("dtype must be FP16, BF16 or FP32")
     rows, stride = _rows(x if x.ndim == 2 else x.reshape(-1, k), k)
     m = rows.shape[0]
-    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=x.device)
     if m == 0:
         return y
-    ws_bytes = int(_native.lib().m2r_int8_linear_workspace(m, n, k))
-    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-    p = _native.ptr
+    at, p = rows.data_ptr(), _native.ptr
+    ws_bytes = _native.lib().m2r_int8_linear_workspace(at, stride, m, n, k)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     with _native.device_of(x):
-        _native.call("m2r_int8_linear", p(rows), _TYPES[x.dtype], stride, p(weight.tiles), p(weight.scale), p(y),
+        _native.call("m2r_int8_linear", at, _TYPES[x.dtype], stride, p(weight.tiles), p(weight.scale), p(y),
                      _TYPES[dtype], n, m, n, k, p(ws), ws_bytes, _native.stream_of(x))
     return y

@@ -16,9 +16,9 @@ def _filter(value, name, dtype, like, low, high):
     """(tensor or None, scalar) of one filter: a number for every row, or a
     tensor with a value for each."""
     if isinstance(value, torch.Tensor):
-        if value.dtype != dtype or tuple(value.shape) != (like.shape[0],) or value.device != like.device:
+        if value.dtype is not dtype or value.shape != (like.shape[0],) or value.device != like.device:
             raise ValueError(f"{name} must be a number or {str(dtype).split('.')[1]}[batch] on the logits' device")
-        return value.contiguous(), 0
+        return value if value.shape[0] < 2 or value.stride(0) == 1 else value.contiguous(), 0
     if isinstance(value, bool) or not isinstance(value, (int, float) if dtype == torch.float32 else int) \
             or not low <= value <= high:
         raise ValueError(f"{name} must lie in [{low}, {high}]")
@@ -42,21 +42,28 @@ def penalties(like, repetition, presence, frequency):
             _filter(frequency, "frequency", torch.float32, like, -1e30, 1e30))
 
 
-def _list(ids, lengths, name, like):
+# An eager call on small tensors is bound by the host: the checks below ask a
+# tensor for its type, shape and device number once each.
+def _list(ids, lengths, name, batch, device):
     """A list of ids a row as the C entry takes it: (ids, is int64, row stride, ids a row, lengths)."""
     if ids is None:
         if lengths is not None:
             raise ValueError(f"{name}: lengths without ids")
         return None, 0, 0, 0, None
-    if (not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32) or ids.ndim != 2
-            or ids.shape[0] != like.shape[0] or ids.device != like.device):
+    if (not isinstance(ids, torch.Tensor) or ids.dtype is not torch.int64 and ids.dtype is not torch.int32
+            or ids.ndim != 2 or ids.shape[0] != batch or ids.get_device() != device):
         raise ValueError(f"{name} must be int64 or int32 [batch,ids] on the logits' device")
-    if lengths is not None and (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
-                                or tuple(lengths.shape) != (like.shape[0],) or lengths.device != like.device):
-        raise ValueError(f"The lengths of {name} must be int32[batch] on the logits' device")
-    if ids.shape[1] > 1 and ids.stride(1) != 1:
-        ids = ids.contiguous()
-    return ids, ids.dtype is torch.int64, ids.stride(0), ids.shape[1], None if lengths is None else lengths.contiguous()
+    if lengths is not None:
+        if (not isinstance(lengths, torch.Tensor) or lengths.dtype is not torch.int32 or lengths.shape != (batch,)
+                or lengths.get_device() != device):
+            raise ValueError(f"The lengths of {name} must be int32[batch] on the logits' device")
+        if batch > 1 and lengths.stride(0) != 1:
+            lengths = lengths.contiguous()
+    stride, unit = ids.stride()
+    count = ids.shape[1]
+    if count > 1 and unit != 1:
+        ids, stride = ids.contiguous(), count
+    return ids, ids.dtype is torch.int64, stride, count, lengths
 
 
 def biases(like, bias):
@@ -67,14 +74,17 @@ def biases(like, bias):
     if not isinstance(bias, (tuple, list)) or len(bias) != 2 or not all(isinstance(t, torch.Tensor) for t in bias):
         raise ValueError("bias must be a pair of tensors, ids and values")
     ids, values = bias
-    batch = like.shape[0]
-    if (ids.dtype != torch.int32 or values.dtype != torch.float32 or ids.shape != values.shape
-            or ids.ndim not in (1, 2) or ids.ndim == 2 and ids.shape[0] != batch
-            or ids.device != like.device or values.device != like.device):
+    batch, shape = like.shape[0], ids.shape
+    if (ids.dtype is not torch.int32 or values.dtype is not torch.float32 or shape != values.shape
+            or len(shape) not in (1, 2) or len(shape) == 2 and shape[0] != batch
+            or not like.get_device() == ids.get_device() == values.get_device()):
         raise ValueError("bias must be int32 ids and FP32 values, both [n] or [batch,n], on the logits' device")
-    if ids.ndim == 1:
+    if len(shape) == 1:
         ids, values = ids.expand(batch, -1), values.expand(batch, -1)
-    return tuple(t if t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous() for t in (ids, values))
+    if shape[-1] > 1:
+        ids = ids if ids.stride(1) == 1 else ids.contiguous()
+        values = values if values.stride(1) == 1 else values.contiguous()
+    return ids, values
 
 
 def masks(like, vocab, allowed, allowed_rows):
@@ -85,8 +95,8 @@ def masks(like, vocab, allowed, allowed_rows):
             raise ValueError("allowed_rows without allowed")
         return None, None
     words, batch = (vocab + 31) // 32, like.shape[0]
-    if (not isinstance(allowed, torch.Tensor) or allowed.dtype != torch.int32 or allowed.ndim not in (1, 2)
-            or allowed.shape[-1] != words or allowed.shape[0] < 1 or allowed.device != like.device):
+    if (not isinstance(allowed, torch.Tensor) or allowed.dtype is not torch.int32 or allowed.ndim not in (1, 2)
+            or allowed.shape[-1] != words or allowed.shape[0] < 1 or allowed.get_device() != like.get_device()):
         raise ValueError(f"allowed must be int32 [{words}] or [masks,{words}], a bit a token, on the logits' device")
     if allowed.ndim == 1:
         if allowed_rows is not None:
@@ -95,12 +105,14 @@ def masks(like, vocab, allowed, allowed_rows):
     elif allowed_rows is None:
         if allowed.shape[0] != batch:
             raise ValueError("A mask for each row, or allowed_rows, required")
-    elif (not isinstance(allowed_rows, torch.Tensor) or allowed_rows.dtype != torch.int32
-          or tuple(allowed_rows.shape) != (batch,) or allowed_rows.device != like.device):
+    elif (not isinstance(allowed_rows, torch.Tensor) or allowed_rows.dtype is not torch.int32
+          or allowed_rows.shape != (batch,) or allowed_rows.get_device() != like.get_device()):
         raise ValueError("allowed_rows must be int32[batch] on the logits' device")
+    elif batch > 1 and allowed_rows.stride(0) != 1:
+        allowed_rows = allowed_rows.contiguous()
     if words > 1 and allowed.stride(1) != 1:
         allowed = allowed.contiguous()
-    return allowed, None if allowed_rows is None else allowed_rows.contiguous()
+    return allowed, allowed_rows
 
 
 def _span(t):
@@ -140,8 +152,9 @@ def adjust(logits, *, prompt=None, prompt_lengths=None, tokens=None, lengths=Non
     if vocab < 1:
         raise ValueError("A vocabulary of at least one token required")
     (r, r_all), (pr, pr_all), (f, f_all) = penalties(logits, repetition, presence, frequency)
-    prompt, p64, ps, pn, prompt_lengths = _list(prompt, prompt_lengths, "prompt", logits)
-    tokens, t64, ts, tn, lengths = _list(tokens, lengths, "tokens", logits)
+    device = logits.get_device()
+    prompt, p64, ps, pn, prompt_lengths = _list(prompt, prompt_lengths, "prompt", batch, device)
+    tokens, t64, ts, tn, lengths = _list(tokens, lengths, "tokens", batch, device)
     ids, values = biases(logits, bias)
     allowed, allowed_rows = masks(logits, vocab, allowed, allowed_rows)
     source = logits
