@@ -80,13 +80,9 @@ __device__ __forceinline__ Chunk load_chunk(const RowArgs& a, const uint16_t* x,
   Chunk v;
   const int last = (int)(a.K >> 4);
   if constexpr (WHOLE) {
-    const uint16_t* p = x + 16 * (int64_t)(c < last ? c : last - 1);
-    v.h[0] = *(const u16x8*)p;
-    v.h[1] = *(const u16x8*)(p + 8);
-    const uint32_t keep = c < last ? ~0u : 0u;
-    u32x4 *w = (u32x4*)&v;
-    w[0] &= keep;
-    w[1] &= keep;
+    const auto row = __builtin_amdgcn_make_buffer_rsrc((void*)x, 0, (int)(2 * a.K), 0x00027000);   // zeros past its end
+    v.h[0] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(row, 32 * c, 0, 0));
+    v.h[1] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(row, 32 * c + 16, 0, 0));
   } else if (c < last) {
     __builtin_memcpy(&v, x + 16 * (int64_t)c, 32);
   } else {
