@@ -6,14 +6,17 @@ attention with a decay for each head, as the Mamba-2 mixer runs it
 rounds to FP16 after every token).  The carries of many requests live in one
 pool, FP32[slots,H,P,128]; a call names the slot and the token count of each
 batch row, so prompts of different lengths and idle rows share a launch.
-The scan runs the gfx950 HIP kernels of libm2r_hip.so (m2r_full_scan).
+convolve is the mixer's convolution before it, over a pool of windows in the
+same manner.  They run the gfx950 HIP kernels of libm2r_hip.so (m2r_full_scan,
+m2r_conv_pool).
 """
 from __future__ import annotations
 
 import torch
+from torch import nn
 
 from . import _native
-from .state_quant import _MixerController
+from .state_quant import _MixerController, _plain
 
 N = 128
 
@@ -190,7 +193,10 @@ def convolve(value, weight, bias, window, sizes, *, lengths=None, slots=None, si
 
 class FullState(_MixerController):
     """Controller with the full-precision carry: prompts in one scan call a
-    layer, decode one token at a time, no table and no quantization."""
+    layer, of different lengths if backbone() is given them, decode one token
+    at a time, no table and no quantization."""
+
+    ragged = True
 
     def __init__(self, model):
         super().__init__(model, "full", None, False)
@@ -202,7 +208,15 @@ class FullState(_MixerController):
         return allocate_state(batch_size, self.HEADS, self.HEADDIM, self.D_STATE, self.device)
 
     def _scan_layer(self, index, mx, x, dt, aa, bm, cm, entry):
-        return scan(x, dt, aa, bm, cm, mx.D, mx.dt_bias, entry.state)
+        return scan(x, dt, aa, bm, cm, mx.D, mx.dt_bias, entry.state, lengths=self._lengths)
+
+    def _conv_prefill(self, mx, xbc, layer):
+        if self._lengths is None:
+            return super()._conv_prefill(mx, xbc, layer)
+        if not (_plain(mx.conv1d, nn.Conv1d) and _plain(mx.act, nn.SiLU)):
+            raise ValueError("Rows of different lengths need a plain nn.Conv1d and nn.SiLU, without hooks")
+        return convolve(xbc, mx.conv1d.weight[:, 0, :], mx.conv1d.bias, layer.conv, self._conv_sizes,
+                        lengths=self._lengths)
 
     def assert_finite_cache(self):
         """True when every window and carry is finite, else FloatingPointError."""

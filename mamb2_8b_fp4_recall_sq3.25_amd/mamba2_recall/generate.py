@@ -12,7 +12,10 @@ matrix rate, and controller.use_adapters gives every request its own adapter:
         new, logprobs = generate.generate(controller, lm_head, prompt, uniforms,
                                           temperature=0.8, top_k=50, top_p=0.95)
 
-All prompts of a call have the same length.
+A queue of prompts of different lengths is padded on the right and goes in one
+call through full_state.FullState; its projections and the head may be in 8-bit
+integers (int8), and each request may have penalties, biases and a grammar of
+its own.
 """
 from __future__ import annotations
 
@@ -22,27 +25,56 @@ from . import sampling
 
 
 @torch.no_grad()
-def generate(controller, lm_head, prompt, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def generate(controller, lm_head, prompt, uniforms, *, lengths=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+             repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
     """Continue `prompt` int64[batch,tokens] by as many tokens as `uniforms`
     FP32[batch,new] has columns; returns (ids int64[batch,new], log
-    probabilities FP32[batch,new]).  The filters are sampling.sample's: numbers,
-    or a value for each request.  The controller's request is reset first and
-    stands after the last token but one."""
+    probabilities FP32[batch,new]).  The filters are sampling.sample's, the
+    penalties, bias and masks sampling.adjust's: numbers, or a value for each
+    request.  `allowed` is the masks for all steps, or a function of the ids
+    drawn so far, int64[batch,step], that gives the next step's, or None.
+    `lengths` int32[batch] (a controller that takes it): the tokens of each
+    prompt, at least one; those behind them count for nothing.  The
+    controller's request is reset first and stands after the last token but
+    one."""
     if (not isinstance(uniforms, torch.Tensor) or uniforms.ndim != 2 or uniforms.dtype != torch.float32
             or uniforms.shape[1] < 1):
         raise ValueError("uniforms must be FP32[batch,new] with at least one new token")
     if not isinstance(prompt, torch.Tensor) or prompt.ndim != 2 or prompt.shape[0] != uniforms.shape[0]:
         raise ValueError("prompt must be [batch,tokens] with a row for each row of uniforms")
-    sampling.filters(uniforms, temperature, top_k, top_p, min_p)   # refused before the request is reset
-    hidden = controller.backbone(prompt, reset=True)
+    # refused before the request is reset
+    sampling.filters(uniforms, temperature, top_k, top_p, min_p)
+    sampling.penalties(uniforms, repetition, presence, frequency)
+    sampling.biases(uniforms, bias)
+    batch, new = uniforms.shape
+    if lengths is not None and (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
+                                or tuple(lengths.shape) != (batch,) or lengths.device != uniforms.device):
+        raise ValueError("lengths must be int32[batch] on the device of uniforms")
+    if allowed is not None and not callable(allowed) and not isinstance(allowed, torch.Tensor):
+        raise ValueError("allowed must be a tensor of masks or a function that gives them")
+    counted = any(isinstance(v, torch.Tensor) or v != d for v, d in ((repetition, 1), (presence, 0), (frequency, 0)))
+    if lengths is None:
+        last = controller.backbone(prompt, reset=True)[:, -1]
+    else:
+        hidden = controller.backbone(prompt, reset=True, lengths=lengths)
+        at = lengths.long().clamp(1, prompt.shape[1]) - 1
+        last = hidden[torch.arange(batch, device=hidden.device), at]
     columns = uniforms.t().contiguous()
-    ids, logprobs = [], []
-    for step in range(columns.shape[0]):
+    ids, logprobs = torch.empty((batch, new), dtype=torch.int64, device=uniforms.device), []
+    for step in range(new):
+        drawn = ids[:, :step]
         if step:
             # a row whose logits hold nothing to draw (-1) goes on with token 0
-            hidden = controller.backbone(ids[-1].clamp(min=0)[:, None])
-        token, logprob = sampling.sample(lm_head(hidden[:, -1]), columns[step], temperature=temperature, top_k=top_k,
-                                         top_p=top_p, min_p=min_p)
-        ids.append(token)
+            last = controller.backbone(drawn[:, -1:].clamp(min=0))[:, -1]
+        logits = lm_head(last)
+        masks = allowed(drawn) if callable(allowed) else allowed
+        if counted or bias is not None or masks is not None:
+            logits = sampling.adjust(logits, prompt=prompt if counted else None,
+                                     prompt_lengths=lengths if counted else None,
+                                     tokens=drawn if counted and step else None, repetition=repetition,
+                                     presence=presence, frequency=frequency, bias=bias, allowed=masks)
+        token, logprob = sampling.sample(logits, columns[step], temperature=temperature, top_k=top_k, top_p=top_p,
+                                         min_p=min_p)
+        ids[:, step] = token
         logprobs.append(logprob)
-    return torch.stack(ids, 1), torch.stack(logprobs, 1)
+    return ids, torch.stack(logprobs, 1)

@@ -9,8 +9,20 @@ value, and multiplies the whole numbers:
 
 The reference keeps decoded FP16 weights for all its projections
 (mamba2_recall/fp4_checkpoint.py:345-405); this is for prompts and batches,
-where fp4.gemv_g16 ends.  Runs the gfx950 HIP kernels of libm2r_hip.so
-(m2r_int8_quantize, m2r_int8_linear)."""
+where fp4.gemv_g16 ends.  A queue of prompts of different lengths, projections
+and head in 8-bit integers, with penalties, biases and a grammar for each:
+
+    weights = [{name: int8.Int8Weight.quantize(getattr(layer.mixer, name).weight) for name in ("in_proj", "out_proj")}
+               for layer in model.backbone.layers]
+    head = int8.Int8Weight.quantize(model.lm_head.weight)
+    with full_state.FullState(model) as controller:
+        controller.use_int8_projections(weights)
+        new, logprobs = generate.generate(controller, lambda rows: head(rows, torch.float32), prompt, uniforms,
+                                          lengths=lengths, temperature=0.8, top_p=0.95, repetition=1.1, frequency=0.2,
+                                          bias=(bias_ids, bias_values), allowed=lambda drawn: masks)
+
+Runs the gfx950 HIP kernels of libm2r_hip.so (m2r_int8_quantize,
+m2r_int8_linear)."""
 from __future__ import annotations
 
 import torch

@@ -26,7 +26,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _native, adapters, fp4, state_codec
+from . import _native, adapters, fp4, int8, state_codec
 
 # Installed controllers, keyed by the identity of the model each owns.  Values
 # are held weakly; the installed per-layer hooks keep a controller alive until
@@ -250,6 +250,8 @@ class _MixerController:
     # another order, so outputs can differ from it in the last bit of some
     # channels (that kernel's arithmetic is not available here to pin).
     native_norm = True
+    # whether backbone() takes prompts of different lengths
+    ragged = False
     PARAMETER_TENSORS, PARAMETER_COUNT = 507, 8_236_999_680
     TABLE_SHAPE = (56, 8, 128)
 
@@ -274,6 +276,8 @@ class _MixerController:
         self._running = False     # inside backbone()
         self._rates = {}
         self._packed = None
+        self._int8 = None         # a dict of Int8Weight or None for each layer
+        self._lengths = None      # of the rows of the call in flight, int32[batch]
         self._adapters = None     # (a dict of AdapterSet or None for each layer, ids int32[batch])
         self._stat_sums = {}      # layer index -> FP64 [groups, 128] totals
         self._stat_counts = [0] * len(self._mixers)
@@ -425,9 +429,12 @@ class _MixerController:
         pass
 
     @torch.no_grad()
-    def backbone(self, ids, reset=False):
+    def backbone(self, ids, reset=False, lengths=None):
         """model.backbone(ids) with every mixer going through this controller
-        (state_quant.py:195-217): the request's caches are used and advanced."""
+        (state_quant.py:195-217): the request's caches are used and advanced.
+        `lengths` int32[batch] (full_state.FullState): the tokens of each row
+        that count; a row's caches stand after its last, and the hidden rows
+        past it say nothing."""
         if not self._installed:
             raise RuntimeError("StateQuant controller is not installed")
         if not isinstance(ids, torch.Tensor) or ids.ndim != 2 or ids.shape[1] == 0:
@@ -438,9 +445,15 @@ class _MixerController:
             raise RuntimeError("Concurrent/reentrant backbone invocation is unsupported")
         if self._adapters is not None and self._adapters[1].shape[0] != ids.shape[0]:
             raise ValueError("Adapter ids and batch differ")
+        if lengths is not None:
+            if not self.ragged:
+                raise ValueError("This controller takes rows of one length")
+            if (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
+                    or tuple(lengths.shape) != (ids.shape[0],) or lengths.device != self.device):
+                raise ValueError("lengths must be int32[batch] on the model device")
         if reset or self._request is None:
             self.reset(ids.shape[0])
-        self._running = True
+        self._running, self._lengths = True, lengths
         try:
             hidden = self.model.backbone(ids)
             if self._request.next_layer != 0:
@@ -450,7 +463,7 @@ class _MixerController:
                 self._request.failed = True
             raise
         finally:
-            self._running = False
+            self._running, self._lengths = False, None
         return hidden
 
     # ---------------------------------------------------------------- one layer
@@ -501,11 +514,11 @@ class _MixerController:
         batch, tokens = u.shape[0], u.shape[1]
         # a one-token continuation runs the projections and the norm on rank-2
         # inputs (the shapes the native step uses, and the ones norm hooks see)
-        step = layer.tokens > 0 and tokens == 1
+        step = layer.tokens > 0 and tokens == 1 and self._lengths is None
         if step:
-            zxbcdt = self._project(index, "in_proj", mx, u[:, 0])[:, None]
+            zxbcdt = self._project(index, "in_proj", mx, u[:, 0], step)[:, None]
         else:
-            zxbcdt = mx.in_proj(u)
+            zxbcdt = self._project(index, "in_proj", mx, u, step)
         zxbcdt = self._adapt(index, "in_proj", zxbcdt, u)
         z, xbc, dt = torch.split(zxbcdt, self._in_sizes, dim=-1)
         if step:
@@ -525,11 +538,11 @@ class _MixerController:
         y = y.reshape(batch, tokens, self.D_INNER)
         if step:
             v = mx.norm(y[:, 0], z[:, 0])
-            out = self._project(index, "out_proj", mx, v)[:, None]
+            out = self._project(index, "out_proj", mx, v, step)[:, None]
             v = v[:, None]
         else:
             v = mx.norm(y, z)
-            out = mx.out_proj(v)
+            out = self._project(index, "out_proj", mx, v, step)
         out = self._adapt(index, "out_proj", out, v)
         layer.tokens += tokens
         return out
@@ -577,12 +590,39 @@ class _MixerController:
         self._packed = checked
         return self
 
-    def _project(self, index, name, mx, value):
-        """One-token projection: the packed GEMV when registered and the batch
-        size is supported, else the module."""
-        entry = self._packed[index] if self._packed is not None else None
+    def use_int8_projections(self, weights):
+        """Run the in_proj and out_proj of every layer in 8-bit integers
+        (int8.linear), prompts and single tokens, any batch.  `weights[i]` is a
+        dict of int8.Int8Weight under in_proj and out_proj (either may be
+        missing) for layer i, or None to keep that layer on its modules;
+        `weights=None` turns the mode off.  Where packed projections are
+        registered as well, they keep the one-token calls that they take."""
+        if weights is None:
+            self._int8 = None
+            return self
+        if len(weights) != len(self._mixers):
+            raise ValueError("One entry of 8-bit weights per layer required")
+        for mx, entry in zip(self._mixers, weights):
+            for name, item in (entry or {}).items():
+                if name not in ("in_proj", "out_proj") or not isinstance(item, int8.Int8Weight):
+                    raise ValueError("8-bit entries are Int8Weights under in_proj and out_proj")
+                module = getattr(mx, name)
+                if (module.bias is not None or item.features != tuple(reversed(module.weight.shape))
+                        or item.tiles.device != self.device):
+                    raise ValueError(f"8-bit weights of {name} do not match the layer's projection")
+        self._int8 = list(weights) if any(weights) else None
+        return self
+
+    def _project(self, index, name, mx, value, step):
+        """A projection: for one token the packed GEMV when registered and the
+        batch size is supported; the 8-bit product when registered, else the
+        module."""
+        entry = self._packed[index] if step and self._packed is not None else None
         if entry is not None and fp4.gemv_supported(value.shape[0], value.shape[1]):
             return fp4.gemv_g16(*entry[name], value)
+        weight = (self._int8[index] or {}).get(name) if self._int8 is not None else None
+        if weight is not None:
+            return int8.linear(value, weight)
         return getattr(mx, name)(value)
 
     def use_adapters(self, sets, ids=None):
