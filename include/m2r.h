@@ -454,8 +454,8 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   N may hold anything).  Channel 32 a + 8 g + 4 t + r lies in row 4 g + r of tile
  *   row 2 a + t, and byte 256 c + 16 r + i of a tile is row r, input 16 c + i.
  * m2r_int8_linear: x rows of K (x_dtype as above, element row stride), y rows of N
- *   (y_dtype 2 binary32, too; element row stride of at most 2^25); K at most
- *   131,072; workspace: 16-byte aligned device memory of the bytes that
+ *   (y_dtype 2 binary32, too; element row stride of at most 2^25; no memory of an
+ *   operand); K at most 131,072; workspace: 16-byte aligned device memory of the bytes that
  *   m2r_int8_linear_workspace() names for this call (x is not read; null where that
  *   is 0), used on `stream` only.  Scales whose product
  *   is below binary32's normal numbers cost digits.

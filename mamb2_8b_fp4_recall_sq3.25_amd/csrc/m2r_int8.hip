@@ -199,7 +199,6 @@ struct ProductArgs {
   uint64_t* parts;               // its splits' sums
   uint32_t row_blocks, channel_blocks;   // of large tiles
   uint32_t whole;                // workgroups with a large tile; the others have parts of one
-  int32_t wide;                  // whole eights of channels of y, dword-aligned: stores of 16 bytes
 };
 
 // Eight sums of a row and eight channels, scaled and stored.  The scales'
@@ -856,6 +855,7 @@ extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, con
     return m2r_fail("int8: workspace too small or not 16-byte aligned");
   const int64_t MT = row_tiles(M), NT = channel_tiles(N);
   if ((MT + kBig - 1) / kBig * ((NT + kBig - 1) / kBig) > 0x7fffffff / 64) return m2r_fail("int8: grid limits exceeded");
+  // wide: whole eights of channels, dword-aligned, stored by 16 bytes
   const bool whole = whole_rows(x, x_stride, K), wide = !(N & 7) && !(y_stride & 1) && !((uintptr_t)y & 3);
   const Plan p = int8_plan(M, N, K, whole);
   uint8_t* codes = (uint8_t*)workspace;
@@ -866,7 +866,7 @@ extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, con
   if (!p.fused)
     if (int rc = int8_rows(r, x_dtype, stream)) return rc;
   const ProductArgs a{codes, (const uint8_t*)w_tiles, scale, w_scale, y, y_stride, M, N, (int32_t)MT, (int32_t)NT,
-                      (int32_t)(padded_inputs(K) / 64), p.splits, tickets, parts, p.rb, p.cb, p.whole, (int32_t)wide};
+                      (int32_t)(padded_inputs(K) / 64), p.splits, tickets, parts, p.rb, p.cb, p.whole};
   if (y_dtype == 0)
     return wide ? int8_product<0, true>(p, a, r, x_dtype, stream) : int8_product<0, false>(p, a, r, x_dtype, stream);
   if (y_dtype == 1)

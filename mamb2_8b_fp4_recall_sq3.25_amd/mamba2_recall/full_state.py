@@ -152,43 +152,48 @@ def convolve(value, weight, bias, window, sizes, *, lengths=None, slots=None, si
     if not isinstance(value, torch.Tensor) or value.dtype != torch.float16 or value.ndim != 3 or not value.is_cuda:
         raise ValueError("value must be CUDA FP16[batch,tokens,channels]")
     batch, tokens, channels = value.shape
-    if min(batch, tokens, channels) < 1:
+    if batch < 1 or tokens < 1 or channels < 1:
         raise ValueError("Positive geometry required")
     if not isinstance(sizes, (tuple, list)) or len(sizes) != 3 \
             or not all(isinstance(n, int) and n > 0 for n in sizes) or sum(sizes) != channels:
         raise ValueError("sizes must be three positive channel counts that add up to value's")
-    for t, shape, name in ((weight, (channels, 4), "weight"), (bias, (channels,), "bias")):
-        if t is None and name == "bias":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape \
-                or t.device != value.device:
-            raise ValueError(f"{name} must be FP16{list(shape)} on the device of value")
-    if (not isinstance(window, torch.Tensor) or window.dtype != torch.float16 or window.ndim != 3
-            or tuple(window.shape[1:]) != (channels, 4) or window.shape[0] < 1 or window.device != value.device
-            or channels > 1 and window.stride(1) != 1 or window.stride(2) < channels
-            or window.shape[0] > 1 and window.stride(0) < 3 * window.stride(2) + channels):
-        raise ValueError("window must be FP16[slots,channels,4] with channels next to each other (allocate_windows)")
-    if slots is None and window.shape[0] < batch:
+    # (a call of one token is bound by the host: each tensor is asked once)
+    f16, device, rows = torch.float16, value.get_device(), (batch,)
+    if not isinstance(weight, torch.Tensor) or weight.dtype is not f16 or weight.shape != (channels, 4) \
+            or weight.get_device() != device:
+        raise ValueError(f"weight must be FP16[{channels}, 4] on the device of value")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype is not f16 or bias.shape != (channels,)
+                             or bias.get_device() != device):
+        raise ValueError(f"bias must be FP16[{channels}] on the device of value")
+    if (not isinstance(window, torch.Tensor) or window.dtype is not f16 or window.ndim != 3
+            or window.shape[1:] != (channels, 4) or window.shape[0] < 1 or window.get_device() != device):
+        raise ValueError("window must be FP16[slots,channels,4] on the device of value")
+    pool = window.shape[0]
+    ws_s, ws_c, ws_t = window.stride()
+    if channels > 1 and ws_c != 1 or ws_t < channels or pool > 1 and ws_s < 3 * ws_t + channels:
+        raise ValueError("window must have its channels next to each other and none twice (allocate_windows)")
+    if slots is None and pool < batch:
         raise ValueError("A window for every batch row, or slots, required")
     for name, t in (("lengths", lengths), ("slots", slots)):
-        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (batch,)
-                              or t.device != value.device):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != rows
+                              or t.get_device() != device):
             raise ValueError(f"{name} must be int32[batch] on the device of value")
     if channels > 1 and value.stride(2) != 1:
         value = value.contiguous()
-    weight = weight.contiguous()
-    if weight.data_ptr() % 8:
-        weight = weight.clone()
-    bias = bias.contiguous() if bias is not None else None
+    if not weight.is_contiguous() or weight.data_ptr() % 8:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     lengths = lengths.contiguous() if lengths is not None else None
     slots = slots.contiguous() if slots is not None else None
-    parts = [value.new_empty((batch, tokens, n)) for n in sizes]
+    x, b, c = (value.new_empty((batch, tokens, n)) for n in sizes)
+    vs_b, vs_l, _ = value.stride()
     p = _native.ptr
     with _native.device_of(value):
-        _native.call("m2r_conv_pool", p(window), window.shape[0], window.stride(0), window.stride(2), p(value),
-                     value.stride(0), value.stride(1), p(weight), p(bias), p(slots), p(lengths), *map(p, parts), *sizes,
-                     batch, tokens, 4, 1 if silu else 0, _native.stream_of(value))
-    return parts
+        _native.call("m2r_conv_pool", window.data_ptr(), pool, ws_s, ws_t, value.data_ptr(), vs_b, vs_l, weight.data_ptr(),
+                     p(bias), p(slots), p(lengths), x.data_ptr(), b.data_ptr(), c.data_ptr(), *sizes, batch, tokens, 4,
+                     1 if silu else 0, _native.stream_of(value))
+    return [x, b, c]
 
 
 class FullState(_MixerController):

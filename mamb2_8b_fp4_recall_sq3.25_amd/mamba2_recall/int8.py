@@ -64,7 +64,8 @@ class Int8Weight:
 
     @classmethod
     def quantize(cls, weight):
-        """FP16 or BF16 weights [N,K], each channel by its largest value."""
+        """FP16 or BF16 weights [N,K], each channel by its largest value.  A
+        channel with a value that is not finite has the scale NaN."""
         if (not isinstance(weight, torch.Tensor) or weight.dtype not in (torch.float16, torch.bfloat16)
                 or weight.ndim != 2 or not weight.is_cuda):
             raise ValueError("weight must be CUDA FP16 or BF16 [N,K]")

@@ -595,8 +595,9 @@ class _MixerController:
         (int8.linear), prompts and single tokens, any batch.  `weights[i]` is a
         dict of int8.Int8Weight under in_proj and out_proj (either may be
         missing) for layer i, or None to keep that layer on its modules;
-        `weights=None` turns the mode off.  Where packed projections are
-        registered as well, they keep the one-token calls that they take."""
+        `weights=None` turns the mode off.  The projections' modules, and hooks
+        on them, do not run then.  Where packed projections are registered as
+        well, they keep the one-token calls that they take."""
         if weights is None:
             self._int8 = None
             return self

@@ -1,4 +1,5 @@
-"""Runs of the cases of perf/operators.py through the framework's kernels.
+"""Runs of the cases of perf/operators.py and perf/more_operators.py through the
+framework's kernels.
 
   python perf/operator_times.py loop CASE PASSES
       passes on one state, for a profiler to look at
@@ -13,29 +14,31 @@ import torch
 
 ROOT = Path(__file__).resolve().parents[1]
 sys.path.insert(0, str(ROOT))
-from perf import operators  # noqa: E402
+from perf import more_operators, operators  # noqa: E402
 
-operators.own = True
-CASES = {case["name"]: case for case in operators.listed()}
+operators.own = more_operators.own = True
+CASES = {case["name"]: (module, case) for module in (operators, more_operators) for case in module.listed()}
 
 
 def loop(name, passes):
-    state = operators.prepare(CASES[name], 1)
+    module, case = CASES[name]
+    state = module.prepare(case, 1)
     for _ in range(passes):
-        operators.run(state)
+        module.run(state)
     torch.cuda.synchronize()
 
 
 def graph(name):
     """(median, least) microseconds of a pass."""
-    states = [operators.prepare(CASES[name], seed) for seed in (1, 2, 3)]
+    module, case = CASES[name]
+    states = [module.prepare(case, seed) for seed in (1, 2, 3)]
     for state in states:
-        operators.run(state)
+        module.run(state)
     torch.cuda.synchronize()
     passes = torch.cuda.CUDAGraph()
     with torch.cuda.graph(passes):
         for k in range(30):
-            operators.run(states[k % 3])
+            module.run(states[k % 3])
     times = []
     for _ in range(15):
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)

@@ -259,3 +259,31 @@ def test_refusals(device):
         sampling.adjust(buffer[:2], out=buffer[1:])
     with pytest.raises(ValueError, match="apart"):
         sampling.adjust(buffer.flatten()[:128].view(2, 64), out=buffer.flatten()[8:136].view(2, 64))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,vocab,prompt,tokens,wide", [
+    (2, 30011, 9000, 40, True), (2, 9001, 0, 8192, False),      # long lists, few rows
+    (130, 333, 8150, 60, True), (64, 17001, 8192, 5, False),    # long lists, many rows
+    (300, 1000, 30, 20, True), (1, 5000, 4100, 0, True)])       # many rows; a list of some length
+def test_launch_shapes(device, dtype, batch, vocab, prompt, tokens, wide):
+    logits, kw = _case(device, dtype, batch, vocab, prompt, tokens, 6, 5, seed=batch + vocab, wide=wide)
+    _check(logits, **kw)
+
+
+def test_offsets_past_32_bits(device):
+    """More than 2^31 logits: the last rows are those of a small call."""
+    from mamba2_recall import sampling
+    gen = torch.Generator(device=device).manual_seed(11)
+    logits = torch.empty(8500, 256000, dtype=torch.float16, device=device).normal_(generator=gen)
+    tokens = torch.randint(0, 256000, (8500, 9), generator=gen, device=device)
+    masks = torch.full((1, 8000), -1, dtype=torch.int32, device=device)
+    masks[0, 7999] = 0
+    kw = dict(presence=0.5, frequency=0.25, repetition=1.1)
+    rows = torch.zeros(8500, dtype=torch.int32, device=device)
+    last = sampling.adjust(logits[-4:], tokens=tokens[-4:], allowed=masks, allowed_rows=rows[-4:], **kw)
+    got = sampling.adjust(logits, tokens=tokens, allowed=masks, allowed_rows=rows, **kw)
+    assert torch.equal(got[-4:], last) and bool((got[-1, -32:] == -INF).all())
+    del got
+    sampling.adjust(logits, tokens=tokens, allowed=masks, allowed_rows=rows, out=logits, **kw)
+    assert torch.equal(logits[-4:], last)

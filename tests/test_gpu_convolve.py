@@ -183,3 +183,17 @@ def test_long_row(device):
     tail[0].copy_(value[0, -30:-26].T)
     last = full_state.convolve(value[:, -26:], weight, None, tail, sizes)
     assert all(torch.equal(p[:, -26:], q) for p, q in zip(parts, last))
+
+
+@pytest.mark.parametrize("tokens", [97, 128, 131])
+def test_many_workgroups(device, tokens):
+    """Enough rows for 32 tokens a thread: whole and ragged runs, idle rows."""
+    sizes, batch = (64, 16, 16), 70
+    value, weight, bias, window = _inputs(device, batch, tokens, sizes, 80, seed=9, pad=32)
+    gen = torch.Generator(device=device).manual_seed(10)
+    slots = torch.randperm(80, generator=gen, device=device)[:batch].to(torch.int32)
+    slots[::17] = -1
+    lengths = torch.randint(0, tokens + 1, (batch,), generator=gen, device=device, dtype=torch.int32)
+    lengths[:6] = torch.tensor([tokens, 32, 33, 31, 64, 96], dtype=torch.int32, device=device)
+    _check(device, value, weight, bias, window, sizes, lengths, slots)
+    _check(device, value, weight, bias, window, sizes)

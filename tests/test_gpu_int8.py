@@ -269,3 +269,27 @@ def test_refusals(device):
     for bad in (x.float(), x[0], x.cpu(), x[:0]):
         with pytest.raises(ValueError):
             int8.Int8Weight.quantize(bad)
+
+
+def test_offsets_past_32_bits(device):
+    """More than 2^31 outputs, codes and weights: the last rows and channels are
+    those of small calls."""
+    from mamba2_recall import int8
+    gen = torch.Generator(device=device).manual_seed(17)
+    codes, scale, weight = _weight(device, 256000, 64, 18)
+    x = torch.randn(8500, 64, generator=gen, device=device).half()
+    y = int8.linear(x, weight)
+    assert torch.equal(y[-5:], int8.linear(x[-5:], weight)) and torch.equal(y[:5], int8.linear(x[:5], weight))
+    del y
+    _, _, weight = _weight(device, 40, 4096, 19)
+    x = torch.empty(600001, 4096, dtype=F16, device=device).normal_(generator=gen)
+    y = int8.linear(x, weight)
+    assert torch.equal(y[-70:], int8.linear(x[-70:], weight)) and torch.equal(y[:3], int8.linear(x[:3], weight))
+    del x, y
+    codes = torch.empty(600001, 4096, dtype=torch.int8, device=device).random_(-127, 128, generator=gen)
+    scale = torch.rand(600001, generator=gen, device=device) * 1e-4
+    weight, tail = int8.Int8Weight(codes, scale), int8.Int8Weight(codes[-33:], scale[-33:])
+    del codes
+    for m in (2, 30, 140):
+        x = _rows(device, m, 4096, F16, m)
+        assert torch.equal(int8.linear(x, weight)[:, -33:], int8.linear(x, tail))
