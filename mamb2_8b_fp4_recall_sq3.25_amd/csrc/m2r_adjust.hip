@@ -76,7 +76,7 @@ __device__ __forceinline__ typename LogitType<DTYPE>::T logit_rounded(float v) {
 __device__ __forceinline__ float row_value(const RowValue& v, int64_t row) { return v.row ? v.row[row] : v.all; }
 
 // Calls f(token of the slice) for each id of the row's list in [v0, v0 + size).
-// Sixteen bytes of ids a thread, four such loads at a time.
+// Sixteen bytes of ids a thread, kLoads such loads at a time.
 template <int THREADS, int kLoads, typename F>
 __device__ __forceinline__ void for_ids(const IdList& l, int64_t row, int64_t v0, int size, F f) {
   if (!l.ids) return;

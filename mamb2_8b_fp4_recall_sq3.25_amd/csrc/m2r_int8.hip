@@ -18,9 +18,9 @@
 //   1 row, 4,096 -> 18,560      15   5.1 TB/s: memory
 //   64 rows, 8,192 -> 4,096     15   2.4 TB/s: two launches, operands' way from L2
 //   24 rows, 4,096 -> 256,000  200   5.4 TB/s: memory
-//   901 rows, 8,192 -> 4,096    41   1.5 POP/s: a block of 128 x 128 a CU, which
-//                                    moves 64 KB through LDS for 512 clocks of products
-//   2,048 rows, 4,096 -> 18,560 147  2.1 POP/s: see tile_block
+//   901 rows, 8,192 -> 4,096    43   1.4 POP/s: a block of 128 x 128 a CU, whose
+//                                    operands come from L2 at half of what a CU can take
+//   2,048 rows, 4,096 -> 18,560 146  2.1 POP/s: see tile_block
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 #include "m2r_tile.h"
@@ -203,7 +203,7 @@ struct ProductArgs {
 
 // Eight sums of a row and eight channels, scaled and stored.  The scales'
 // product first: it is the same in either order, and while it is a normal
-// number the result is within two roundings of the formula.  Held as binary32
+// number of binary32 the result is within three roundings of the formula.  Held as binary32
 // before it is rounded to the output's type, in every kernel alike.
 struct Row8 { int v[8]; };
 template <int DTYPE, bool WIDE>
@@ -296,7 +296,9 @@ __device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory");
 // 1,700 (a tenth of that are operands that miss the L2).  8,192 cubed: 410 us, 2.7
 // POP/s.  Four waves with 128 x 128 outputs each (a quarter less LDS traffic, one
 // wave a SIMD), five stages, wave priorities and all reads in front of the
-// products were not faster; the stores at the end are 5 us a block.
+// products were not faster; the stores at the end are 5 us a block.  In the block
+// of 128 x 128, two groups of four waves with every other input tile each (a
+// quarter less LDS traffic) gained 3% and were left out.
 template <int DTYPE, bool WIDE, int BM, int BN, int WM, int WN, int STAGES, int KS, bool SPLIT = false>
 __device__ __forceinline__ void tile_block(const ProductArgs& a, uint8_t* lds, int m0, int n0, int k0, int k1, int split,
                                            uint32_t block, uint32_t* shared) {
