@@ -13,6 +13,9 @@ int m2r_check(hipError_t e, const char* what);
 // (0 = automatic), encoded as waves_per_block * 16 + heads_per_wave.
 int m2r_forced_step_shape();
 
+// Whether a launch of `blocks` workgroups stays below the runtime's 2^32 threads.
+inline bool m2r_grid_fits(int64_t blocks, int threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 // Lets a kernel have `bytes` of dynamic LDS, once on each device; `done` is the
 // kernel's own, a bit for each of the first 64 devices.
 inline int m2r_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(THREADS) void k_adjust(AdjustArgs a) {
 template <int DTYPE, int THREADS, int SLICE, int LOADS>
 static int adjust_launch(AdjustArgs& a, int64_t batch, hipStream_t stream) {
   const int64_t slices = (a.V + SLICE - 1) / SLICE;
-  if (slices > 0x7fffffff / batch) return m2r_fail("adjust: grid limits exceeded");
+  if (!m2r_grid_fits(slices * batch, THREADS)) return m2r_fail("adjust: grid limits exceeded");
   a.slices = (uint32_t)slices;
   const size_t lds = 4 * (size_t)SLICE * ((a.prompt.ids || a.tokens.ids) + (a.bias_ids != nullptr));
   static std::atomic<uint64_t> allowed{0};

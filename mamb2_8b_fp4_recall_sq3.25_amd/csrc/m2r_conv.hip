@@ -122,7 +122,8 @@ __global__ __launch_bounds__(256) void k_conv_pool(ConvArgs a) {
 template <int VEC, int TOKENS, int STEP>
 static int conv_launch(ConvArgs& a, hipStream_t stream) {
   const int64_t cb = (a.C + 256 * VEC - 1) / (256 * VEC), tb = (a.tokens + TOKENS - 1) / TOKENS;
-  if (cb * tb > 0x7fffffff / a.batch) return m2r_fail("conv pool: grid limits exceeded");
+  if (cb * tb > 0x7fffffff / a.batch || !m2r_grid_fits(cb * tb * a.batch, 256))
+    return m2r_fail("conv pool: grid limits exceeded");
   a.channel_blocks = (uint32_t)cb;
   a.token_blocks = (uint32_t)tb;
   hipLaunchKernelGGL((k_conv_pool<VEC, TOKENS, STEP>), dim3((unsigned)(cb * tb * a.batch)), dim3(256), 0, stream, a);

@@ -805,9 +805,10 @@ static bool whole_rows(const void* x, int64_t stride, int64_t K) {
   return !((uintptr_t)x & 15) && !(stride & 7) && !(K & 15);
 }
 
+// (k_int8_rows has 256 threads a row and whole 128s of rows.)
 static int int8_limits(int64_t rows, int64_t K) {
   if (rows <= 0 || K <= 0) return m2r_fail("int8: non-positive shape");
-  if (rows > (int64_t)1 << 24 || K > 131072) return m2r_fail("int8: size limits");
+  if (!m2r_grid_fits((rows + 127) / 128 * 128, 256) || K > 131072) return m2r_fail("int8: size limits");
   return 0;
 }
 
@@ -860,6 +861,7 @@ extern "C" int m2r_int8_linear(const void* x, int x_dtype, int64_t x_stride, con
   // wide: whole eights of channels, dword-aligned, stored by 16 bytes
   const bool whole = whole_rows(x, x_stride, K), wide = !(N & 7) && !(y_stride & 1) && !((uintptr_t)y & 3);
   const Plan p = int8_plan(M, N, K, whole);
+  if (!p.few && !m2r_grid_fits(p.grid, 512)) return m2r_fail("int8: grid limits exceeded");
   uint8_t* codes = (uint8_t*)workspace;
   float* scale = (float*)(codes + int8_codes_bytes(M, K));
   uint32_t* tickets = (uint32_t*)((uint8_t*)scale + up256(4 * M));

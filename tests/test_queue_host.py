@@ -156,3 +156,16 @@ def test_masks_and_lists_of_the_wrong_shape():
                          (torch.zeros(3, 4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))):
         with pytest.raises(ValueError):
             sampling._list(ids, lengths, "prompt", 3, -1)
+
+
+@pytest.mark.parametrize("name,args,text", [
+    ("m2r_int8_linear", _linear_args(M=1 << 24, K=16, xs=16, N=1, ys=1), "size limits"),
+    ("m2r_int8_linear", _linear_args(M=1 << 22, K=16, xs=16, N=1 << 18, ys=1 << 18, work_bytes=1 << 50), "grid limits"),
+    ("m2r_int8_quantize", [FAKE, 0, 16, FAKE, FAKE, (1 << 24) - 127, 16, None], "size limits"),
+    ("m2r_adjust_logits", _adjust_args(V=1, ls=1, os=1, batch=1 << 24), "grid limits"),
+    ("m2r_adjust_logits", _adjust_args(batch=1 << 23, tokens=FAKE, tn=8192), "grid limits"),
+    ("m2r_conv_pool", _conv_args(batch=8, pool=8, n_x=1, n_b=1, n_c=1, tokens=1 << 24), "grid limits"),
+    ("m2r_conv_pool", _conv_args(batch=1 << 24, pool=1 << 24, tokens=1), "grid limits")])
+def test_launches_of_2_to_the_32_threads_are_refused(name, args, text):
+    """A launch has fewer than 2^32 threads: calls that would need more are refused before it."""
+    _fails(name, args, text)
