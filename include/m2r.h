@@ -458,7 +458,8 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   operand); K at most 131,072; workspace: 16-byte aligned device memory of the bytes that
  *   m2r_int8_linear_workspace() names for this call (x is not read; null where that
  *   is 0), used on `stream` only.  Scales whose product
- *   is not a normal number of binary32 cost digits, or give NaN if it overflows.
+ *   is not a normal number of binary32 cost digits, or if it overflows give an
+ *   infinity (NaN for a sum of 0).
  */
 int64_t m2r_int8_weight_bytes(int64_t N, int64_t K);
 int m2r_int8_quantize(const void* w, int dtype, int64_t w_stride, void* tiles, float* scale, int64_t N, int64_t K,

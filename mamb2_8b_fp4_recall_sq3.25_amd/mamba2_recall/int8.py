@@ -112,8 +112,9 @@ def linear(x, weight, dtype=None):
 
     The sum of a row's products is exact, its product with the two scales is
     formed in FP32 and rounded once, so a row's result depends on the row
-    alone.  A row with a value that is not finite gives NaN, as do scales whose
-    product overflows FP32.  Forward only."""
+    alone.  A row with a value that is not finite gives NaN; two scales whose
+    product overflows FP32 give infinities, and NaN for a sum of 0.  Forward
+    only."""
     if not isinstance(weight, Int8Weight):
         raise ValueError("weight must be an Int8Weight")
     k, n = weight.features
