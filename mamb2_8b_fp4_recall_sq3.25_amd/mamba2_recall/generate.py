@@ -34,9 +34,9 @@ def generate(controller, lm_head, prompt, uniforms, *, lengths=None, temperature
     request.  `allowed` is the masks for all steps, or a function of the ids
     drawn so far, int64[batch,step], that gives the next step's, or None.
     `lengths` int32[batch] (a controller that takes it): the tokens of each
-    prompt, at least one; those behind them count for nothing.  The
-    controller's request is reset first and stands after the last token but
-    one."""
+    prompt, at least one; those behind them, of any value, count for nothing.
+    The controller's request is reset first and stands after the last token
+    but one."""
     if (not isinstance(uniforms, torch.Tensor) or uniforms.ndim != 2 or uniforms.dtype != torch.float32
             or uniforms.shape[1] < 1):
         raise ValueError("uniforms must be FP32[batch,new] with at least one new token")

@@ -433,8 +433,8 @@ class _MixerController:
         """model.backbone(ids) with every mixer going through this controller
         (state_quant.py:195-217): the request's caches are used and advanced.
         `lengths` int32[batch] (full_state.FullState): the tokens of each row
-        that count; a row's caches stand after its last, and the hidden rows
-        past it say nothing."""
+        that count; a row's caches stand after its last, the ids past it may
+        have any value, and the hidden rows there say nothing."""
         if not self._installed:
             raise RuntimeError("StateQuant controller is not installed")
         if not isinstance(ids, torch.Tensor) or ids.ndim != 2 or ids.shape[1] == 0:
@@ -451,6 +451,8 @@ class _MixerController:
             if (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
                     or tuple(lengths.shape) != (ids.shape[0],) or lengths.device != self.device):
                 raise ValueError("lengths must be int32[batch] on the model device")
+            # padding of any value, as one outside the vocabulary may not reach the embedding
+            ids = ids.masked_fill(torch.arange(ids.shape[1], device=ids.device) >= lengths[:, None], 0)
         if reset or self._request is None:
             self.reset(ids.shape[0])
         self._running, self._lengths = True, lengths

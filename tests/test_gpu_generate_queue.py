@@ -258,3 +258,24 @@ def test_example_runs(small, device, monkeypatch):  # noqa: F811
     new = names["new"]
     assert new.shape == names["logprobs"].shape == (BATCH, 4)
     assert bool(((new >= 0) & (new < VOCAB) & (new % 32 != 0)).all())
+
+
+@pytest.mark.parametrize("padding", [-1, VOCAB + 7, 1 << 40])
+def test_padding_of_any_value(small, device, padding):  # noqa: F811
+    """Prompts filled up with ids outside the vocabulary give what those filled up with tokens give."""
+    from mamba2_recall import generate
+    from mamba2_recall.full_state import FullState
+    prompt, gen = _prompts(device, 30, seed=8)
+    lengths = _int32(device, 30, 4, 17)
+    padded = prompt.clone()
+    for i, n in enumerate(lengths.tolist()):
+        padded[i, n:] = padding
+    uniforms = torch.rand(BATCH, 3, generator=gen, device=device)
+    head = torch.nn.functional.linear
+    weight = torch.randn(VOCAB, small.backbone.layers[0].mixer.in_proj.weight.shape[1], generator=gen, device=device).half()
+    with _few(FullState, small) as c:
+        def run(ids):
+            return generate.generate(c, lambda rows: head(rows, weight).float(), ids, uniforms, lengths=lengths,
+                                     repetition=1.2, presence=0.1)
+        (ids, logprobs), (same, same_logprobs) = run(prompt), run(padded)
+    assert torch.equal(ids, same) and torch.equal(logprobs, same_logprobs)

@@ -169,3 +169,22 @@ def test_masks_and_lists_of_the_wrong_shape():
 def test_launches_of_2_to_the_32_threads_are_refused(name, args, text):
     """A launch has fewer than 2^32 threads: calls that would need more are refused before it."""
     _fails(name, args, text)
+
+
+def test_padding_is_never_looked_up():
+    """Ids behind a row's length, of any value, do not reach the embedding: one
+    outside the vocabulary would end a process there."""
+    from types import SimpleNamespace
+    class OnHost(full_state.FullState):
+        device, _installed = torch.device("cpu"), True
+    c = OnHost.__new__(OnHost)
+    seen = []
+    c._running, c._adapters = False, None
+    c._request = SimpleNamespace(next_layer=0, failed=False)
+    c.model = SimpleNamespace(backbone=lambda ids: seen.append(ids) or torch.nn.functional.embedding(ids, torch.zeros(50, 8)))
+    ids = torch.tensor([[7, 8, 9, -1], [3, -1, -1, -1], [4, 5, 6, 7], [1 << 40, -100, 50, 99]])
+    given = ids.clone()
+    c.backbone(ids, lengths=torch.tensor([3, 1, 9, -2], dtype=torch.int32))
+    assert seen[0].tolist() == [[7, 8, 9, 0], [3, 0, 0, 0], [4, 5, 6, 7], [0, 0, 0, 0]] and torch.equal(ids, given)
+    c.backbone(ids[2:3])
+    assert seen[1].tolist() == [[4, 5, 6, 7]]
