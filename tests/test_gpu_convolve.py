@@ -197,3 +197,25 @@ def test_many_workgroups(device, tokens):
     lengths[:6] = torch.tensor([tokens, 32, 33, 31, 64, 96], dtype=torch.int32, device=device)
     _check(device, value, weight, bias, window, sizes, lengths, slots)
     _check(device, value, weight, bias, window, sizes)
+
+
+@pytest.mark.parametrize("sizes", [(64, 16, 16), (33, 6, 9)])
+@pytest.mark.parametrize("tokens", [1, 7, 45])
+def test_what_stands_behind_a_row_does_not_count(device, sizes, tokens):
+    """NaN and infinities behind the rows' lengths, in the windows of idle and empty rows and in the
+    window's first place reach nothing."""
+    counts = torch.tensor([tokens, tokens // 2, 1, 0, tokens], dtype=torch.int32, device=device)
+    slots = torch.tensor([0, 1, 2, 3, -1], dtype=torch.int32, device=device)
+    value, weight, bias, window = _inputs(device, 5, tokens, sizes, 5, seed=9)
+    dirty, windows = value.clone(), window.clone()
+    windows[:, :, 0] = float("nan")
+    windows[3:] = float("inf")
+    for i, n in enumerate((tokens, tokens // 2, 1, 0, 0)):
+        dirty[i, n:] = float("nan") if i % 2 else float("-inf")
+    want = _check(device, value, weight, bias, window, sizes, counts, slots)
+    from mamba2_recall import full_state
+    got = full_state.convolve(dirty, weight, bias, windows, sizes, lengths=counts, slots=slots)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    live = [i for i, n in enumerate(counts[:3].tolist()) if n]
+    # (a window of fewer than four tokens shifts: its first place goes)
+    assert torch.equal(windows[live], window[live]) and bool(torch.isinf(windows[3:]).all())
