@@ -200,19 +200,12 @@ def prepare(case, seed):
 
 
 # ---------------------------------------------------------------- the framework's calls
-_modules = {}
-
-
 def _package(name):
-    """A module of the framework, found once: a program imports what it calls
-    at its start, not in every pass."""
-    if name not in _modules:
-        root = str(Path(__file__).resolve().parents[1] / "mamb2_8b_fp4_recall_sq3.25_amd")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        import importlib
-        _modules[name] = importlib.import_module("mamba2_recall." + name)
-    return _modules[name]
+    root = str(Path(__file__).resolve().parents[1] / "mamb2_8b_fp4_recall_sq3.25_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import importlib
+    return importlib.import_module("mamba2_recall." + name)
 
 
 def _run_own(s):
