@@ -42,7 +42,8 @@ def generate(controller, lm_head, prompt, uniforms, *, lengths=None, temperature
         raise ValueError("uniforms must be FP32[batch,new] with at least one new token")
     if not isinstance(prompt, torch.Tensor) or prompt.ndim != 2 or prompt.shape[0] != uniforms.shape[0]:
         raise ValueError("prompt must be [batch,tokens] with a row for each row of uniforms")
-    # refused before the request is reset
+    # refused before the request is reset; what needs the vocabulary (the width of masks) and what a function of
+    # masks gives, when it meets the logits
     sampling.filters(uniforms, temperature, top_k, top_p, min_p)
     sampling.penalties(uniforms, repetition, presence, frequency)
     sampling.biases(uniforms, bias)
@@ -50,9 +51,13 @@ def generate(controller, lm_head, prompt, uniforms, *, lengths=None, temperature
     if lengths is not None and (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
                                 or tuple(lengths.shape) != (batch,) or lengths.device != uniforms.device):
         raise ValueError("lengths must be int32[batch] on the device of uniforms")
-    if allowed is not None and not callable(allowed) and not isinstance(allowed, torch.Tensor):
-        raise ValueError("allowed must be a tensor of masks or a function that gives them")
+    if not callable(allowed):
+        if allowed is not None and not isinstance(allowed, torch.Tensor):
+            raise ValueError("allowed must be a tensor of masks or a function that gives them")
+        sampling.masks(uniforms, None, allowed, None)
     counted = any(isinstance(v, torch.Tensor) or v != d for v, d in ((repetition, 1), (presence, 0), (frequency, 0)))
+    if counted:
+        sampling._list(prompt, lengths, "prompt", batch, uniforms.get_device())
     if lengths is None:
         last = controller.backbone(prompt, reset=True)[:, -1]
     else:

@@ -89,14 +89,16 @@ def biases(like, bias):
 
 def masks(like, vocab, allowed, allowed_rows):
     """(masks int32[masks,words], the row's mask int32[batch] or None), checked
-    for as many rows as `like` has, on its device."""
+    for as many rows as `like` has, on its device.  `vocab` None: not known
+    yet, any number of words passes."""
     if allowed is None:
         if allowed_rows is not None:
             raise ValueError("allowed_rows without allowed")
         return None, None
-    words, batch = (vocab + 31) // 32, like.shape[0]
+    words, batch = "words" if vocab is None else (vocab + 31) // 32, like.shape[0]
     if (not isinstance(allowed, torch.Tensor) or allowed.dtype is not torch.int32 or allowed.ndim not in (1, 2)
-            or allowed.shape[-1] != words or allowed.shape[0] < 1 or allowed.get_device() != like.get_device()):
+            or 0 in allowed.shape or vocab is not None and allowed.shape[-1] != words
+            or allowed.get_device() != like.get_device()):
         raise ValueError(f"allowed must be int32 [{words}] or [masks,{words}], a bit a token, on the logits' device")
     if allowed.ndim == 1:
         if allowed_rows is not None:
@@ -110,7 +112,7 @@ def masks(like, vocab, allowed, allowed_rows):
         raise ValueError("allowed_rows must be int32[batch] on the logits' device")
     elif batch > 1 and allowed_rows.stride(0) != 1:
         allowed_rows = allowed_rows.contiguous()
-    if words > 1 and allowed.stride(1) != 1:
+    if allowed.shape[1] > 1 and allowed.stride(1) != 1:
         allowed = allowed.contiguous()
     return allowed, allowed_rows
 
