@@ -215,11 +215,13 @@ class FullState(_MixerController):
     def _scan_layer(self, index, mx, x, dt, aa, bm, cm, entry):
         return scan(x, dt, aa, bm, cm, mx.D, mx.dt_bias, entry.state, lengths=self._lengths)
 
+    def _refuse_ragged(self):
+        if not all(_plain(mx.conv1d, nn.Conv1d) and _plain(mx.act, nn.SiLU) for mx in self._mixers):
+            raise ValueError("Rows of different lengths need a plain nn.Conv1d and nn.SiLU, without hooks")
+
     def _conv_prefill(self, mx, xbc, layer):
         if self._lengths is None:
             return super()._conv_prefill(mx, xbc, layer)
-        if not (_plain(mx.conv1d, nn.Conv1d) and _plain(mx.act, nn.SiLU)):
-            raise ValueError("Rows of different lengths need a plain nn.Conv1d and nn.SiLU, without hooks")
         return convolve(xbc, mx.conv1d.weight[:, 0, :], mx.conv1d.bias, layer.conv, self._conv_sizes,
                         lengths=self._lengths)
 

@@ -252,6 +252,7 @@ class _MixerController:
     native_norm = True
     # whether backbone() takes prompts of different lengths
     ragged = False
+    _mixers = ()              # of the model, from __init__
     PARAMETER_TENSORS, PARAMETER_COUNT = 507, 8_236_999_680
     TABLE_SHAPE = (56, 8, 128)
 
@@ -428,6 +429,10 @@ class _MixerController:
     def _after_reset(self, batch_size):
         pass
 
+    def _refuse_ragged(self):
+        """Raises ValueError where the modules do not allow rows of different
+        lengths; the request has not been touched then."""
+
     @torch.no_grad()
     def backbone(self, ids, reset=False, lengths=None):
         """model.backbone(ids) with every mixer going through this controller
@@ -451,6 +456,7 @@ class _MixerController:
             if (not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32
                     or tuple(lengths.shape) != (ids.shape[0],) or lengths.device != self.device):
                 raise ValueError("lengths must be int32[batch] on the model device")
+            self._refuse_ragged()
             # padding of any value, as one outside the vocabulary may not reach the embedding
             ids = ids.masked_fill(torch.arange(ids.shape[1], device=ids.device) >= lengths[:, None], 0)
         if reset or self._request is None:
