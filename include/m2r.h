@@ -446,8 +446,8 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   y_mn = (sum_k q_mk w_nk) s_m t_n, the sum exact, the rest binary32, rounded
  *   once.  A row with a non-finite value gives NaN, a row of zeros zeros.  The
  *   reference keeps decoded FP16 weights (mamba2_recall/fp4_checkpoint.py:345-405).
- * m2r_int8_quantize writes weights (N rows of K, dtype 0 binary16, 1 bfloat16;
- * w_stride in elements) as codes and scales f32[N].
+ * m2r_int8_quantize writes weights (N rows of K, N at most 16,777,088; dtype 0
+ * binary16, 1 bfloat16; w_stride in elements) as codes and scales f32[N].
  *   tiles: i8, 16-byte aligned, m2r_int8_weight_bytes(N, K) bytes: tiles of 16
  *   channels by 64 inputs, those of one row of tiles after each other, K filled up
  *   with zeros to a multiple of 128 and N to one of 32 (the bytes of channels past
@@ -455,7 +455,7 @@ int64_t m2r_sample_call_workspace(int64_t batch, int64_t V, int per_row, float t
  *   row 2 a + t, and byte 256 c + 16 r + i of a tile is row r, input 16 c + i.
  * m2r_int8_linear: x rows of K (x_dtype as above, element row stride), y rows of N
  *   (y_dtype 2 binary32, too; element row stride of at most 2^25; no memory of an
- *   operand); K at most 131,072; workspace: 16-byte aligned device memory of the bytes that
+ *   operand); M at most 16,777,088, N 2^24, K 131,072; workspace: 16-byte aligned device memory of the bytes that
  *   m2r_int8_linear_workspace() names for this call (x is not read; null where that
  *   is 0), used on `stream` only.  Scales whose product
  *   is not a normal number of binary32 cost digits, or if it overflows give an

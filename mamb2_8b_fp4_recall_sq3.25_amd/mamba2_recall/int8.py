@@ -30,6 +30,8 @@ import torch
 from . import _native
 
 MAX_INPUTS = 131072          # sums of that many products fit 32 bits
+MAX_CHANNELS = 1 << 24       # of a product
+MAX_QUANTIZED = MAX_CHANNELS - 128   # channels whose codes one launch forms: 256 threads each, fewer than 2^32
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -41,18 +43,23 @@ def _groups(n, k):
     return (n + 31) // 32, (k + 127) // 128 * 2
 
 
+def _geometry(shape, channels):
+    n, k = shape
+    if min(n, k) < 1 or k > MAX_INPUTS or n > channels:
+        raise ValueError(f"Positive geometry, at most {MAX_INPUTS} inputs and {channels} channels required")
+    return n, k
+
+
 class Int8Weight:
-    """The weights of one projection: `codes` int8[N,K] and `scale` FP32[N],
-    the value of a weight being its code times its channel's scale.  Kept in
-    the order in which the kernels read them; call it, or `linear`, with rows
-    of K."""
+    """The weights of one projection: `codes` int8[N,K] and `scale` FP32[N] (N
+    at most 2^24, K at most 131,072), the value of a weight being its code times
+    its channel's scale.  Kept in the order in which the kernels read them; call
+    it, or `linear`, with rows of K."""
 
     def __init__(self, codes, scale):
         if not isinstance(codes, torch.Tensor) or codes.dtype != torch.int8 or codes.ndim != 2 or not codes.is_cuda:
             raise ValueError("codes must be CUDA int8[N,K]")
-        n, k = codes.shape
-        if min(n, k) < 1 or k > MAX_INPUTS:
-            raise ValueError(f"Positive geometry and at most {MAX_INPUTS} inputs required")
+        n, k = _geometry(codes.shape, MAX_CHANNELS)
         if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (n,)
                 or scale.device != codes.device):
             raise ValueError("scale must be FP32[N] on the device of codes")
@@ -64,14 +71,13 @@ class Int8Weight:
 
     @classmethod
     def quantize(cls, weight):
-        """FP16 or BF16 weights [N,K], each channel by its largest value.  A
-        channel with a value that is not finite has the scale NaN."""
+        """FP16 or BF16 weights [N,K] (N at most 16,777,088), each channel by
+        its largest value.  A channel with a value that is not finite has the
+        scale NaN."""
         if (not isinstance(weight, torch.Tensor) or weight.dtype not in (torch.float16, torch.bfloat16)
                 or weight.ndim != 2 or not weight.is_cuda):
             raise ValueError("weight must be CUDA FP16 or BF16 [N,K]")
-        n, k = weight.shape
-        if min(n, k) < 1 or k > MAX_INPUTS:
-            raise ValueError(f"Positive geometry and at most {MAX_INPUTS} inputs required")
+        n, k = _geometry(weight.shape, MAX_QUANTIZED)
         self = cls.__new__(cls)
         self.features = k, n
         weight, stride = _rows(weight.detach(), k)
