@@ -233,7 +233,9 @@ class FullState(_MixerController):
         return True
 
     def cache_breakdown(self):
-        """Bytes the request holds per kind of tensor."""
+        """Bytes the request holds per kind of tensor, and the places of a row
+        that each layer was called with: the padding of rows of different
+        lengths counts, as the rows' own tokens are known to the device only."""
         layers = self._cache
         conv = sum(c.conv.numel() * c.conv.element_size() for c in layers)
         state = sum(c.state.numel() * c.state.element_size() for c in layers)

@@ -439,7 +439,8 @@ class _MixerController:
         (state_quant.py:195-217): the request's caches are used and advanced.
         `lengths` int32[batch] (full_state.FullState): the tokens of each row
         that count; a row's caches stand after its last, the ids past it may
-        have any value, and the hidden rows there say nothing."""
+        have any value, and the hidden rows there say nothing.  (The tokens that
+        cache_breakdown() names are places of a row, padding among them.)"""
         if not self._installed:
             raise RuntimeError("StateQuant controller is not installed")
         if not isinstance(ids, torch.Tensor) or ids.ndim != 2 or ids.shape[1] == 0:
