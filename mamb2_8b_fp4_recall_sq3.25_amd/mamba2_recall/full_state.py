@@ -148,7 +148,7 @@ def convolve(value, weight, bias, window, sizes, *, lengths=None, slots=None, si
     three precede its tokens; zeros for a new request.  `slots` and `lengths`
     are scan's: outputs past a row's length, and an idle row's, are zero, and an
     idle or empty row leaves its window alone.  The sum and the SiLU are formed
-    in FP32 and rounded once."""
+    in FP32 and rounded once.  Forward only."""
     if not isinstance(value, torch.Tensor) or value.dtype != torch.float16 or value.ndim != 3 or not value.is_cuda:
         raise ValueError("value must be CUDA FP16[batch,tokens,channels]")
     batch, tokens, channels = value.shape

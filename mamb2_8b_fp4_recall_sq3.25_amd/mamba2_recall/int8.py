@@ -67,7 +67,7 @@ class Int8Weight:
         filled = torch.nn.functional.pad(codes, (0, 64 * steps - k, 0, 32 * groups - n))
         self.features = k, n
         self.tiles = filled.view(groups, 4, 2, 4, steps, 4, 16).permute(0, 2, 4, 5, 1, 3, 6).contiguous()
-        self.scale = scale.clone(memory_format=torch.contiguous_format)
+        self.scale = scale.detach().clone(memory_format=torch.contiguous_format)
 
     @classmethod
     def quantize(cls, weight):

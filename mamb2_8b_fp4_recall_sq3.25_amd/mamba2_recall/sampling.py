@@ -147,7 +147,7 @@ def adjust(logits, *, prompt=None, prompt_lengths=None, tokens=None, lengths=Non
 
     repetition (above 0), presence and frequency are numbers, or FP32[B].  A
     logit that nothing touches keeps its bits, and the others are rounded once
-    to their type."""
+    to their type.  Forward only."""
     if not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError("logits must be CUDA FP16, BF16 or FP32 [batch,vocabulary]")
     batch, vocab = logits.shape
