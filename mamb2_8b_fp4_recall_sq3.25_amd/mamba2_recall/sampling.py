@@ -126,7 +126,7 @@ def adjust(logits, *, prompt=None, prompt_lengths=None, tokens=None, lengths=Non
            frequency=0.0, bias=None, allowed=None, allowed_rows=None, out=None):
     """Logits with each request's penalties, biases and grammar mask: a new
     tensor of their type and shape, or `out` (`logits` itself, or memory apart
-    from them).
+    from them: no rows of one between rows of the other).
 
     logits[B,V] in FP16, BF16 or FP32 (unit column stride).  `prompt` and
     `tokens` (int64 or int32 [B,n], unit column stride) are the ids that a
