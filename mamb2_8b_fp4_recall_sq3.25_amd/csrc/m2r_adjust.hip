@@ -20,8 +20,6 @@
 #include "m2r_device.h"
 #include "m2r_abi_util.h"
 
-#include <initializer_list>
-
 namespace m2r {
 
 struct IdList {
