@@ -3,9 +3,10 @@ framework's kernels.
 
   python perf/operator_times.py loop CASE PASSES
       passes on one state, for a profiler to look at
-  python perf/operator_times.py graph [CASE ...]
-      time of a pass among 30 captured into one graph, three sets of inputs in
-      turn: median and least of 15 replays (all cases by default)
+  python perf/operator_times.py graph [CASE[:SETS] ...]
+      time of a pass among 30 captured into one graph, SETS sets of inputs in
+      turn (three by default; more where three stay in the last-level cache):
+      median and least of 15 replays (all cases by default)
 """
 import sys
 from pathlib import Path
@@ -28,17 +29,17 @@ def loop(name, passes):
     torch.cuda.synchronize()
 
 
-def graph(name):
+def graph(name, sets=3):
     """(median, least) microseconds of a pass."""
     module, case = CASES[name]
-    states = [module.prepare(case, seed) for seed in (1, 2, 3)]
+    states = [module.prepare(case, 1 + seed) for seed in range(sets)]
     for state in states:
         module.run(state)
     torch.cuda.synchronize()
     passes = torch.cuda.CUDAGraph()
     with torch.cuda.graph(passes):
         for k in range(30):
-            module.run(states[k % 3])
+            module.run(states[k % sets])
     times = []
     for _ in range(15):
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -51,11 +52,18 @@ def graph(name):
     return times[7], times[0]
 
 
+def _asked(text):
+    """(case, sets) of CASE or CASE:SETS, or None."""
+    name, _, sets = text.partition(":")
+    if name in CASES and (not sets or sets.isdigit() and 0 < int(sets) <= 30):
+        return name, int(sets or 3)
+
+
 if __name__ == "__main__":
     if len(sys.argv) == 4 and sys.argv[1] == "loop" and sys.argv[2] in CASES:
         loop(sys.argv[2], int(sys.argv[3]))
-    elif len(sys.argv) > 1 and sys.argv[1] == "graph" and all(a in CASES for a in sys.argv[2:]):
-        for name in sys.argv[2:] or CASES:
-            print("%-20s median %7.2f us  least %7.2f us" % ((name,) + graph(name)), flush=True)
+    elif len(sys.argv) > 1 and sys.argv[1] == "graph" and all(_asked(a) for a in sys.argv[2:]):
+        for asked in sys.argv[2:] or CASES:
+            print("%-20s median %7.2f us  least %7.2f us" % ((asked,) + graph(*_asked(asked))), flush=True)
     else:
         sys.exit(__doc__)
