@@ -232,11 +232,11 @@ static int adjust_launch(AdjustArgs& a, int64_t batch, hipStream_t stream) {
 }
 template <int DTYPE>
 static int adjust_dtype(AdjustArgs& a, int64_t batch, hipStream_t stream) {
-  // Threads and slice by the lists' length and the number of workgroups.  us, 256 x 1,024 / 512 x 4,096 /
-  // 1,024 x 4,096 / 1,024 x 16,384:
-  //   1 row of 256,000, 1,000 ids     4.4 / 4.4 / 4.9 / 6.5      64 such rows (binary32)     28 / 26 / 45 / 31
-  //   1 row, 50,000 ids                20 / 13 / 9.7 / 12        64 rows, 16,000 ids         98 / 46 / 73 / 45
-  //   16 rows of 256,000, 8,000 ids    19 / 12 / 17 / 12         64 rows, 50,000 ids        289 / 104 / 137 / 67
+  // Threads and slice by the lists' length and the number of workgroups.  us on binary32, 256 x 1,024 /
+  // 512 x 4,096 / 1,024 x 4,096 / 1,024 x 16,384:
+  //   1 row of 256,000, 1,000 ids     3.7 / 4.5 / 4.1 / 6.4      64 such rows                31 / 28 / 45 / 31
+  //   1 row, 50,000 ids                19 / 13 / 8.8 / 12        64 rows, 16,000 ids        100 / 47 / 73 / 46
+  //   16 rows of 256,000, 8,000 ids    19 / 12 / 17 / 12         64 rows, 50,000 ids        288 / 104 / 137 / 67
   const int64_t ids = a.prompt.n + a.tokens.n;
   if (ids >= 8192) {
     if (batch * ((a.V + 16383) / 16384) >= 128) return adjust_launch<DTYPE, 1024, 16384, 4>(a, batch, stream);

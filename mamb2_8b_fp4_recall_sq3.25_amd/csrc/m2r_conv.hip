@@ -163,8 +163,8 @@ extern "C" int m2r_conv_pool(void* window, int64_t pool, int64_t ws_s, int64_t w
   if (tokens == 1) return wide ? conv_launch<8, 1, 1>(a, stream) : conv_launch<1, 1, 1>(a, stream);
   if (!wide) return conv_launch<1, 8, 8>(a, stream);
   // 32 tokens a thread once that leaves a workgroup a CU.  us with 8 a thread (11 loads for 8 outputs) / 32, 10,240
-  // channels: 8,192 tokens of one row 100 / 76, 1,000 of three 40 / 30, 128 of 16 28 / 24, 200 of four 14 / 16, 500 of
-  // one 12 / 15, 77 of one 6 / 13
+  // channels: 8,192 tokens of one row 101 / 76, 1,000 of three 39 / 30, 128 of 16 27 / 24, 200 of four 14 / 16, 500 of
+  // one 11 / 15, 77 of one 6 / 13
   const int64_t blocks = (C + 2047) / 2048 * batch * ((tokens + 31) / 32);
   return blocks >= 256 ? conv_launch<8, 32, 8>(a, stream) : conv_launch<8, 8, 8>(a, stream);
 }

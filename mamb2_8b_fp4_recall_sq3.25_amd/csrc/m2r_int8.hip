@@ -13,10 +13,11 @@
 // lane that holds rows 4 g ... + 3 of both products holds channels 8 g ... + 7.
 //
 // One launch forms the rows' codes, one multiplies; up to four rows have both in
-// one.  Times in a graph of calls (us; a large copy has 5.0 TB/s, a library
-// product of 8,192 cubed in these types 2.2 POP/s):
-//   1 row, 4,096 -> 18,560      15   5.1 TB/s: memory
-//   64 rows, 8,192 -> 4,096     15   2.4 TB/s: two launches, operands' way from L2
+// one.  Times in a graph of calls (us; reads alone reach 7.0 TB/s, a large copy
+// 5.0, a library product of 8,192 cubed in these types 2.2 POP/s):
+//   1 row, 4,096 -> 18,560      18   4.3 TB/s: memory, a launch's start and end (15 where the
+//                                    weights are in the last-level cache)
+//   64 rows, 8,192 -> 4,096     20   1.8 TB/s: two launches, operands' way from L2 (15 likewise)
 //   24 rows, 4,096 -> 256,000  200   5.4 TB/s: memory
 //   901 rows, 8,192 -> 4,096    43   1.4 POP/s: a block of 128 x 128 a CU, whose
 //                                    operands come from L2 at half of what a CU can take
@@ -294,7 +295,7 @@ __device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory");
 // A large block's input tile is 1,024 clocks of products a SIMD and 128 KB of LDS
 // traffic, about as many clocks; alone it takes 1,250, with all CUs at it up to
 // 1,700 (a tenth of that are operands that miss the L2).  8,192 cubed: 410 us, 2.7
-// POP/s.  Four waves with 128 x 128 outputs each (a quarter less LDS traffic, one
+// POP/s (450 with the codes' launch).  Four waves with 128 x 128 outputs each (a quarter less LDS traffic, one
 // wave a SIMD), five stages, wave priorities and all reads in front of the
 // products were not faster; the stores at the end are 5 us a block.  In the block
 // of 128 x 128, two groups of four waves with every other input tile each (a
@@ -672,10 +673,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) void k_int8_few(Pro
 }
 
 // ---------------------------------------------------------------- which kernel
-// Rows up to which k_int8_few is taken: 64 rows, 4,096 -> 18,560 24 us, 65 in blocks
-// of 128 x 128 21 (23 at 128 rows, where k_int8_few takes 42).  Where these blocks
-// are few, twice the rows: 128 rows, 8,192 -> 4,096 17.6 us against 20.5 with the
-// inputs of 32 blocks split in four.
+// Rows up to which k_int8_few is taken: 32 rows, 4,096 -> 18,560 20 us, 64 rows 24
+// and 21 in blocks of 128 x 128, 65 rows 30 and 20, 128 rows 33 and 21: for so many
+// channels the border could lie somewhat lower.  Where these blocks are few, twice
+// the rows: 128 rows, 8,192 -> 4,096 17.5 us against 20.6 with the inputs of 32
+// blocks split in four.
 constexpr int64_t kFewRows = 64;
 
 struct Plan {
@@ -696,8 +698,8 @@ static Plan int8_plan(int64_t M, int64_t N, int64_t K, bool whole) {
   if (M <= kFewRows || (M <= 2 * kFewRows && pairs < 256)) {
     p.few = MT == 1 ? 1 : (MT == 2 ? 2 : (MT <= 4 ? 4 : 8));
     if (M <= 4 && K <= kFusedInputs && whole) p.fused = M <= 2 ? (int)M : 4;
-    // us by shape 0 / 1 / 2: 24 rows, 4,096 -> 256,000 197 / 220 / 249; 32 rows, 4,096 -> 18,560 22 / 20 / 22; 16 rows,
-    // 8,192 -> 4,096 13.6 / 13.6 / 12.7, 64 rows 16.2 / 16.6 / 14.8
+    // us by shape 0 / 1 / 2: 24 rows, 4,096 -> 256,000 200 / 220 / 275; 32 rows, 4,096 -> 18,560 23 / 20 / 23; 16 rows,
+    // 8,192 -> 4,096 14.0 / 12.5 / 12.4, 64 rows 18.1 / 16.7 / 14.6
     p.shape = p.fused ? 1 : (pairs < 256 ? 2 : (pairs < 2048 ? 1 : 0));
     p.grid = (uint32_t)(p.shape ? pairs : (NT + 3) / 4);
     if (p.shape == 2) {
@@ -716,15 +718,16 @@ static Plan int8_plan(int64_t M, int64_t N, int64_t K, bool whole) {
   const int64_t rs = (MT + 7) / 8, cs = (NT + 7) / 8, small = rs * cs;
   // Rounds of 256 workgroups, in large blocks: the last round's blocks whole, in
   // halves, in quarters, or everything in blocks of a quarter's size.  A round of
-  // 4,096 inputs takes 45 us, 31 in halves, 19 in quarters.  2,048 rows, 4,096 ->
-  // 18,560: 155 us whole, 147 with the last 72 of 584 in halves; 512 rows 47 whole,
-  // 60 in quarters.
+  // 4,096 inputs takes 45 us, 31 in halves, 19 in quarters (68, 43 and 30 with the
+  // codes' launch and the call's start and end).  2,048 rows, 4,096 -> 18,560: 164 us
+  // whole, 151 with the last 72 of 584 in halves, 155 in quarters; 512 rows 51 whole,
+  // 61 in halves or quarters.
   const double full = (double)(all / 256), rounds[4] = {full + (rest ? 1 : 0), full + 0.62 * ((2 * rest + 255) / 256),
                                                         full + 0.42 * ((4 * rest + 255) / 256),
                                                         0.42 * ((small + 255) / 256)};
   for (int i = 1; i < 4; ++i)
     if (rounds[i] < rounds[p.part]) p.part = i;
-  if (2 * small <= 256) p.part = 3;       // and split inputs: 192 rows, 8,192 -> 4,096 33 us unsplit, 23 in four
+  if (2 * small <= 256) p.part = 3;       // and split inputs: 192 rows, 8,192 -> 4,096 32 us unsplit, 23 in four
   p.rb = (uint32_t)(p.part == 3 ? rs : rb);
   p.cb = (uint32_t)(p.part == 3 ? cs : cb);
   p.whole = (uint32_t)(p.part == 0 ? all : (p.part == 3 ? 0 : all - rest));
